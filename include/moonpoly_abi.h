@@ -67,6 +67,33 @@ int mp_linear(int dtype, int M, int N, int K, const void* X, const void* W, void
  * added in the output type -- bit-identical to the two-step `linear` followed by `+ bias`.  bias may be NULL. */
 int mp_linear_bias(int dtype, int M, int N, int K, const void* X, const void* W, const void* bias, void* Y, void* stream);
 
+/* Linear with softmax cross entropy (no counterpart in the reference): the output layer of a language model and its
+ * loss, without holding the logits.  z[M,V] = X[M,H] * W[V,H]^T with fp32 accumulation; for every row
+ *   lse[m]  = log(sum over v of exp(z[m,v]))
+ *   loss[m] = lse[m] - z[m, target[m]],   0 where target[m] == ignore_index,   NaN where target[m] is neither
+ *             ignore_index nor in [0, V).
+ * dtype: MP_FP16 or MP_BF16 (X and W); loss, lse: M floats.  X and W are row-major with row strides ldx, ldw >= H in
+ * elements.  target: target_bytes = 4 (int32) or 8 (int64).  Operands whose rows are not 16-byte aligned are copied into
+ * the workspace once per call.  M = 0 computes nothing. */
+int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx, const void* W, long long ldw, const void* target,
+                   int target_bytes, long long ignore_index, float* loss, float* lse, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* Its gradients, for the gradient grad_loss[M] (fp32) of a scalar with respect to loss:
+ *   d[m,v] = grad_loss[m] * (exp(z[m,v] - lse[m]) - (v == target[m])),   0 in rows whose target is ignore_index
+ *   dX[M,H] = d * W,   dW[V,H] = d^T * X          (packed rows, the type of X and W)
+ * lse is what mp_linear_xent returned for the same operands.  dX or dW may be NULL.  grad_loss is not read for ignored
+ * rows' results.  A target out of range gives NaN gradients.  dW is overwritten, not accumulated. */
+int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long ldx, const void* W, long long ldw,
+                        const void* target, int target_bytes, long long ignore_index, const float* lse, const float* grad_loss,
+                        void* dX, void* dW, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that mp_linear_xent (backward = 0) or mp_linear_xent_grad (1) needs for these operands (X and W are
+ * only looked at for their alignment).  The workspace is 256-byte aligned device memory, needs no initialisation, and
+ * must not be shared by calls, or replays of captured graphs, that can overlap. */
+int mp_linear_xent_workspace(int dtype, int M, int V, int H, const void* X, long long ldx, const void* W, long long ldw,
+                             int backward, size_t* bytes);
+
 /* run_moonpoly_gemm_{fp16,fp32,int8}_row_col_col (core/fp16/fp16_rcc.cu:3263-3269,
  * core/fp32/fp32_rcc.cu:2272-2282, core/int8/i8_rcc.cu:3143-3157): online selector, then the
  * chosen pattern/pid in one launch. */

@@ -13,6 +13,7 @@
 
 #include "../../include/moonpoly_abi.h"
 #include "mp_gemv.cuh"
+#include "mp_host.h"
 #include "mp_stream_mma.cuh"
 #include "mp_select.h"
 #include "mp_simt_gemm.cuh"
@@ -1090,6 +1091,66 @@ int run_twin(const Problem& p, int split_n, cudaStream_t stream) {
 }
 
 }  // namespace
+
+// ================================================================================================
+// what the other translation units of the library share with this one (mp_host.h)
+// ================================================================================================
+namespace mp {
+
+int host_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+void host_count_launches(int n) { g_launches.fetch_add((unsigned long long)n, std::memory_order_relaxed); }
+
+bool host_use_pdl() { return g_use_pdl; }
+
+int host_device(HostDevice* out) {
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  int dev = 0;
+  MP_CUDA_TRY(cudaGetDevice(&dev));
+  static std::atomic<int*> status[kMaxDevices] = {};
+  int* p = status[dev].load(std::memory_order_acquire);
+  if (p == nullptr) {
+    MP_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_mp_status));
+    status[dev].store(p, std::memory_order_release);
+  }
+  out->index = dev;
+  out->sms = d->sms;
+  out->status = p;
+  return MP_OK;
+}
+
+int host_tmap(CUtensorMap* tm, int type, const void* ptr, long long inner, long long rows, long long row_bytes, int box_inner,
+              int box_rows, int swizzle) {
+  const cuuint64_t gdim[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+  const cuuint64_t gstride[1] = {(cuuint64_t)row_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapSwizzle sw = swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
+  const CUresult r = g_encode(tm, type == kTmap16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
+                              const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MP_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return MP_OK;
+}
+
+int host_pad_rows16(const void* src, long long ld, void* dst, int rows, int k, int kp, cudaStream_t stream) {
+  const long long words = (long long)rows * (kp / 8);
+  const int grid = (int)std::min<long long>((words + 255) / 256, 148 * 16);
+  pad_rows_kernel<uint16_t><<<grid, 256, 0, stream>>>(reinterpret_cast<const uint16_t*>(src), ld, reinterpret_cast<uint16_t*>(dst),
+                                                      rows, k, kp);
+  MP_CUDA_TRY(cudaGetLastError());
+  host_count_launches(1);
+  return MP_OK;
+}
+
+}  // namespace mp
 
 // ================================================================================================
 // exported entry points

@@ -1,0 +1,440 @@
+// Persistent tcgen05 GEMM on CTA pairs (cta_group::2):   D[rows x cols] = A * B^T over a common contraction index.
+//
+// A pair of CTAs (a cluster of two) owns a 256 x bn tile: CTA r of the pair holds rows 128 r ... 128 r + 127 of the tile
+// in its TMEM, loads its own 128 rows of A and its own half of the bn rows of B, and the tensor cores of both SMs read
+// both halves of B.  Per 64 contraction elements a CTA thus ingests 16 KB + bn / 2 * 128 bytes for 128 * bn * 64 FMAs --
+// the operand traffic of a 256 x bn single-CTA tile -- while a tile's accumulator needs only bn TMEM columns, so two
+// accumulators fit and the drain of one tile overlaps the main loop of the next.
+//
+// Either operand may be stored with the contraction index contiguous ("K-major", as the RCC contract gives) or with its
+// own row index contiguous ("MN-major": what the gradients need, dX = dY * W and dW = dY^T * X read W, dY and X as they
+// lie, without transposed copies).  Both forms are TMA boxes of 128 contiguous bytes per line, 128-byte swizzled.
+//
+// Roles per CTA: warp 0 = TMA producer, warp 1 = MMA issuer (rank 0 of the pair only) and TMEM owner, warps 2..9 =
+// epilogue (TMEM lane quadrant = warp % 4, two warps per quadrant taking the two halves of the columns).
+// Barriers: full[s] lives in rank 0 and counts the bytes of both CTAs; empty[s] and tfull[b] exist in both CTAs and are
+// signalled by multicast commits; tempty[b] lives in rank 0 and takes the arrivals of the 16 epilogue warps of the pair.
+// No TMA load uses cluster multicast.  Every wait is bounded (mbar_wait*), as in mp_umma_gemm.cuh.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "mp_ptx.cuh"
+
+namespace mp {
+
+constexpr int kPairRows = 256;               // rows of D per tile
+constexpr int kPairMaxBN = 256;
+constexpr int kPairThreads = 320;
+constexpr int kPairABytes = 128 * 128;       // one CTA's share of A per 64 contraction elements
+constexpr int kPairMaxStages = 8;
+constexpr int kPairSmem = 232448;            // 227 KB opt-in limit per CTA
+
+enum { PAIR_STORE = 0, PAIR_LSE = 1, PAIR_DLOGITS = 2 };
+
+// One GEMM of a launch.  A launch may hold two (they share the persistent grid, so the partly empty last wave of one is
+// filled by the other).
+struct PairProblem {
+  int rows, cols, kblocks;       // extents of D, 64-element blocks of the contraction
+  int tiles_m, tiles_n, bn;
+  int a_mn, b_mn;                // 1: MN-major operand
+  int group_m;                   // raster: tiles are walked in groups of `group_m` row tiles
+  int tile0;                     // index of the problem's first tile in the launch
+  // PAIR_STORE: out16 = scale * acc (+ acc32 before scaling), or acc32 (+)= acc when out16 is null
+  void* out16;
+  float* acc32;
+  long long ld_out;              // row stride of out16 in elements
+  long long ld_acc;
+  int add_acc32;                 // 1: acc32 holds earlier contributions
+  const float* scale;            // device scalar, may be null (1.0)
+};
+
+struct PairParams {
+  int num_problems;
+  PairProblem prob[2];
+  int total_tiles;
+  int stages, stage_bytes;
+  int bf16;                      // operand and output type: 1 = bf16, 0 = fp16
+  int* status;
+  // PAIR_LSE / PAIR_DLOGITS (the columns of D are vocabulary entries col0 ... col0 + cols - 1)
+  const void* target; int target64;
+  long long ignore_index;
+  int col0;
+  float2* partial;               // PAIR_LSE: [2 * tiles_n][rows] (max, sum of exp(z - max))
+  float* target_logit;           // PAIR_LSE: [rows]
+  const float* lse;              // PAIR_DLOGITS
+  const float* coef;             // PAIR_DLOGITS: row factor
+  uint16_t* dlogits; long long ld_dl;
+};
+
+// ------------------------------------------------------------------------------------------------- PTX for CTA pairs
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_smem, const CUtensorMap* tm, uint32_t cluster_bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tm)), "r"(cluster_bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// Arrive on the barrier at this shared-memory offset in both CTAs once all MMAs issued so far have completed.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// MN-major tile, 128-byte swizzle: lines of 64 row indices (128 bytes), one line per contraction index, 8 lines per
+// swizzle atom (1024 bytes apart); `block_bytes` separates consecutive blocks of 64 row indices.
+__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t saddr, uint32_t block_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3ffffu) >> 4);
+  d |= static_cast<uint64_t>(block_bytes >> 4) << 16;         // leading byte offset: next 64 row indices
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;                // stride byte offset: next 8 contraction indices
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {        // 2^x, 2 ulp, subnormal results flushed to zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// After an error: give copies already under way (their barrier may be the peer's) ample time to land.
+__device__ __forceinline__ void settle_copies() {
+  const unsigned long long t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 5000000ull) {}
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, int bf16) {
+  if (bf16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// `n` consecutive 16-bit outputs starting at o from v[0..31] (n <= 32); 16-byte stores where the address allows.
+__device__ __forceinline__ void store_row32(uint16_t* o, const float (&v)[32], int n, int bf16) {
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = pack16(v[2 * j], v[2 * j + 1], bf16);
+  if (n == 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) reinterpret_cast<uint4*>(o)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < n) o[j] = (uint16_t)(j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
+  }
+}
+
+struct PairUnit { int prob, tm, tn; };
+
+__host__ __device__ __forceinline__ PairUnit pair_unit(const PairParams& p, int unit) {
+  PairUnit u;
+  u.prob = (p.num_problems == 2 && unit >= p.prob[1].tile0) ? 1 : 0;
+  const PairProblem& q = p.prob[u.prob];
+  const int t = unit - q.tile0;
+  const int group = q.group_m * q.tiles_n;
+  const int g = t / group, first = g * q.group_m;
+  const int height = q.tiles_m - first < q.group_m ? q.tiles_m - first : q.group_m;
+  const int in = t - g * group;
+  u.tn = in / height;
+  u.tm = first + (in - u.tn * height);
+  return u;
+}
+
+// ------------------------------------------------------------------------------------------------------ the epilogues
+// Softmax statistics of this warp's half of the tile's columns, one row per lane.  Two passes over the accumulator (the
+// maximum, then the sum): no rescaling, and z - max is formed before the multiplication by log2(e), so that the sum is
+// exact to a few units in the last place whatever the logits' size.  An infinite maximum is replaced by 0 (exp then
+// gives 0 or infinity as the definition does); NaN passes through the sum.
+__device__ __forceinline__ void pair_epilogue_lse(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
+                                                  int tn, int half, int ncols, int half_cols) {
+  const bool live = row < q.rows;
+  long long target = -1;
+  if (live) {
+    const long long t = p.target64 ? reinterpret_cast<const long long*>(p.target)[row] : reinterpret_cast<const int*>(p.target)[row];
+    if (t != p.ignore_index) target = t - c_begin;                       // column inside this warp's half, if any
+  }
+  float m = -INFINITY;
+  for (int c0 = 0; c0 < half_cols; c0 += 32) {
+    uint32_t v[32];
+    __syncwarp();
+    tmem_ld_x32(t_addr + (uint32_t)c0, v);
+    tmem_ld_wait();
+    if (c0 + 32 <= ncols) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) m = fmaxf(m, __uint_as_float(v[j]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) if (c0 + j < ncols) m = fmaxf(m, __uint_as_float(v[j]));
+    }
+    if (target >= c0 && target < c0 + 32) {
+      float z = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) if (target == c0 + j) z = __uint_as_float(v[j]);
+      if (target < ncols) p.target_logit[row] = z;
+    }
+  }
+  const float base = isinf(m) ? 0.0f : m;
+  float s0 = 0.0f, s1 = 0.0f;
+  for (int c0 = 0; c0 < half_cols; c0 += 32) {
+    uint32_t v[32];
+    __syncwarp();
+    tmem_ld_x32(t_addr + (uint32_t)c0, v);
+    tmem_ld_wait();
+    if (c0 + 32 <= ncols) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 2) {
+        s0 += exp2_approx((__uint_as_float(v[j]) - base) * kLog2e);
+        s1 += exp2_approx((__uint_as_float(v[j + 1]) - base) * kLog2e);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) if (c0 + j < ncols) s0 += exp2_approx((__uint_as_float(v[j]) - base) * kLog2e);
+    }
+  }
+  // a half without columns keeps (-inf, 0); an infinite maximum is stored as its base
+  const float mm = m == -INFINITY ? m : base;
+  if (live) p.partial[(size_t)(2 * tn + half) * q.rows + row] = make_float2(mm, s0 + s1);
+}
+
+// d = coef[row] * (softmax - onehot), rounded once to the operand type and parked for the two gradient products.
+__device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
+                                                      int ncols, int half_cols) {
+  const bool live = row < q.rows;
+  long long target = -1;
+  float lse = 0.0f, coef = 0.0f;
+  bool kept = false;
+  if (live) {
+    const long long t = p.target64 ? reinterpret_cast<const long long*>(p.target)[row] : reinterpret_cast<const int*>(p.target)[row];
+    kept = t != p.ignore_index;
+    target = t - p.col0 - c_begin;
+    lse = p.lse[row];
+    coef = p.coef[row];
+  }
+  uint16_t* o = p.dlogits + (long long)row * p.ld_dl + c_begin;
+  for (int c0 = 0; c0 < half_cols; c0 += 32) {
+    uint32_t v[32];
+    __syncwarp();
+    tmem_ld_x32(t_addr + (uint32_t)c0, v);
+    tmem_ld_wait();
+    float d[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) d[j] = kept ? coef * exp2_approx((__uint_as_float(v[j]) - lse) * kLog2e) : 0.0f;
+    if (kept && target >= c0 && target < c0 + 32) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (target == c0 + j) d[j] = coef * (exp2_approx((__uint_as_float(v[j]) - lse) * kLog2e) - 1.0f);
+    }
+    const int n = ncols - c0 < 32 ? ncols - c0 : 32;
+    if (live && n > 0) store_row32(o + c0, d, n, p.bf16);
+  }
+}
+
+__device__ __forceinline__ void pair_epilogue_store(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
+                                                    int ncols, int half_cols) {
+  const bool live = row < q.rows;
+  const float scale = (q.out16 != nullptr && q.scale != nullptr) ? *q.scale : 1.0f;
+  for (int c0 = 0; c0 < half_cols; c0 += 32) {
+    uint32_t r[32];
+    __syncwarp();
+    tmem_ld_x32(t_addr + (uint32_t)c0, r);
+    tmem_ld_wait();
+    const int n = ncols - c0 < 32 ? ncols - c0 : 32;
+    if (!live || n <= 0) continue;
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+    float* a = q.acc32 + (long long)row * q.ld_acc + c_begin + c0;
+    if (q.add_acc32) {                                  // ld_acc is a multiple of 32: rows of the scratch are padded
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 t = reinterpret_cast<const float4*>(a)[j];
+        v[4 * j] += t.x; v[4 * j + 1] += t.y; v[4 * j + 2] += t.z; v[4 * j + 3] += t.w;
+      }
+    }
+    if (q.out16 != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= scale;
+      store_row32(reinterpret_cast<uint16_t*>(q.out16) + (long long)row * q.ld_out + c_begin + c0, v, n, p.bf16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) reinterpret_cast<float4*>(a)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------- the kernel
+template <int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0,
+                 const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB1, const PairParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  // both CTAs of the pair see the same dynamic shared-memory offset, so the rounding agrees
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t smem_base = smem_u32(smem);
+  const int stages = p.stages;
+  const uint32_t bar_base = smem_base + (uint32_t)stages * (uint32_t)p.stage_bytes;
+  auto full_bar = [&](int s) { return bar_base + 8u * (uint32_t)s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (uint32_t)(stages + s); };
+  auto tfull_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + b); };
+  auto tempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 2 + b); };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+  int* status = p.status;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), 16); }
+    mbar_fence_init();
+    tma_prefetch_desc(&tmA0);
+    tma_prefetch_desc(&tmB0);
+    if (p.num_problems == 2) { tma_prefetch_desc(&tmA1); tma_prefetch_desc(&tmB1); }
+  }
+  if (warp == 1) tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  cluster_sync_all();                       // the peer's barriers are initialised, its TMEM is allocated
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------------------ TMA producer (one lane)
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0, it = 0;
+      bool ok = true;
+      for (int unit = pair; ok && unit < p.total_tiles; unit += pairs) {
+        const PairUnit u = pair_unit(p, unit);
+        const PairProblem& q = p.prob[u.prob];
+        const CUtensorMap* tmA = u.prob ? &tmA1 : &tmA0;
+        const CUtensorMap* tmB = u.prob ? &tmB1 : &tmB0;
+        const int hb = q.bn >> 1;
+        const int a0 = u.tm * kPairRows + (int)rank * 128, b0 = u.tn * q.bn + (int)rank * hb;
+        const uint32_t tx = 2u * (uint32_t)(kPairABytes + hb * 128);      // both CTAs' bytes
+        for (int kb = 0; kb < q.kblocks; ++kb, ++it) {
+          if (!mbar_wait_cluster(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
+          const uint32_t a_dst = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes, b_dst = a_dst + kPairABytes;
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), tx);
+          const uint32_t bar = mapa_shared(full_bar(s), 0);
+          if (q.a_mn) {
+            tma_load_2d_pair(a_dst, tmA, bar, a0, kb * 64);
+            tma_load_2d_pair(a_dst + 8192u, tmA, bar, a0 + 64, kb * 64);
+          } else {
+            tma_load_2d_pair(a_dst, tmA, bar, kb * 64, a0);
+          }
+          if (q.b_mn) {
+            for (int j = 0; j < hb; j += 64) tma_load_2d_pair(b_dst + (uint32_t)j * 128u, tmB, bar, b0 + j, kb * 64);
+          } else {
+            tma_load_2d_pair(b_dst, tmB, bar, kb * 64, b0);
+          }
+          if (++s == stages) { s = 0; ph ^= 1u; }
+        }
+      }
+      // every stage handed back: all copies have landed and all commits have reached this CTA's barriers
+      for (int i = 0; ok && i < stages; ++i) {
+        ok = mbar_wait_cluster(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_DRAIN);
+        if (++s == stages) { s = 0; ph ^= 1u; }
+      }
+      if (!ok) settle_copies();
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------------------- MMA issuer (one lane of rank 0's warp)
+    if (lane == 0 && rank == 0) {
+      int s = 0;
+      uint32_t ph = 0, ui = 0;
+      bool ok = true;
+      for (int unit = pair; ok && unit < p.total_tiles; unit += pairs, ++ui) {
+        const PairUnit u = pair_unit(p, unit);
+        const PairProblem& q = p.prob[u.prob];
+        const uint32_t buf = ui & 1u, use = ui >> 1;
+        if (!mbar_wait_cluster(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * (uint32_t)kPairMaxBN;
+        const uint32_t idesc = umma_idesc(1u, p.bf16 ? 1u : 0u, kPairRows, (uint32_t)q.bn) | ((uint32_t)q.a_mn << 15) | ((uint32_t)q.b_mn << 16);
+        const uint64_t a_base = q.a_mn ? umma_smem_desc_mn(smem_base, 8192u) : umma_smem_desc_sw128(smem_base);
+        const uint64_t b_base = (q.b_mn ? umma_smem_desc_mn(smem_base, 8192u) : umma_smem_desc_sw128(smem_base)) + (kPairABytes >> 4);
+        // 16 contraction elements further: 32 bytes along a K-major line, or 16 lines of an MN-major tile
+        const uint32_t a_step = q.a_mn ? 2048u >> 4 : 2u, b_step = q.b_mn ? 2048u >> 4 : 2u;
+        const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4;
+        uint32_t first = 0u;
+        for (int kb = 0; kb < q.kblocks; ++kb) {
+          if (!mbar_wait_cluster(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t ad = a_base + (uint64_t)((uint32_t)s * stage16), bd = b_base + (uint64_t)((uint32_t)s * stage16);
+#pragma unroll
+          for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_pair(d_tmem, ad + kk * a_step, bd + kk * b_step, idesc, kk > 0 ? 1u : first);
+          first = 1u;
+          tc_commit_pair(empty_bar(s));
+          if (++s == stages) { s = 0; ph ^= 1u; }
+        }
+        if (ok) tc_commit_pair(tfull_bar((int)buf));
+      }
+    }
+  } else {
+    // -------------------------------------------------------------------------------------------------- epilogue warps
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    uint32_t ui = 0;
+    for (int unit = pair; unit < p.total_tiles; unit += pairs, ++ui) {
+      const PairUnit u = pair_unit(p, unit);
+      const PairProblem& q = p.prob[u.prob];
+      const uint32_t buf = ui & 1u, use = ui >> 1;
+      if (!mbar_wait_cluster(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
+      tc_fence_after();
+      const int half_cols = q.bn >> 1;
+      const int row = u.tm * kPairRows + (int)rank * 128 + quad * 32 + lane;
+      const int c_begin = u.tn * q.bn + half * half_cols;                // first column of this warp's half
+      const int ncols = min(half_cols, q.cols - c_begin);                // may be <= 0 in the last column tile
+      const uint32_t t_addr = tmem_base + buf * (uint32_t)kPairMaxBN + (uint32_t)(half * half_cols) + ((uint32_t)(quad * 32) << 16);
+      if constexpr (EPI == PAIR_LSE) pair_epilogue_lse(p, q, t_addr, row, c_begin, u.tn, half, ncols, half_cols);
+      else if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols);
+      else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar((int)buf), 0));
+    }
+  }
+
+  // Neither CTA may leave while the other can still read its shared memory, signal its barriers or use its TMEM.
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+}  // namespace mp

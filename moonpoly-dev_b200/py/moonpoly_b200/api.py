@@ -79,6 +79,11 @@ def lib() -> ctypes.CDLL:
         L.mp_peer_open.argtypes = [ctypes.c_char_p, ctypes.POINTER(vp)]
         L.mp_peer_close.argtypes = [vp]
         L.mp_peer_free.argtypes = [vp]
+        ll = ctypes.c_longlong
+        xent = [ci, ci, ci, ci, vp, ll, vp, ll]
+        L.mp_linear_xent_workspace.argtypes = xent + [ci, ctypes.POINTER(sz)]
+        L.mp_linear_xent.argtypes = xent + [vp, ci, ll, vp, vp, vp, sz, vp]
+        L.mp_linear_xent_grad.argtypes = xent + [vp, ci, ll, vp, vp, vp, vp, vp, sz, vp]
         _lib = L
     return _lib
 
@@ -407,6 +412,86 @@ def scaled_int8_mm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_s
                                  _ptr(b_scales), int(b_scales.numel() == 1), _ptr(bias), _ptr(out), N,
                                  0 if out_dtype == torch.float16 else 1, _stream(a)))
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# Linear with softmax cross entropy (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------------
+def _dtype16(t: torch.Tensor, op: str) -> int:
+    if t.dtype == torch.float16:
+        return MP_FP16
+    if t.dtype == torch.bfloat16:
+        return MP_BF16
+    raise ValueError(f"{op} serves fp16 and bf16")
+
+
+def _rows(t: torch.Tensor):
+    """(tensor, row stride) of a 2-D operand whose rows are packed; anything else is copied."""
+    if t.stride(1) != 1 and t.shape[1] > 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _xent_checks(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor) -> None:
+    _linear_checks(x, w)
+    _dtype16(x, "linear_cross_entropy")
+    if w.shape[0] == 0 or w.shape[1] == 0:
+        raise ValueError("the weight [V, H] must not be empty")
+    if target.dim() != 1 or target.shape[0] != x.shape[0] or target.dtype not in (torch.int64, torch.int32):
+        raise ValueError("target must be M integers (int64 or int32)")
+    if x.device != w.device or target.device != x.device:
+        raise ValueError("x, w and target must be on one device")
+
+
+def _xent_workspace(code, M, V, H, x, ldx, w, ldw, backward) -> torch.Tensor:
+    # a fresh tensor per call: calls on other streams and captured graphs never share it
+    need = ctypes.c_size_t()
+    _check(lib().mp_linear_xent_workspace(code, M, V, H, _ptr(x), ldx, _ptr(w), ldw, backward, ctypes.byref(need)))
+    return torch.empty((need.value,), dtype=torch.uint8, device=x.device)
+
+
+def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, ignore_index: int = -100):
+    """(loss [M], lse [M]) in fp32 of the logits z = x[M,H] @ w[V,H]^T, which are never held: lse = logsumexp(z) per row,
+    loss = lse - z[target], 0 where target == ignore_index, NaN where target is any other value outside [0, V).
+    x and w fp16 or bf16.  Take the mean (or any other weighting) of `loss` outside; `linear_cross_entropy_grad` gives
+    the gradients from `lse` and the gradient with respect to `loss`."""
+    _xent_checks(x, w, target)
+    code = _dtype16(x, "linear_cross_entropy")
+    (M, H), V = x.shape, w.shape[0]
+    with torch.cuda.device(x.device):
+        x, ldx = _rows(x)
+        w, ldw = _rows(w)
+        target = target.contiguous()
+        loss = torch.empty((M,), dtype=torch.float32, device=x.device)
+        lse = torch.empty_like(loss)
+        ws = _xent_workspace(code, M, V, H, x, ldx, w, ldw, 0)
+        _check(lib().mp_linear_xent(code, M, V, H, _ptr(x), ldx, _ptr(w), ldw, _ptr(target), target.element_size(), ignore_index,
+                                    _ptr(loss), _ptr(lse), _ptr(ws), ws.numel(), _stream(x)))
+    return loss, lse
+
+
+def linear_cross_entropy_grad(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, grad_loss: torch.Tensor,
+                              ignore_index: int = -100, need_dx: bool = True, need_dw: bool = True):
+    """(dx [M,H], dw [V,H]) of `linear_cross_entropy` for grad_loss [M] (fp32, the gradient with respect to `loss`); `lse`
+    is what the forward call returned.  A gradient that is not needed is None and costs nothing.  The logits are computed
+    again, a piece of the vocabulary at a time.  Deterministic: no atomics, fixed order of sums."""
+    _xent_checks(x, w, target)
+    code = _dtype16(x, "linear_cross_entropy_grad")
+    (M, H), V = x.shape, w.shape[0]
+    for name, t in (("lse", lse), ("grad_loss", grad_loss)):
+        if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != M or t.device != x.device:
+            raise ValueError(f"{name} must be M fp32 values on the operands' device")
+    with torch.cuda.device(x.device):
+        dx = torch.empty((M, H), dtype=x.dtype, device=x.device) if need_dx else None
+        dw = torch.empty((V, H), dtype=x.dtype, device=x.device) if need_dw else None
+        x, ldx = _rows(x)
+        w, ldw = _rows(w)
+        target, lse, grad_loss = target.contiguous(), lse.contiguous(), grad_loss.contiguous()
+        ws = _xent_workspace(code, M, V, H, x, ldx, w, ldw, 1)
+        _check(lib().mp_linear_xent_grad(code, M, V, H, _ptr(x), ldx, _ptr(w), ldw, _ptr(target), target.element_size(),
+                                         ignore_index, _ptr(lse), _ptr(grad_loss), _ptr(dx), _ptr(dw), _ptr(ws), ws.numel(),
+                                         _stream(x)))
+    return dx, dw
 
 
 # ------------------------------------------------------------------------------------------------

@@ -1140,6 +1140,18 @@ int host_tmap(CUtensorMap* tm, int type, const void* ptr, long long inner, long 
   return MP_OK;
 }
 
+int host_tmap_blocks(CUtensorMap* tm, const void* ptr, long long inner, long long rows, long long row_bytes, int box_rows, int box_blocks) {
+  const cuuint64_t gdim[3] = {64, (cuuint64_t)rows, (cuuint64_t)(inner / 64)};
+  const cuuint64_t gstride[2] = {(cuuint64_t)row_bytes, 128};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_blocks};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(ptr), gdim, gstride, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MP_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return MP_OK;
+}
+
 int host_pad_rows16(const void* src, long long ld, void* dst, int rows, int k, int kp, cudaStream_t stream) {
   const long long words = (long long)rows * (kp / 8);
   const int grid = (int)std::min<long long>((words + 255) / 256, 148 * 16);

@@ -19,6 +19,9 @@ int host_device(HostDevice* out);
 enum { kTmap16 = 0, kTmapByte = 1 };
 int host_tmap(CUtensorMap* tm, int type, const void* ptr, long long inner, long long rows, long long row_bytes, int box_inner,
               int box_rows, int swizzle);
+// The same matrix of 16-bit elements as [inner / 64][rows][64] (inner a multiple of 64): a box brings `box_blocks` blocks
+// of 128 bytes, contiguous in memory, of every line; 128-byte swizzle.
+int host_tmap_blocks(CUtensorMap* tm, const void* ptr, long long inner, long long rows, long long row_bytes, int box_rows, int box_blocks);
 
 // dst[r][0 .. kp) = src[r][0 .. k) followed by zeros, 16-bit elements; kp a multiple of 8, dst 16-byte aligned.
 int host_pad_rows16(const void* src, long long ld, void* dst, int rows, int k, int kp, cudaStream_t stream);

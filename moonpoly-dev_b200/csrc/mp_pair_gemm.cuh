@@ -10,7 +10,7 @@
 // own row index contiguous ("MN-major": what the gradients need, dX = dY * W and dW = dY^T * X read W, dY and X as they
 // lie, without transposed copies).  Both forms are TMA boxes of 128 contiguous bytes per line, 128-byte swizzled.
 //
-// Roles per CTA: warp 0 = TMA producer, warp 1 = MMA issuer (rank 0 of the pair only) and TMEM owner, warps 2..9 =
+// Roles per CTA: warp 0 = TMA producer, warp 1 = MMA issuer (rank 0 of the pair only) and TMEM owner, warps 4..11 =
 // epilogue (TMEM lane quadrant = warp % 4, two warps per quadrant taking the two halves of the columns).
 // Barriers: full[s] lives in rank 0 and counts the bytes of both CTAs; empty[s] and tfull[b] exist in both CTAs and are
 // signalled by multicast commits; tempty[b] lives in rank 0 and takes the arrivals of the 16 epilogue warps of the pair.
@@ -25,7 +25,7 @@ namespace mp {
 
 constexpr int kPairRows = 256;               // rows of D per tile
 constexpr int kPairMaxBN = 256;
-constexpr int kPairThreads = 320;
+constexpr int kPairThreads = 384;             // warps 2 and 3 only fill the first warpgroup up
 constexpr int kPairABytes = 128 * 128;       // one CTA's share of A per 64 contraction elements
 constexpr int kPairMaxStages = 8;
 constexpr int kPairSmem = 232448;            // 227 KB opt-in limit per CTA
@@ -38,6 +38,7 @@ struct PairProblem {
   int rows, cols, kblocks;       // extents of D, 64-element blocks of the contraction
   int tiles_m, tiles_n, bn;
   int a_mn, b_mn;                // 1: MN-major operand
+  int a_wide, b_wide;            // 1: the operand's tensor map is 3-D and one box brings 256 contiguous bytes per line
   int group_m;                   // raster: tiles are walked in groups of `group_m` row tiles
   int tile0;                     // index of the problem's first tile in the launch
   // PAIR_STORE: out16 = scale * acc (+ acc32 before scaling), or acc32 (+)= acc when out16 is null
@@ -54,6 +55,7 @@ struct PairParams {
   PairProblem prob[2];
   int total_tiles;
   int stages, stage_bytes;
+  int kc;                        // 64-element blocks of the contraction per stage (1 or 2)
   int bf16;                      // operand and output type: 1 = bf16, 0 = fp16
   int* status;
   // PAIR_LSE / PAIR_DLOGITS (the columns of D are vocabulary entries col0 ... col0 + cols - 1)
@@ -73,6 +75,13 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_smem, const CUtens
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tm)), "r"(cluster_bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst_smem, const CUtensorMap* tm, uint32_t cluster_bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tm)), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
@@ -117,6 +126,9 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
+// Registers per thread of a warpgroup from here on.  The launch has 384 x 168; 128 x 88 + 256 x 208 is just that.
+__device__ __forceinline__ void regs_fewer_88() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
+__device__ __forceinline__ void regs_more_208() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
 __device__ __forceinline__ float exp2_approx(float x) {        // 2^x, 2 ulp, subnormal results flushed to zero
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -154,6 +166,19 @@ __device__ __forceinline__ void store_row32(uint16_t* o, const float (&v)[32], i
   }
 }
 
+// One stage of one operand: `rows` row indices from r0, contraction blocks kb ... kb + kc - 1.  K-major: [block][row][128 B];
+// MN-major: [64 row indices][kc * 64 contraction indices][128 B].  Blocks past the end of the contraction are filled with
+// zeros and count their bytes like the others.
+__device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int mn, int wide, int rows, int r0, int kb, int kc) {
+  if (mn) {
+    if (wide) tma_load_3d_pair(dst, tm, bar, 0, kb * 64, r0 >> 6);
+    else for (int j = 0; j < rows; j += 64) tma_load_2d_pair(dst + (uint32_t)(j * kc * 128), tm, bar, r0 + j, kb * 64);
+  } else {
+    if (wide) tma_load_3d_pair(dst, tm, bar, 0, r0, kb);
+    else for (int c = 0; c < kc; ++c) tma_load_2d_pair(dst + (uint32_t)(c * rows * 128), tm, bar, (kb + c) * 64, r0);
+  }
+}
+
 struct PairUnit { int prob, tm, tn; };
 
 __host__ __device__ __forceinline__ PairUnit pair_unit(const PairParams& p, int unit) {
@@ -171,55 +196,43 @@ __host__ __device__ __forceinline__ PairUnit pair_unit(const PairParams& p, int 
 }
 
 // ------------------------------------------------------------------------------------------------------ the epilogues
-// Softmax statistics of this warp's half of the tile's columns, one row per lane.  Two passes over the accumulator (the
-// maximum, then the sum): no rescaling, and z - max is formed before the multiplication by log2(e), so that the sum is
-// exact to a few units in the last place whatever the logits' size.  An infinite maximum is replaced by 0 (exp then
-// gives 0 or infinity as the definition does); NaN passes through the sum.
-__device__ __forceinline__ void pair_epilogue_lse(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
-                                                  int tn, int half, int ncols, int half_cols) {
+// Softmax statistics of this warp's half (128 columns) of a 256-column tile, one row per lane.  The tensor cores drop the
+// bits that an addition shifts out, always towards zero, so a long contraction pulls every logit to zero (H = 4096:
+// 2e-5, which the mean over a vocabulary does not average away).  The contraction therefore comes in chunks of
+// kLseChunk blocks, each in an accumulator of its own, and the chunks are added here, rounded to nearest: 1.6e-6 ->
+// 0.6e-6 relative error of the loss at H = 4096, while the other accumulator is being filled.
+// The maximum is taken first and z - max is formed before the multiplication by log2(e), so that the sum is exact to a
+// few units in the last place whatever the logits' size.  An infinite maximum is replaced by 0 (exp then gives 0 or
+// infinity as the definition does); NaN passes through the sum.
+constexpr int kLseChunk = 16;                // blocks of 64 contraction elements per accumulator
+__device__ __forceinline__ void pair_epilogue_lse(const PairParams& p, const PairProblem& q, const float (&z)[128], int row, int c_begin,
+                                                  int tn, int half, int ncols) {
   const bool live = row < q.rows;
   long long target = -1;
   if (live) {
     const long long t = p.target64 ? reinterpret_cast<const long long*>(p.target)[row] : reinterpret_cast<const int*>(p.target)[row];
     if (t != p.ignore_index) target = t - c_begin;                       // column inside this warp's half, if any
   }
-  float m = -INFINITY;
-  for (int c0 = 0; c0 < half_cols; c0 += 32) {
-    uint32_t v[32];
-    __syncwarp();
-    tmem_ld_x32(t_addr + (uint32_t)c0, v);
-    tmem_ld_wait();
-    if (c0 + 32 <= ncols) {
+  float m = -INFINITY, s0 = 0.0f, s1 = 0.0f;
+  const bool full = ncols >= 128;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) m = fmaxf(m, __uint_as_float(v[j]));
-    } else {
+  for (int j = 0; j < 128; ++j) if (full || j < ncols) m = fmaxf(m, z[j]);
+  if (target >= 0 && target < ncols && target < 128) {
+    float t = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) if (c0 + j < ncols) m = fmaxf(m, __uint_as_float(v[j]));
-    }
-    if (target >= c0 && target < c0 + 32) {
-      float z = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 32; ++j) if (target == c0 + j) z = __uint_as_float(v[j]);
-      if (target < ncols) p.target_logit[row] = z;
-    }
+    for (int j = 0; j < 128; ++j) if (target == j) t = z[j];
+    p.target_logit[row] = t;
   }
   const float base = isinf(m) ? 0.0f : m;
-  float s0 = 0.0f, s1 = 0.0f;
-  for (int c0 = 0; c0 < half_cols; c0 += 32) {
-    uint32_t v[32];
-    __syncwarp();
-    tmem_ld_x32(t_addr + (uint32_t)c0, v);
-    tmem_ld_wait();
-    if (c0 + 32 <= ncols) {
+  if (full) {
 #pragma unroll
-      for (int j = 0; j < 32; j += 2) {
-        s0 += exp2_approx((__uint_as_float(v[j]) - base) * kLog2e);
-        s1 += exp2_approx((__uint_as_float(v[j + 1]) - base) * kLog2e);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) if (c0 + j < ncols) s0 += exp2_approx((__uint_as_float(v[j]) - base) * kLog2e);
+    for (int j = 0; j < 128; j += 2) {
+      s0 += exp2_approx((z[j] - base) * kLog2e);
+      s1 += exp2_approx((z[j + 1] - base) * kLog2e);
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 128; ++j) if (j < ncols) s0 += exp2_approx((z[j] - base) * kLog2e);
   }
   // a half without columns keeps (-inf, 0); an infinite maximum is stored as its base
   const float mm = m == -INFINITY ? m : base;
@@ -329,11 +342,12 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
   const uint32_t tmem_base = *tmem_slot;
   cluster_sync_all();                       // the peer's barriers are initialised, its TMEM is allocated
 
-  if (warp == 0) {
+  if (warp < 4) {
+    if constexpr (EPI == PAIR_LSE) regs_fewer_88();      // its epilogue holds 128 sums per thread
     // ------------------------------------------------------------------------------------------ TMA producer (one lane)
-    if (lane == 0) {
+    if (warp == 0 && lane == 0) {
       int s = 0;
-      uint32_t ph = 0, it = 0;
+      uint32_t ph = 0;
       bool ok = true;
       for (int unit = pair; ok && unit < p.total_tiles; unit += pairs) {
         const PairUnit u = pair_unit(p, unit);
@@ -342,23 +356,14 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         const CUtensorMap* tmB = u.prob ? &tmB1 : &tmB0;
         const int hb = q.bn >> 1;
         const int a0 = u.tm * kPairRows + (int)rank * 128, b0 = u.tn * q.bn + (int)rank * hb;
-        const uint32_t tx = 2u * (uint32_t)(kPairABytes + hb * 128);      // both CTAs' bytes
-        for (int kb = 0; kb < q.kblocks; ++kb, ++it) {
+        const uint32_t a_bytes = (uint32_t)(p.kc * kPairABytes), tx = 2u * (a_bytes + (uint32_t)(p.kc * hb * 128));   // both CTAs
+        for (int kb = 0; kb < q.kblocks; kb += p.kc) {
           if (!mbar_wait_cluster(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
-          const uint32_t a_dst = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes, b_dst = a_dst + kPairABytes;
+          const uint32_t dst = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), tx);
           const uint32_t bar = mapa_shared(full_bar(s), 0);
-          if (q.a_mn) {
-            tma_load_2d_pair(a_dst, tmA, bar, a0, kb * 64);
-            tma_load_2d_pair(a_dst + 8192u, tmA, bar, a0 + 64, kb * 64);
-          } else {
-            tma_load_2d_pair(a_dst, tmA, bar, kb * 64, a0);
-          }
-          if (q.b_mn) {
-            for (int j = 0; j < hb; j += 64) tma_load_2d_pair(b_dst + (uint32_t)j * 128u, tmB, bar, b0 + j, kb * 64);
-          } else {
-            tma_load_2d_pair(b_dst, tmB, bar, kb * 64, b0);
-          }
+          pair_load(dst, tmA, bar, q.a_mn, q.a_wide, 128, a0, kb, p.kc);
+          pair_load(dst + a_bytes, tmB, bar, q.b_mn, q.b_wide, hb, b0, kb, p.kc);
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
       }
@@ -369,60 +374,98 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
       }
       if (!ok) settle_copies();
     }
-  } else if (warp == 1) {
     // ---------------------------------------------------------------------------- MMA issuer (one lane of rank 0's warp)
-    if (lane == 0 && rank == 0) {
+    if (warp == 1 && lane == 0 && rank == 0) {
       int s = 0;
       uint32_t ph = 0, ui = 0;
       bool ok = true;
-      for (int unit = pair; ok && unit < p.total_tiles; unit += pairs, ++ui) {
+      for (int unit = pair; ok && unit < p.total_tiles; unit += pairs) {
         const PairUnit u = pair_unit(p, unit);
         const PairProblem& q = p.prob[u.prob];
+        const uint32_t idesc = umma_idesc(1u, p.bf16 ? 1u : 0u, kPairRows, (uint32_t)q.bn) | ((uint32_t)q.a_mn << 15) | ((uint32_t)q.b_mn << 16);
+        const uint32_t mn_block = (uint32_t)p.kc * 8192u;
+        const uint64_t a_base = q.a_mn ? umma_smem_desc_mn(smem_base, mn_block) : umma_smem_desc_sw128(smem_base);
+        const uint64_t b_base = (q.b_mn ? umma_smem_desc_mn(smem_base, mn_block) : umma_smem_desc_sw128(smem_base)) +
+                                (uint64_t)((uint32_t)(p.kc * kPairABytes) >> 4);
+        // 16 contraction elements further: 32 bytes along a K-major line, or 16 lines of an MN-major tile; 64 further: the
+        // next K-major block, or 64 lines
+        const uint32_t a_step = q.a_mn ? 2048u >> 4 : 2u, b_step = q.b_mn ? 2048u >> 4 : 2u;
+        const uint32_t a_blk = q.a_mn ? 8192u >> 4 : kPairABytes >> 4, b_blk = q.b_mn ? 8192u >> 4 : (uint32_t)(q.bn >> 1) * 128u >> 4;
+        const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4;
+        // an accumulator takes the whole contraction, or a chunk of it (PAIR_LSE)
+        const int chunk = EPI == PAIR_LSE ? kLseChunk : q.kblocks;
+        for (int k0 = 0; ok && k0 < q.kblocks; k0 += chunk, ++ui) {
         const uint32_t buf = ui & 1u, use = ui >> 1;
         if (!mbar_wait_cluster(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * (uint32_t)kPairMaxBN;
-        const uint32_t idesc = umma_idesc(1u, p.bf16 ? 1u : 0u, kPairRows, (uint32_t)q.bn) | ((uint32_t)q.a_mn << 15) | ((uint32_t)q.b_mn << 16);
-        const uint64_t a_base = q.a_mn ? umma_smem_desc_mn(smem_base, 8192u) : umma_smem_desc_sw128(smem_base);
-        const uint64_t b_base = (q.b_mn ? umma_smem_desc_mn(smem_base, 8192u) : umma_smem_desc_sw128(smem_base)) + (kPairABytes >> 4);
-        // 16 contraction elements further: 32 bytes along a K-major line, or 16 lines of an MN-major tile
-        const uint32_t a_step = q.a_mn ? 2048u >> 4 : 2u, b_step = q.b_mn ? 2048u >> 4 : 2u;
-        const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4;
+        const int k1 = min(q.kblocks, k0 + chunk);
         uint32_t first = 0u;
-        for (int kb = 0; kb < q.kblocks; ++kb) {
+        for (int kb = k0; kb < k1; kb += p.kc) {
           if (!mbar_wait_cluster(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
           tc_fence_after();
-          const uint64_t ad = a_base + (uint64_t)((uint32_t)s * stage16), bd = b_base + (uint64_t)((uint32_t)s * stage16);
+          uint64_t ad = a_base + (uint64_t)((uint32_t)s * stage16), bd = b_base + (uint64_t)((uint32_t)s * stage16);
+          const int nc = min(p.kc, k1 - kb);
+          for (int c = 0; c < nc; ++c, ad += a_blk, bd += b_blk) {
 #pragma unroll
-          for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_pair(d_tmem, ad + kk * a_step, bd + kk * b_step, idesc, kk > 0 ? 1u : first);
-          first = 1u;
+            for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_pair(d_tmem, ad + kk * a_step, bd + kk * b_step, idesc, kk > 0 ? 1u : first);
+            first = 1u;
+          }
           tc_commit_pair(empty_bar(s));
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
         if (ok) tc_commit_pair(tfull_bar((int)buf));
+        }
       }
     }
   } else {
     // -------------------------------------------------------------------------------------------------- epilogue warps
-    const int quad = warp & 3, half = (warp - 2) >> 2;
+    if constexpr (EPI == PAIR_LSE) regs_more_208();
+    const int quad = warp & 3, half = (warp - 4) >> 2;
     uint32_t ui = 0;
-    for (int unit = pair; unit < p.total_tiles; unit += pairs, ++ui) {
+    bool ok = true;
+    for (int unit = pair; ok && unit < p.total_tiles; unit += pairs) {
       const PairUnit u = pair_unit(p, unit);
       const PairProblem& q = p.prob[u.prob];
-      const uint32_t buf = ui & 1u, use = ui >> 1;
-      if (!mbar_wait_cluster(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
-      tc_fence_after();
       const int half_cols = q.bn >> 1;
       const int row = u.tm * kPairRows + (int)rank * 128 + quad * 32 + lane;
       const int c_begin = u.tn * q.bn + half * half_cols;                // first column of this warp's half
       const int ncols = min(half_cols, q.cols - c_begin);                // may be <= 0 in the last column tile
-      const uint32_t t_addr = tmem_base + buf * (uint32_t)kPairMaxBN + (uint32_t)(half * half_cols) + ((uint32_t)(quad * 32) << 16);
-      if constexpr (EPI == PAIR_LSE) pair_epilogue_lse(p, q, t_addr, row, c_begin, u.tn, half, ncols, half_cols);
-      else if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols);
-      else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar((int)buf), 0));
+      const uint32_t t_half = tmem_base + (uint32_t)(half * half_cols) + ((uint32_t)(quad * 32) << 16);
+      if constexpr (EPI == PAIR_LSE) {
+        float z[128];
+#pragma unroll
+        for (int j = 0; j < 128; ++j) z[j] = 0.0f;
+        for (int k0 = 0; ok && k0 < q.kblocks; k0 += kLseChunk, ++ui) {
+          const uint32_t buf = ui & 1u, use = ui >> 1;
+          if (!mbar_wait_cluster(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            __syncwarp();
+            tmem_ld_x32(t_half + buf * (uint32_t)kPairMaxBN + 32u * c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[32 * c + j] += __uint_as_float(v[j]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar((int)buf), 0));
+        }
+        if (ok) pair_epilogue_lse(p, q, z, row, c_begin, u.tn, half, ncols);
+      } else {
+        const uint32_t buf = ui & 1u, use = ui >> 1;
+        if (!mbar_wait_cluster(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
+        tc_fence_after();
+        const uint32_t t_addr = t_half + buf * (uint32_t)kPairMaxBN;
+        if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols);
+        else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar((int)buf), 0));
+        ++ui;
+      }
     }
   }
 

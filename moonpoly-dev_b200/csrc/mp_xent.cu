@@ -166,9 +166,16 @@ int check_workspace(const char* op, void* ws, size_t have, size_t need) {
   return MP_OK;
 }
 
-// TMA view of a row-major 16-bit matrix as a K-major operand (`box_rows` rows per box) or as an MN-major one.
-int operand_map(CUtensorMap* tm, const void* ptr, long long inner, long long rows, long long ld, bool mn, int box_rows) {
-  return host_tmap(tm, kTmap16, ptr, inner, rows, ld * 2, 64, mn ? 64 : box_rows, 128);
+// 64-element contraction blocks per pipeline stage.
+constexpr int kStageBlocks = 2;
+
+// TMA view of a row-major 16-bit matrix as a K-major operand of which a CTA takes `rows_cta` rows, or as an MN-major one of
+// which it takes `rows_cta` columns.
+int operand_map(CUtensorMap* tm, const void* ptr, long long inner, long long rows, long long ld, bool mn, int rows_cta, int* wide) {
+  const int kc = kStageBlocks;
+  *wide = inner % 64 == 0 && kc > 1;
+  if (*wide) return host_tmap_blocks(tm, ptr, inner, rows, ld * 2, mn ? kc * 64 : rows_cta, mn ? rows_cta / 64 : kc);
+  return host_tmap(tm, kTmap16, ptr, inner, rows, ld * 2, 64, mn ? kc * 64 : rows_cta, 128);
 }
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -193,7 +200,8 @@ int launch_pair(const HostDevice& d, PairParams& p, const CUtensorMap (&tm)[4], 
     ready[d.index & 63] = true;
   }
   const int bn = p.num_problems == 2 ? std::max(p.prob[0].bn, p.prob[1].bn) : p.prob[0].bn;
-  p.stage_bytes = kPairABytes + bn / 2 * 128;
+  p.kc = kStageBlocks;
+  p.stage_bytes = p.kc * (kPairABytes + bn / 2 * 128);
   p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - 256) / p.stage_bytes);
   p.status = d.status;
   const int pairs = std::max(1, std::min(p.total_tiles, d.sms / 2));
@@ -249,8 +257,8 @@ int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx,
   p.partial = reinterpret_cast<float2*>(ws + l.partial);
   p.target_logit = reinterpret_cast<float*>(ws + l.target_logit);
   CUtensorMap tm[4];
-  if (int rc = operand_map(&tm[0], X, H, M, ldx, false, 128)) return rc;
-  if (int rc = operand_map(&tm[1], W, H, V, ldw, false, p.prob[0].bn / 2)) return rc;
+  if (int rc = operand_map(&tm[0], X, H, M, ldx, false, 128, &p.prob[0].a_wide)) return rc;
+  if (int rc = operand_map(&tm[1], W, H, V, ldw, false, p.prob[0].bn / 2, &p.prob[0].b_wide)) return rc;
   tm[2] = tm[0]; tm[3] = tm[1];
   if (int rc = launch_pair<PAIR_LSE>(d, p, tm, stream)) return rc;
   xent_join_kernel<<<ceil_div(M, 32), 1024, 0, stream>>>(p.partial, 2 * p.prob[0].tiles_n, M, p.target_logit, target, p.target64,
@@ -305,8 +313,8 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       p.bf16 = bf16;
       p.target = target; p.target64 = target64; p.ignore_index = ignore_index;
       p.col0 = col0; p.lse = lse; p.coef = coef; p.dlogits = dl; p.ld_dl = l.ld_dl;
-      if (int rc = operand_map(&tm[0], X, H, M, ldx, false, 128)) return rc;
-      if (int rc = operand_map(&tm[1], Wp, H, cols, ldw, false, p.prob[0].bn / 2)) return rc;
+      if (int rc = operand_map(&tm[0], X, H, M, ldx, false, 128, &p.prob[0].a_wide)) return rc;
+      if (int rc = operand_map(&tm[1], Wp, H, cols, ldw, false, p.prob[0].bn / 2, &p.prob[0].b_wide)) return rc;
       tm[2] = tm[0]; tm[3] = tm[1];
       if (int rc = launch_pair<PAIR_DLOGITS>(d, p, tm, stream)) return rc;
     }
@@ -320,8 +328,8 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       q.ld_acc = l.ld_acc;
       q.add_acc32 = i > 0;
       if (i == l.pieces - 1) { q.out16 = dX; q.ld_out = H; q.scale = scale; }
-      if (int rc = operand_map(&tm[2 * n], dl, cols, M, l.ld_dl, false, 128)) return rc;
-      if (int rc = operand_map(&tm[2 * n + 1], Wp, H, cols, ldw, true, 0)) return rc;
+      if (int rc = operand_map(&tm[2 * n], dl, cols, M, l.ld_dl, false, 128, &q.a_wide)) return rc;
+      if (int rc = operand_map(&tm[2 * n + 1], Wp, H, cols, ldw, true, q.bn / 2, &q.b_wide)) return rc;
       p.total_tiles += q.tiles_m * q.tiles_n;
       ++n;
     }
@@ -331,8 +339,8 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       q.out16 = reinterpret_cast<uint16_t*>(dW) + (long long)col0 * H;
       q.ld_out = H;
       q.scale = scale;
-      if (int rc = operand_map(&tm[2 * n], dl, cols, M, l.ld_dl, true, 0)) return rc;
-      if (int rc = operand_map(&tm[2 * n + 1], X, H, M, ldx, true, 0)) return rc;
+      if (int rc = operand_map(&tm[2 * n], dl, cols, M, l.ld_dl, true, 128, &q.a_wide)) return rc;
+      if (int rc = operand_map(&tm[2 * n + 1], X, H, M, ldx, true, q.bn / 2, &q.b_wide)) return rc;
       p.total_tiles += q.tiles_m * q.tiles_n;
       ++n;
     }

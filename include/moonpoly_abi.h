@@ -67,6 +67,30 @@ int mp_linear(int dtype, int M, int N, int K, const void* X, const void* W, void
  * added in the output type -- bit-identical to the two-step `linear` followed by `+ bias`.  bias may be NULL. */
 int mp_linear_bias(int dtype, int M, int N, int K, const void* X, const void* W, const void* bias, void* Y, void* stream);
 
+/* Linear with 4-bit weights (no counterpart in the reference).  W[n,k] = (q[n,k] - zero[n, k / group]) * scale[n, k / group].
+ *
+ * Packed weight: rows of 16 * ceil(K / 128) 32-bit words, 16-byte aligned.  A block of 128 weights is 16 words; word
+ * 4 t + i of a block (t, i = 0..3) holds weights k = 32 i + 8 t ... + 7 of the block, weight 2 j of the eight in bits 4 j ...
+ * 4 j + 3 and weight 2 j + 1 in bits 16 + 4 j ... 19 + 4 j; weights past K are zero bits.  mp_w4_pack brings q [N, K] (one byte
+ * each, the low four bits count; rows ldq bytes apart) into it, once, when a model is loaded. */
+int mp_w4_pack(int N, int K, const uint8_t* q, long long ldq, uint32_t* packed, void* stream);
+
+/* Y[M,N] = X[M,K] * W[N,K]^T (+ bias[N]); dtype MP_FP16 or MP_BF16 is the type of X, scales, bias and Y.  scales: [N, G] and
+ * zeros: [N, G] bytes of 0..128 (NULL: 8 everywhere), G = ceil(K / group_size); group_size: a power of two of at least 32
+ * (one of at least K gives one scale per row); K a multiple of 32.  X has rows ldx >= K elements apart, Y packed rows.
+ * fp32 sums; the bias is added to the sum before the only rounding of the result.  Up to 32 rows of X the scale multiplies
+ * fp32 sums; beyond, each weight (q - zero) * scale is rounded once to dtype, so it has to be representable there. */
+int mp_linear_w4(int dtype, int M, int N, int K, const void* X, long long ldx, const uint32_t* packed, const void* scales,
+                 const uint8_t* zeros, int group_size, const void* bias, void* Y, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dX[M,K] = dY[M,N] * W[N,K]: what a frozen 4-bit Linear hands back.  Rows of dY lddy >= N elements apart, dX packed. */
+int mp_linear_w4_grad_input(int dtype, int M, int N, int K, const void* dY, long long lddy, const uint32_t* packed, const void* scales,
+                            const uint8_t* zeros, int group_size, void* dX, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that mp_linear_w4 (grad_input = 0) or mp_linear_w4_grad_input (1) needs; X (or dY) is only looked at for
+ * its alignment.  256-byte aligned device memory, not initialised, not shared by calls or graph replays that can overlap. */
+int mp_linear_w4_workspace(int M, int N, int K, const void* X, long long ldx, int grad_input, size_t* bytes);
+
 /* Linear with softmax cross entropy (no counterpart in the reference): the output layer of a language model and its
  * loss, without holding the logits.  z[M,V] = X[M,H] * W[V,H]^T with fp32 accumulation; for every row
  *   lse[m]  = log(sum over v of exp(z[m,v]))

@@ -1,0 +1,224 @@
+// Linear with 4-bit weights (mp_w4_pack, mp_linear_w4, mp_linear_w4_grad_input): argument checks, choice of the kernel,
+// workspaces, launches.  The kernels and the packed format are in mp_w4.cuh.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/moonpoly_abi.h"
+#include "mp_host.h"
+#include "mp_w4.cuh"
+
+namespace {
+
+using namespace mp;
+
+size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+constexpr int kW4StreamMaxTokens = 32;
+constexpr int kSmsModel = 148;            // workspace sizes must not depend on the device that is asked
+
+struct Plan {
+  bool stream;
+  int bn, tiles_m, tiles_n, steps, split, steps_per_split;
+  size_t copy, partial, total;            // workspace: aligned copy of the tokens, partial sums
+  long long ld_copy, ld_partial;
+};
+
+bool tokens_aligned(const void* x, long long ld) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld % 8 == 0; }
+
+// rows = output features of this direction, contraction = input features.
+Plan w4_plan(int T, int N, int K, bool grad, bool copy_tokens) {
+  Plan p{};
+  const int rows = grad ? K : N, contraction = grad ? N : K;
+  p.stream = !grad && T <= kW4StreamMaxTokens;
+  if (copy_tokens) {
+    p.ld_copy = (long long)round_up((size_t)contraction, 8);
+    p.copy = p.total;
+    p.total += round_up((size_t)T * p.ld_copy * 2, 256);
+  }
+  if (p.stream) return p;
+  p.bn = T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+  p.tiles_m = ceil_div(rows, kPairRows);
+  p.tiles_n = ceil_div(T, p.bn);
+  p.steps = ceil_div(contraction, 128);
+  // few tiles: cut the contraction so that every pair of SMs has work, in pieces of at least four steps
+  const int tiles = p.tiles_m * p.tiles_n, pairs = kSmsModel / 2;
+  int split = std::max(1, std::min(pairs / std::max(tiles, 1), p.steps / 4));
+  p.steps_per_split = ceil_div(p.steps, split);
+  p.split = ceil_div(p.steps, p.steps_per_split);
+  if (p.split > 1) {
+    p.ld_partial = (long long)round_up((size_t)rows, 32);
+    p.partial = p.total;
+    p.total += round_up((size_t)p.split * T * p.ld_partial * 4, 256);
+  }
+  return p;
+}
+
+int check_args(const char* op, int dtype, int M, int N, int K, const void* x, long long ldx, int width, const uint32_t* packed,
+               const void* scales, int group_size) {
+  if (dtype != MP_FP16 && dtype != MP_BF16) return host_fail(MP_ERR_INVALID_ARG, "%s: dtype must be MP_FP16 or MP_BF16", op);
+  if (M < 0 || N <= 0 || K <= 0 || M > (1 << 28) || N > (1 << 28) || K > (1 << 28))
+    return host_fail(MP_ERR_INVALID_ARG, "%s: needs M >= 0, N > 0, K > 0, none above 2^28 (got %d, %d, %d)", op, M, N, K);
+  if (K % 32 != 0) return host_fail(MP_ERR_UNALIGNED_K, "%s: K = %d is not a multiple of 32", op, K);
+  if (group_size < 32 || (group_size & (group_size - 1)) != 0)
+    return host_fail(MP_ERR_INVALID_ARG, "%s: group_size %d is not a power of two of at least 32", op, group_size);
+  if (ldx < width) return host_fail(MP_ERR_INVALID_ARG, "%s: row stride %lld below the row's %d elements", op, ldx, width);
+  if (packed == nullptr || scales == nullptr || (M > 0 && x == nullptr)) return host_fail(MP_ERR_INVALID_ARG, "%s: null pointer", op);
+  if (reinterpret_cast<uintptr_t>(packed) & 15) return host_fail(MP_ERR_INVALID_ARG, "%s: the packed weight must be 16-byte aligned", op);
+  return MP_OK;
+}
+
+W4Weight weight_of(int N, int K, const uint32_t* packed, const void* scales, const uint8_t* zeros, int group_size) {
+  W4Weight w{};
+  w.packed = reinterpret_cast<const uint4*>(packed);
+  w.scale = reinterpret_cast<const uint16_t*>(scales);
+  w.zero = zeros;
+  w.N = N; w.K = K;
+  w.blocks = ceil_div(K, 128);
+  w.groups = ceil_div(K, group_size);
+  for (w.shift = 0; (32 << w.shift) < group_size; ++w.shift) {}
+  return w;
+}
+
+template <bool BF16, int RT, int NT>
+int launch_stream(const W4StreamParams& p, cudaStream_t stream) {
+  const int grid = ceil_div(p.w.N, RT * 16);
+  if (p.w.shift >= 2) w4_stream_kernel<BF16, RT, NT, false><<<grid, 256, 0, stream>>>(p);
+  else w4_stream_kernel<BF16, RT, NT, true><<<grid, 256, 0, stream>>>(p);
+  MP_HOST_CUDA_TRY(cudaGetLastError());
+  host_count_launches(1);
+  return MP_OK;
+}
+
+template <bool BF16>
+int run_stream(const W4StreamParams& p, cudaStream_t stream) {
+  const bool tall = p.w.N >= 32 * 2 * kSmsModel;           // 32 rows per CTA still give two CTAs per SM
+  if (p.T <= 8) return tall ? launch_stream<BF16, 2, 1>(p, stream) : launch_stream<BF16, 1, 1>(p, stream);
+  if (p.T <= 16) return tall ? launch_stream<BF16, 2, 2>(p, stream) : launch_stream<BF16, 1, 2>(p, stream);
+  return tall ? launch_stream<BF16, 2, 4>(p, stream) : launch_stream<BF16, 1, 4>(p, stream);
+}
+
+template <bool BF16>
+int run_pair(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, int T, const void* x, long long ldx, const void* bias,
+             void* out, uint8_t* ws, cudaStream_t stream) {
+  W4PairParams p{};
+  p.w = w;
+  p.grad = grad;
+  p.rows = grad ? w.K : w.N;
+  p.T = T;
+  p.steps = l.steps;
+  p.tiles_m = l.tiles_m; p.tiles_n = l.tiles_n; p.bn = l.bn;
+  p.split = l.split; p.steps_per_split = l.steps_per_split;
+  p.out = reinterpret_cast<uint16_t*>(out);
+  p.ldo = p.rows;
+  p.bias = reinterpret_cast<const uint16_t*>(bias);
+  p.partial = reinterpret_cast<float*>(ws + l.partial);
+  p.ld_partial = l.ld_partial;
+  p.status = d.status;
+  p.stage_bytes = kW4ABytes + l.bn / 2 * 256;
+  p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - 512 - kW4RawSlots * kW4RawBytes) / p.stage_bytes);
+  const int contraction = grad ? w.N : w.K, hb = l.bn / 2;
+  CUtensorMap tmB, tmW;
+  p.b_wide = contraction % 64 == 0;
+  if (p.b_wide) {
+    if (int rc = host_tmap_blocks(&tmB, x, contraction, T, ldx * 2, hb, 2)) return rc;
+  } else {
+    if (int rc = host_tmap(&tmB, kTmap16, x, contraction, T, ldx * 2, 64, hb, 128)) return rc;
+  }
+  if (int rc = host_tmap(&tmW, kTmapByte, w.packed, (long long)w.blocks * 64, w.N, (long long)w.blocks * 64, 64, 128, 64)) return rc;
+  auto kern = w4_pair_kernel<BF16>;
+  static bool ready[64] = {};
+  if (!ready[d.index & 63]) {
+    MP_HOST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    ready[d.index & 63] = true;
+  }
+  const int pairs = std::max(1, std::min(p.tiles_m * p.tiles_n * p.split, d.sms / 2));
+  kern<<<2 * pairs, kW4Threads, kPairSmem, stream>>>(tmB, tmW, p);
+  MP_HOST_CUDA_TRY(cudaGetLastError());
+  host_count_launches(1);
+  if (p.split > 1) {
+    // the grid's y extent ends at 65535: a split only happens with few tokens (at most 74 tiles of 256)
+    w4_reduce_kernel<BF16><<<dim3((unsigned)ceil_div(p.rows, 256), (unsigned)T), 256, 0, stream>>>(p.partial, p.split, T, p.rows,
+                                                                                                  p.ld_partial, p.bias, p.out, p.ldo);
+    MP_HOST_CUDA_TRY(cudaGetLastError());
+    host_count_launches(1);
+  }
+  return MP_OK;
+}
+
+int run_w4(const char* op, bool grad, int dtype, int M, int N, int K, const void* X, long long ldx, const uint32_t* packed, const void* scales,
+           const uint8_t* zeros, int group_size, const void* bias, void* out, void* workspace, size_t workspace_bytes, void* stream_) {
+  const int width = grad ? N : K;
+  if (int rc = check_args(op, dtype, M, N, K, X, ldx, width, packed, scales, group_size)) return rc;
+  if (M == 0) return MP_OK;
+  if (out == nullptr) return host_fail(MP_ERR_INVALID_ARG, "%s: null output", op);
+  const bool copy = !tokens_aligned(X, ldx);
+  const Plan l = w4_plan(M, N, K, grad, copy);
+  if (l.total > 0) {
+    if (workspace == nullptr || workspace_bytes < l.total)
+      return host_fail(MP_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", op, workspace ? workspace_bytes : (size_t)0, l.total);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255) return host_fail(MP_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", op);
+  }
+  HostDevice d;
+  if (int rc = host_device(&d)) return rc;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  if (copy) {
+    if (int rc = host_pad_rows16(X, ldx, ws + l.copy, M, width, (int)l.ld_copy, stream)) return rc;
+    X = ws + l.copy;
+    ldx = l.ld_copy;
+  }
+  const W4Weight w = weight_of(N, K, packed, scales, zeros, group_size);
+  if (l.stream) {
+    W4StreamParams p{};
+    p.w = w;
+    p.X = reinterpret_cast<const uint16_t*>(X); p.ldx = ldx;
+    p.Y = reinterpret_cast<uint16_t*>(out); p.ldy = N;
+    p.bias = reinterpret_cast<const uint16_t*>(bias);
+    p.T = M;
+    return dtype == MP_BF16 ? run_stream<true>(p, stream) : run_stream<false>(p, stream);
+  }
+  return dtype == MP_BF16 ? run_pair<true>(d, l, w, grad, M, X, ldx, bias, out, ws, stream)
+                          : run_pair<false>(d, l, w, grad, M, X, ldx, bias, out, ws, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mp_w4_pack(int N, int K, const uint8_t* q, long long ldq, uint32_t* packed, void* stream) {
+  if (N < 0 || K < 0 || ldq < K) return host_fail(MP_ERR_INVALID_ARG, "mp_w4_pack: needs N >= 0, K >= 0, ldq >= K");
+  if (N == 0 || K == 0) return MP_OK;
+  if (q == nullptr || packed == nullptr) return host_fail(MP_ERR_INVALID_ARG, "mp_w4_pack: null pointer");
+  HostDevice d;
+  if (int rc = host_device(&d)) return rc;
+  const int blocks = ceil_div(K, 128);
+  const long long words = (long long)N * blocks * 16;
+  w4_pack_kernel<<<(unsigned)std::min<long long>((words + 255) / 256, d.sms * 16), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      q, ldq, packed, N, K, blocks);
+  MP_HOST_CUDA_TRY(cudaGetLastError());
+  host_count_launches(1);
+  return MP_OK;
+}
+
+int mp_linear_w4_workspace(int M, int N, int K, const void* X, long long ldx, int grad_input, size_t* bytes) {
+  if (bytes == nullptr || M < 0 || N <= 0 || K <= 0) return host_fail(MP_ERR_INVALID_ARG, "mp_linear_w4_workspace: needs M >= 0, N > 0, K > 0 and a result pointer");
+  *bytes = M == 0 ? 0 : w4_plan(M, N, K, grad_input != 0, !tokens_aligned(X, ldx)).total;
+  return MP_OK;
+}
+
+int mp_linear_w4(int dtype, int M, int N, int K, const void* X, long long ldx, const uint32_t* packed, const void* scales,
+                 const uint8_t* zeros, int group_size, const void* bias, void* Y, void* workspace, size_t workspace_bytes, void* stream) {
+  return run_w4("mp_linear_w4", false, dtype, M, N, K, X, ldx, packed, scales, zeros, group_size, bias, Y, workspace, workspace_bytes, stream);
+}
+
+int mp_linear_w4_grad_input(int dtype, int M, int N, int K, const void* dY, long long lddy, const uint32_t* packed, const void* scales,
+                            const uint8_t* zeros, int group_size, void* dX, void* workspace, size_t workspace_bytes, void* stream) {
+  return run_w4("mp_linear_w4_grad_input", true, dtype, M, N, K, dY, lddy, packed, scales, zeros, group_size, nullptr, dX, workspace,
+                workspace_bytes, stream);
+}
+
+}  // extern "C"

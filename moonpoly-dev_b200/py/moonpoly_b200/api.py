@@ -84,6 +84,10 @@ def lib() -> ctypes.CDLL:
         L.mp_linear_xent_workspace.argtypes = xent + [ci, ctypes.POINTER(sz)]
         L.mp_linear_xent.argtypes = xent + [vp, ci, ll, vp, vp, vp, sz, vp]
         L.mp_linear_xent_grad.argtypes = xent + [vp, ci, ll, vp, vp, vp, vp, vp, sz, vp]
+        L.mp_w4_pack.argtypes = [ci, ci, vp, ll, vp, vp]
+        L.mp_linear_w4_workspace.argtypes = [ci, ci, ci, vp, ll, ci, ctypes.POINTER(sz)]
+        L.mp_linear_w4.argtypes = [ci, ci, ci, ci, vp, ll, vp, vp, vp, ci, vp, vp, vp, sz, vp]
+        L.mp_linear_w4_grad_input.argtypes = [ci, ci, ci, ci, vp, ll, vp, vp, vp, ci, vp, vp, sz, vp]
         _lib = L
     return _lib
 
@@ -412,6 +416,97 @@ def scaled_int8_mm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_s
                                  _ptr(b_scales), int(b_scales.numel() == 1), _ptr(bias), _ptr(out), N,
                                  0 if out_dtype == torch.float16 else 1, _stream(a)))
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# Linear with 4-bit weights (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------------
+def pack_w4(q: torch.Tensor) -> torch.Tensor:
+    """q [N, K] uint8 of values 0..15 -> the packed weight of `linear_w4`, int32 [N, 16 * ceil(K / 128)] (the bit layout
+    is in moonpoly_abi.h).  Once per weight, when a model is loaded."""
+    if q.dim() != 2 or q.dtype != torch.uint8 or not q.is_cuda:
+        raise ValueError("q must be a 2-D CUDA uint8 tensor [N, K]")
+    N, K = q.shape
+    with torch.cuda.device(q.device):
+        q, ldq = _rows(q)
+        out = torch.empty((N, (K + 127) // 128 * 16), dtype=torch.int32, device=q.device)
+        _check(lib().mp_w4_pack(N, K, _ptr(q), ldq, _ptr(out), _stream(q)))
+    return out
+
+
+def _w4_checks(op: str, x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros, group_size: int, width: str, K: int):
+    if x.dim() != 2 or qweight.dim() != 2:
+        raise ValueError(f"{op}: input and packed weight must be 2-D tensors")
+    code = _dtype16(x, op)
+    N = qweight.shape[0]
+    if qweight.dtype != torch.int32 or qweight.shape[1] != (K + 127) // 128 * 16 or N == 0 or K == 0:
+        raise ValueError(f"{op}: the packed weight must be int32 [N, 16 * ceil(K / 128)]")
+    if x.shape[1] != (K if width == "K" else N):
+        raise ValueError(f"{op}: input must be [M, {width}]")
+    if K % 32:
+        raise ValueError(f"{op}: K = {K} must be a multiple of 32")
+    if group_size == -1:                                   # one group per row
+        group_size = 32
+        while group_size < K:
+            group_size *= 2
+    if group_size < 32 or group_size & (group_size - 1):
+        raise ValueError(f"{op}: group_size must be a power of two of at least 32, or -1")
+    shape = (N, (K + group_size - 1) // group_size)
+    if scales.dtype != x.dtype or tuple(scales.shape) != shape:
+        raise ValueError(f"{op}: scales must be {list(shape)} in the input dtype")
+    if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != shape):
+        raise ValueError(f"{op}: zeros must be {list(shape)} uint8")
+    for t in (x, qweight, scales, zeros):
+        if t is not None and (not t.is_cuda or t.device != x.device):
+            raise ValueError(f"{op}: all tensors must be CUDA tensors on one device")
+    qweight = qweight.contiguous()
+    if qweight.data_ptr() & 15:                            # a view off the 16 bytes the loads want
+        qweight = qweight.clone()
+    return code, N, group_size, qweight, scales.contiguous(), None if zeros is None else zeros.contiguous()
+
+
+def _w4_workspace(M, N, K, x, ldx, grad) -> torch.Tensor:
+    need = ctypes.c_size_t()
+    _check(lib().mp_linear_w4_workspace(M, N, K, _ptr(x), ldx, grad, ctypes.byref(need)))
+    return torch.empty((need.value,), dtype=torch.uint8, device=x.device) if need.value else None
+
+
+def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+              group_size: int = 128, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Y[M,N] = x[M,K] @ W[N,K]^T (+ bias[N]) with W[n,k] = (q[n,k] - zero[n, k // group_size]) * scale[n, k // group_size],
+    qweight from `pack_w4`, scales [N, ceil(K / group_size)] in the type of x (fp16 or bf16), zeros the same shape in uint8
+    (values 0..128; None: 8 everywhere).  group_size is a power of two of at least 32, or -1 for one group per row.  The
+    bias is added before the only rounding of the result."""
+    K = x.shape[1] if x.dim() == 2 else 0
+    code, N, group_size, qweight, scales, zeros = _w4_checks("linear_w4", x, qweight, scales, zeros, group_size, "K", K)
+    M = x.shape[0]
+    if bias is not None:
+        if bias.dtype != x.dtype or bias.numel() != N or bias.device != x.device:
+            raise ValueError("bias must be a CUDA tensor of N elements in the input dtype")
+        bias = bias.contiguous()
+    with torch.cuda.device(x.device):
+        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        x, ldx = _rows(x)
+        ws = _w4_workspace(M, N, K, x, ldx, 0)
+        _check(lib().mp_linear_w4(code, M, N, K, _ptr(x), ldx, _ptr(qweight), _ptr(scales), _ptr(zeros), group_size, _ptr(bias),
+                                  _ptr(y), _ptr(ws), 0 if ws is None else ws.numel(), _stream(x)))
+    return y
+
+
+def linear_w4_grad_input(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+                         group_size: int = 128, in_features: Optional[int] = None) -> torch.Tensor:
+    """dX[M,K] = dy[M,N] @ W[N,K], the gradient that `linear_w4` with a frozen weight hands back.  in_features is K where it
+    is not a multiple of 128 (the packed rows are padded to 128)."""
+    K = qweight.shape[1] * 8 if in_features is None else int(in_features)
+    code, N, group_size, qweight, scales, zeros = _w4_checks("linear_w4_grad_input", dy, qweight, scales, zeros, group_size, "N", K)
+    M = dy.shape[0]
+    with torch.cuda.device(dy.device):
+        dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
+        dy, ld = _rows(dy)
+        ws = _w4_workspace(M, N, K, dy, ld, 1)
+        _check(lib().mp_linear_w4_grad_input(code, M, N, K, _ptr(dy), ld, _ptr(qweight), _ptr(scales), _ptr(zeros), group_size,
+                                             _ptr(dx), _ptr(ws), 0 if ws is None else ws.numel(), _stream(dy)))
+    return dx
 
 
 # ------------------------------------------------------------------------------------------------

@@ -14,7 +14,7 @@
 // epilogue (TMEM lane quadrant = warp % 4, two warps per quadrant taking the two halves of the columns).
 // Barriers: full[s] lives in rank 0 and counts the bytes of both CTAs; empty[s] and tfull[b] exist in both CTAs and are
 // signalled by multicast commits; tempty[b] lives in rank 0 and takes the arrivals of the 16 epilogue warps of the pair.
-// No TMA load uses cluster multicast.  Every wait is bounded (mbar_wait*), as in mp_umma_gemm.cuh.
+// No TMA load uses cluster multicast.  Every wait is bounded (mbar_wait), as in mp_umma_gemm.cuh.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -83,6 +83,12 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst_smem, const CUtens
       " [%0], [%1, {%3, %4, %5}], [%2];"
       ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tm)), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
+}
+// Arrive on a barrier of either CTA of the pair, default semantics: what is handed over is read or written by the tensor
+// cores and TMA only, and is ordered by tcgen05 fences or a proxy fence before the arrival.  The cluster-scope release that
+// plain memory would need costs a fence each time.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
@@ -358,7 +364,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         const int a0 = u.tm * kPairRows + (int)rank * 128, b0 = u.tn * q.bn + (int)rank * hb;
         const uint32_t a_bytes = (uint32_t)(p.kc * kPairABytes), tx = 2u * (a_bytes + (uint32_t)(p.kc * hb * 128));   // both CTAs
         for (int kb = 0; kb < q.kblocks; kb += p.kc) {
-          if (!mbar_wait_cluster(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
           const uint32_t dst = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), tx);
           const uint32_t bar = mapa_shared(full_bar(s), 0);
@@ -369,7 +375,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
       }
       // every stage handed back: all copies have landed and all commits have reached this CTA's barriers
       for (int i = 0; ok && i < stages; ++i) {
-        ok = mbar_wait_cluster(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_DRAIN);
+        ok = mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_DRAIN);
         if (++s == stages) { s = 0; ph ^= 1u; }
       }
       if (!ok) settle_copies();
@@ -396,13 +402,13 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         const int chunk = EPI == PAIR_LSE ? kLseChunk : q.kblocks;
         for (int k0 = 0; ok && k0 < q.kblocks; k0 += chunk, ++ui) {
         const uint32_t buf = ui & 1u, use = ui >> 1;
-        if (!mbar_wait_cluster(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
+        if (!mbar_wait(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * (uint32_t)kPairMaxBN;
         const int k1 = min(q.kblocks, k0 + chunk);
         uint32_t first = 0u;
         for (int kb = k0; kb < k1; kb += p.kc) {
-          if (!mbar_wait_cluster(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+          if (!mbar_wait(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
           tc_fence_after();
           uint64_t ad = a_base + (uint64_t)((uint32_t)s * stage16), bd = b_base + (uint64_t)((uint32_t)s * stage16);
           const int nc = min(p.kc, k1 - kb);
@@ -438,7 +444,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         for (int j = 0; j < 128; ++j) z[j] = 0.0f;
         for (int k0 = 0; ok && k0 < q.kblocks; k0 += kLseChunk, ++ui) {
           const uint32_t buf = ui & 1u, use = ui >> 1;
-          if (!mbar_wait_cluster(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
+          if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -451,19 +457,19 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar((int)buf), 0));
+          if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));
         }
         if (ok) pair_epilogue_lse(p, q, z, row, c_begin, u.tn, half, ncols);
       } else {
         const uint32_t buf = ui & 1u, use = ui >> 1;
-        if (!mbar_wait_cluster(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
+        if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
         tc_fence_after();
         const uint32_t t_addr = t_half + buf * (uint32_t)kPairMaxBN;
         if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols);
         else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar((int)buf), 0));
+        if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));
         ++ui;
       }
     }

@@ -119,7 +119,11 @@ int run_pair(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, i
   p.ld_partial = l.ld_partial;
   p.status = d.status;
   p.stage_bytes = kW4ABytes + l.bn / 2 * 256;
-  p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - 512 - kW4RawSlots * kW4RawBytes) / p.stage_bytes);
+  // three stages, and the rest of the shared memory for packed bytes on their way from HBM
+  p.stages = 3;
+  p.raw_slots = std::min(kW4MaxRawSlots, (kPairSmem - 1024 - 512 - p.stages * p.stage_bytes) / kW4RawBytes);
+  p.vec = w.shift < 2 && w.groups % (4 >> w.shift) == 0 && (reinterpret_cast<uintptr_t>(w.scale) & 7) == 0 &&
+          (reinterpret_cast<uintptr_t>(w.zero) & 3) == 0;
   const int contraction = grad ? w.N : w.K, hb = l.bn / 2;
   CUtensorMap tmB, tmW;
   p.b_wide = contraction % 64 == 0;
@@ -129,21 +133,30 @@ int run_pair(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, i
     if (int rc = host_tmap(&tmB, kTmap16, x, contraction, T, ldx * 2, 64, hb, 128)) return rc;
   }
   if (int rc = host_tmap(&tmW, kTmapByte, w.packed, (long long)w.blocks * 64, w.N, (long long)w.blocks * 64, 64, 128, 64)) return rc;
-  auto kern = w4_pair_kernel<BF16>;
-  static bool ready[64] = {};
-  if (!ready[d.index & 63]) {
+  const bool fine = w.shift < 2;
+  auto kern = fine ? w4_pair_kernel<BF16, true> : w4_pair_kernel<BF16, false>;
+  static bool ready[64][2] = {};
+  if (!ready[d.index & 63][fine]) {
     MP_HOST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-    ready[d.index & 63] = true;
+    ready[d.index & 63][fine] = true;
   }
   const int pairs = std::max(1, std::min(p.tiles_m * p.tiles_n * p.split, d.sms / 2));
   kern<<<2 * pairs, kW4Threads, kPairSmem, stream>>>(tmB, tmW, p);
   MP_HOST_CUDA_TRY(cudaGetLastError());
   host_count_launches(1);
   if (p.split > 1) {
-    // the grid's y extent ends at 65535: a split only happens with few tokens (at most 74 tiles of 256)
-    w4_reduce_kernel<BF16><<<dim3((unsigned)ceil_div(p.rows, 256), (unsigned)T), 256, 0, stream>>>(p.partial, p.split, T, p.rows,
-                                                                                                  p.ld_partial, p.bias, p.out, p.ldo);
-    MP_HOST_CUDA_TRY(cudaGetLastError());
+    const long long threads = (long long)T * (l.ld_partial / 4);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((threads + 255) / 256));
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = host_use_pdl() ? 1 : 0;
+    MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&cfg, w4_reduce_kernel<BF16>, (const float*)p.partial, p.split, T, p.rows, p.ld_partial, p.bias,
+                                        p.out, p.ldo));
     host_count_launches(1);
   }
   return MP_OK;

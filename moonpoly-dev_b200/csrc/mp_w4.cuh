@@ -45,15 +45,17 @@ __device__ __forceinline__ uint32_t fma2_f16(uint32_t a, uint32_t b, uint32_t c)
   return d;
 }
 
-// What unpacking needs to know of a zero point z: 128 + z (bf16) or 1024 + z and -(64 + z) (fp16), in both halves.
+// What unpacking needs to know of a zero point z (0..128): 128 + z (bf16) or 1024 + z and -(64 + z) (fp16), in both halves.
+// Whole numbers this small sit in the mantissa: 128 + z is 0x4300 + z up to 255, 1024 + z is 0x6400 + z, and 64 + z is
+// 0x5400 + 16 z while below 128 (z < 64) and 0x5800 + 8 (z - 64) from there.
 struct W4Zero { uint32_t a, b; };
-template <bool BF16> __device__ __forceinline__ W4Zero w4_zero(int z) {
+template <bool BF16> __device__ __forceinline__ W4Zero w4_zero(uint32_t z) {
   if constexpr (BF16) {
-    const uint32_t a = __bfloat16_as_ushort(__float2bfloat16_rn((float)(128 + z)));   // exact up to 256
-    return {a * 0x10001u, (uint32_t)z};
+    // 256 (z = 128) is the next binade's first number, 0x4380, where the addition arrives by itself
+    return {(0x4300u + z) * 0x10001u, 0u};
   } else {
-    const uint32_t a = __half_as_ushort(__float2half_rn((float)(1024 + z))), b = __half_as_ushort(__float2half_rn((float)(-64 - z)));
-    return {a * 0x10001u, b * 0x10001u};
+    const uint32_t b = z < 64u ? 0xd400u + 16u * z : 0xd800u + 8u * (z - 64u);
+    return {(0x6400u + z) * 0x10001u, b * 0x10001u};
   }
 }
 // The 8 weights of a word as q - zero: out[j] = weights 2 j and 2 j + 1.
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(256) w4_stream_kernel(const W4StreamParams p) 
           uint32_t a[2][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int z = w.zero != nullptr ? (int)__ldg(w.zero + (size_t)rows[r][h] * w.groups + gi) : 8;
+            const uint32_t z = w.zero != nullptr ? (uint32_t)__ldg(w.zero + (size_t)rows[r][h] * w.groups + gi) : 8u;
             const uint4 q = cur[u][r][h];
             w4_unpack<BF16>(i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w, w4_zero<BF16>(z), a[h]);
           }
@@ -230,10 +232,12 @@ __global__ void __launch_bounds__(256) w4_stream_kernel(const W4StreamParams p) 
 // A stage is 128 contraction elements: 32 KB of unpacked weight and bn / 2 token rows per CTA.  Both directions unpack the
 // same thing -- 128 rows of W by one block of 128 k -- into the same swizzled lines of 64 k; forward, the lines are a K-major
 // operand (line = row of D), in the gradient an MN-major one (line = contraction index).
-// Warps: 0 = TMA of the tokens, 1 = MMA, 2 = TMA of the packed weight, 4..7 = epilogue, 8..15 = unpacking.
-constexpr int kW4Threads = 512;
+// Warps: 0 = TMA of the tokens, 1 = MMA, 2 = TMA of the packed weight, 4..7 = epilogue, 8..15 and 16..23 = unpacking, two
+// groups that take alternate stages: a stage's chain (packed bytes, conversion, stores, proxy fence, arrival) lasts about
+// 1600 cycles and its MMAs 1024.
+constexpr int kW4Threads = 768;
 constexpr int kW4RawBytes = 128 * 64;         // packed bytes per stage and CTA
-constexpr int kW4RawSlots = 4;
+constexpr int kW4MaxRawSlots = 12;
 constexpr int kW4ABytes = 128 * 256;
 
 struct W4PairParams {
@@ -242,7 +246,8 @@ struct W4PairParams {
   int rows, T, steps;           // rows of D, tokens, contraction steps of 128
   int tiles_m, tiles_n, bn, split, steps_per_split;
   int b_wide;
-  int stages, stage_bytes;
+  int stages, stage_bytes, raw_slots;
+  int vec;                      // the scales (and zeros) of a block's runs are read in one load each
   uint16_t* out; long long ldo; // out[token][row]
   const uint16_t* bias;
   float* partial;               // split > 1: [split][T][rows_pad]
@@ -263,13 +268,23 @@ __device__ __forceinline__ W4Unit w4_unit(const W4PairParams& p, int unit) {
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ uint4 ld_smem_v4(uint32_t addr) {
+template <int OFF> __device__ __forceinline__ uint4 ld_smem_v4(uint32_t addr) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4+%5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "n"(OFF) : "memory");
   return v;
 }
+template <int OFF> __device__ __forceinline__ void st_smem_v4(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0+%5], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "n"(OFF) : "memory");
+}
+// The 8 weights of a word.
+template <bool BF16> __device__ __forceinline__ uint4 w4_weights(uint32_t word, const W4Zero& zero, uint32_t scale) {
+  uint32_t v[4];
+  w4_unpack<BF16>(word, zero, v);
+  return make_uint4(mul2<BF16>(v[0], scale), mul2<BF16>(v[1], scale), mul2<BF16>(v[2], scale), mul2<BF16>(v[3], scale));
+}
 
-template <bool BF16>
+// FINE: groups of 32 or 64, so the runs of a block have scales of their own.
+template <bool BF16, bool FINE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
 w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmW, const W4PairParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -277,14 +292,15 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
   const uint32_t smem_base = smem_u32(smem);
   const int stages = p.stages;
   const uint32_t raw_base = smem_base + (uint32_t)stages * (uint32_t)p.stage_bytes;
-  const uint32_t bar_base = raw_base + kW4RawSlots * kW4RawBytes;
+  const int raw_slots = p.raw_slots;
+  const uint32_t bar_base = raw_base + (uint32_t)raw_slots * kW4RawBytes;
   auto full_bar = [&](int s) { return bar_base + 8u * (uint32_t)s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (uint32_t)(stages + s); };
   auto tfull_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + b); };
   auto tempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 2 + b); };
   auto rfull_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 4 + b); };
-  auto rempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 4 + kW4RawSlots + b); };
-  const uint32_t slot_off = (uint32_t)stages * (uint32_t)p.stage_bytes + kW4RawSlots * kW4RawBytes + 8u * (uint32_t)(2 * stages + 4 + 2 * kW4RawSlots);
+  auto rempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 4 + raw_slots + b); };
+  const uint32_t slot_off = bar_base - smem_base + 8u * (uint32_t)(2 * stages + 4 + 2 * raw_slots);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + slot_off);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -294,9 +310,9 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
   int* status = p.status;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 17); mbar_init(empty_bar(s), 1); }   // 1 + 8 unpacking warps of each CTA
+    for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 17); mbar_init(empty_bar(s), 1); }   // 1 + 8 unpacking warps per CTA
     for (int b = 0; b < 2; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), 8); }
-    for (int b = 0; b < kW4RawSlots; ++b) { mbar_init(rfull_bar(b), 1); mbar_init(rempty_bar(b), 8); }
+    for (int b = 0; b < raw_slots; ++b) { mbar_init(rfull_bar(b), 1); mbar_init(rempty_bar(b), 8); }
     mbar_fence_init();
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmW);
@@ -307,6 +323,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   cluster_sync_all();
+  griddep_launch_dependents();
 
   const int hb = p.bn >> 1;
   if (warp == 0) {
@@ -319,14 +336,14 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
         const W4Unit u = w4_unit(p, unit);
         const int b0 = u.tn * p.bn + (int)rank * hb;
         for (int st = u.s0; st < u.s1; ++st) {
-          if (!mbar_wait_cluster(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2u * (uint32_t)(hb * 256));
           pair_load(smem_base + (uint32_t)s * (uint32_t)p.stage_bytes + kW4ABytes, &tmB, mapa_shared(full_bar(s), 0), 0, p.b_wide, hb, b0, st * 2, 2);
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
       }
       for (int i = 0; ok && i < stages; ++i) {
-        ok = mbar_wait_cluster(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_DRAIN);
+        ok = mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_DRAIN);
         if (++s == stages) { s = 0; ph ^= 1u; }
       }
       if (!ok) settle_copies();
@@ -344,11 +361,11 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
       for (int unit = pair; ok && unit < units; unit += pairs, ++ui) {
         const W4Unit u = w4_unit(p, unit);
         const uint32_t buf = ui & 1u, use = ui >> 1;
-        if (!mbar_wait_cluster(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
+        if (!mbar_wait(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * (uint32_t)kPairMaxBN;
         for (int st = u.s0; st < u.s1; ++st) {
-          if (!mbar_wait_cluster(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+          if (!mbar_wait(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
           tc_fence_after();
           const uint64_t ad = a_base + (uint64_t)((uint32_t)s * stage16), bd = b_base + (uint64_t)((uint32_t)s * stage16);
 #pragma unroll
@@ -378,7 +395,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
           const int blk = p.grad ? u.tm * 2 + (int)rank : st;
           const int row = p.grad ? st * 128 : u.tm * kPairRows + (int)rank * 128;
           tma_load_2d(raw_base + (uint32_t)rs * kW4RawBytes, &tmW, rfull_bar(rs), blk * 64, row);
-          if (++rs == kW4RawSlots) { rs = 0; rph ^= 1u; }
+          if (++rs == raw_slots) { rs = 0; rph ^= 1u; }
         }
       }
       if (!ok) settle_copies();
@@ -387,68 +404,99 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
     // -------------------------------------------------------------------------------------------------------- unpacking
     // a lane takes the 16-byte chunk t of two rows 8 apart: eight neighbouring lanes are eight rows, which the 64-byte
     // swizzle of the packed tile and the 128-byte swizzle of the operand both spread over all banks
-    const int r0 = (warp - 8) * 16 + (lane & 7), t = lane >> 3;
-    int s = 0, rs = 0;
+    const int group = (warp - 8) >> 3, r0 = ((warp - 8) & 7) * 16 + (lane & 7), t = lane >> 3;
+    const uint32_t raw_off = raw_base + (uint32_t)(r0 * 64 + ((t ^ ((r0 >> 1) & 3)) << 4));
+    const uint32_t even_off = smem_base + (uint32_t)(r0 * 128 + ((t ^ (r0 & 7)) << 4)), odd_off = even_off ^ 64u;   // runs 0, 2 and 1, 3
+    int s = group, rs = group;                          // the host gives at least two of each
     uint32_t ph = 0, rph = 0;
-    bool ok = true;
     const W4Weight& w = p.w;
-    for (int unit = pair; ok && unit < units; unit += pairs) {
-      const W4Unit u = w4_unit(p, unit);
-      uint32_t sc[2][4], zz[2][4];
-      const auto fetch = [&](int st) {                  // scales and zeros of the step's two rows, one per 32-weight run
-        const int blk = p.grad ? u.tm * 2 + (int)rank : st;
-        const int row = (p.grad ? st * 128 : u.tm * kPairRows + (int)rank * 128) + r0;
+    constexpr int R = FINE ? 4 : 1;                     // groups that a block of a row meets
+    // This CTA pair's steps, one after the other across its units.
+    struct Step { int unit, st; W4Unit u; };
+    const auto advance = [&](Step& x) {
+      if (++x.st < x.u.s1) return;
+      x.unit += pairs;
+      if (x.unit < units) { x.u = w4_unit(p, x.unit); x.st = x.u.s0; }
+    };
+    uint32_t sz[2][R];                                  // scale | zero << 16
+    // Scales and zeros of the lane's two rows, a step ahead of their use.  Weights that do not exist (rows past N, runs past
+    // K) get scale 0: they are zero whatever their bits say.
+    const auto fetch = [&](const Step& x) {
+      const int blk = p.grad ? x.u.tm * 2 + (int)rank : x.st;
+      const int row = (p.grad ? x.st * 128 : x.u.tm * kPairRows + (int)rank * 128) + r0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        const long long line = (long long)(row + 8 * h) * w.groups;
+        const bool real = row + 8 * h < w.N;
+        if (FINE && p.vec) {
+          // groups of 32: four per block; of 64: two.  The last block of a row may have fewer, its line is still whole.
+          uint32_t s0 = 0, s1 = 0, z = 0x08080808u;
+          if (real && blk < w.blocks) {
+            if (w.shift == 0) {
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(w.scale + line + 4 * blk));
+              s0 = v.x; s1 = v.y;
+              if (w.zero != nullptr) z = __ldg(reinterpret_cast<const uint32_t*>(w.zero + line + 4 * blk));
+            } else {
+              const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(w.scale + line + 2 * blk));
+              s0 = __byte_perm(v, v, 0x1010); s1 = __byte_perm(v, v, 0x3232);
+              if (w.zero != nullptr) z = __byte_perm(__ldg(reinterpret_cast<const uint16_t*>(w.zero + line + 2 * blk)), 0, 0x1100);
+            }
+          }
+          sz[h][0] = (s0 & 0xffffu) | (z & 0xffu) << 16;
+          sz[h][1 % R] = (s0 >> 16) | (z & 0xff00u) << 8;
+          sz[h][2 % R] = (s1 & 0xffffu) | (z & 0xff0000u);
+          sz[h][3 % R] = (s1 >> 16) | (z >> 24) << 16;
+        } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (i > 0 && w.shift >= 2) { sc[h][i] = sc[h][0]; zz[h][i] = zz[h][0]; continue; }
+          for (int i = 0; i < R; ++i) {
             const int run = blk * 4 + i;
-            // weights that do not exist (rows past N, runs past K) are zero whatever their bits say
-            const bool real = row + 8 * h < w.N && run * 32 < w.K;
-            const size_t at = (size_t)(row + 8 * h) * w.groups + (run >> w.shift);
-            sc[h][i] = real ? (uint32_t)__ldg(w.scale + at) * 0x10001u : 0u;
-            zz[h][i] = real && w.zero != nullptr ? (uint32_t)__ldg(w.zero + at) : 8u;
-          }
-      };
-      fetch(u.s0);
-      for (int st = u.s0; st < u.s1; ++st) {
-        uint32_t scale[2][4], zero[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { scale[h][i] = sc[h][i]; zero[h][i] = zz[h][i]; }
-        if (st + 1 < u.s1) fetch(st + 1);
-        if (!mbar_wait(rfull_bar(rs), rph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
-        uint4 q[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = r0 + 8 * h;
-          q[h] = ld_smem_v4(raw_base + (uint32_t)rs * kW4RawBytes + (uint32_t)(r * 64 + ((t ^ ((r >> 1) & 3)) << 4)));
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(rempty_bar(rs));
-        if (++rs == kW4RawSlots) { rs = 0; rph ^= 1u; }
-        if (!mbar_wait_cluster(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
-        const uint32_t a_dst = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = r0 + 8 * h;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t v[4];
-            w4_unpack<BF16>(i == 0 ? q[h].x : i == 1 ? q[h].y : i == 2 ? q[h].z : q[h].w, w4_zero<BF16>((int)zero[h][i]), v);
-            // the weight in the operand type: one rounding of the exact product
-            const uint32_t c = mul2<BF16>(v[0], scale[h][i]), d = mul2<BF16>(v[1], scale[h][i]);
-            const uint32_t e = mul2<BF16>(v[2], scale[h][i]), f = mul2<BF16>(v[3], scale[h][i]);
-            st_smem_v4(a_dst + (uint32_t)((i >> 1) * 16384 + r * 128 + (((((i & 1) << 2) + t) ^ (r & 7)) << 4)), make_uint4(c, d, e, f));
+            const bool there = real && run * 32 < w.K;
+            const long long at = line + (run >> w.shift);
+            const uint32_t z = there && w.zero != nullptr ? (uint32_t)__ldg(w.zero + at) : 8u;
+            sz[h][i] = (there ? (uint32_t)__ldg(w.scale + at) : 0u) | z << 16;
           }
         }
-        fence_async_smem();                              // the tensor cores read through the async proxy
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(full_bar(s), 0));
-        if (++s == stages) { s = 0; ph ^= 1u; }
       }
+    };
+    Step cur{pair, 0, {}};
+    if (pair < units) {
+      cur.u = w4_unit(p, pair);
+      cur.st = cur.u.s0;
+      if (group) advance(cur);
+      if (cur.unit < units) fetch(cur);
+    }
+    while (cur.unit < units) {
+      uint32_t scale[2][R];
+      W4Zero zero[2][R];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < R; ++i) { scale[h][i] = (sz[h][i] & 0xffffu) * 0x10001u; zero[h][i] = w4_zero<BF16>(sz[h][i] >> 16); }
+      Step nxt = cur;
+      advance(nxt);
+      if (nxt.unit < units) advance(nxt);
+      if (nxt.unit < units) fetch(nxt);
+      if (!mbar_wait(rfull_bar(rs), rph, status, MP_DEV_TIMEOUT_MMA_FULL)) break;
+      const uint4 q0 = ld_smem_v4<0>(raw_off + (uint32_t)rs * kW4RawBytes), q1 = ld_smem_v4<512>(raw_off + (uint32_t)rs * kW4RawBytes);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(rempty_bar(rs));
+      if ((rs += 2) >= raw_slots) { rs -= raw_slots; rph ^= 1u; }
+      if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) break;
+      const uint32_t ev = even_off + (uint32_t)s * (uint32_t)p.stage_bytes, od = odd_off + (uint32_t)s * (uint32_t)p.stage_bytes;
+      // the weight in the operand type: one rounding of the exact product (q - zero) * scale
+      st_smem_v4<0>(ev, w4_weights<BF16>(q0.x, zero[0][0], scale[0][0]));
+      st_smem_v4<0>(od, w4_weights<BF16>(q0.y, zero[0][1 % R], scale[0][1 % R]));
+      st_smem_v4<16384>(ev, w4_weights<BF16>(q0.z, zero[0][2 % R], scale[0][2 % R]));
+      st_smem_v4<16384>(od, w4_weights<BF16>(q0.w, zero[0][3 % R], scale[0][3 % R]));
+      st_smem_v4<1024>(ev, w4_weights<BF16>(q1.x, zero[1][0], scale[1][0]));
+      st_smem_v4<1024>(od, w4_weights<BF16>(q1.y, zero[1][1 % R], scale[1][1 % R]));
+      st_smem_v4<17408>(ev, w4_weights<BF16>(q1.z, zero[1][2 % R], scale[1][2 % R]));
+      st_smem_v4<17408>(od, w4_weights<BF16>(q1.w, zero[1][3 % R], scale[1][3 % R]));
+      fence_async_smem();                              // the tensor cores read through the async proxy
+      __syncwarp();
+      if (lane == 0) mbar_arrive_pair(mapa_shared(full_bar(s), 0));
+      if ((s += 2) >= stages) { s -= stages; ph ^= 1u; }
+      cur = nxt;
     }
   } else if (warp >= 4) {
     // --------------------------------------------------------------------------------------------------------- epilogue
@@ -460,7 +508,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
       const int row = u.tm * kPairRows + (int)rank * 128 + quad * 32 + lane;
       const bool live = row < p.rows;
       const float bias = live && p.bias != nullptr ? from16<BF16>(p.bias[row]) : 0.0f;
-      if (!mbar_wait_cluster(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
+      if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
       const uint32_t t_addr = tmem_base + buf * (uint32_t)kPairMaxBN + ((uint32_t)(quad * 32) << 16);
       const int tok0 = u.tn * p.bn, ntok = min(p.bn, p.T - tok0);
@@ -483,7 +531,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar((int)buf), 0));
+      if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));
     }
   }
 
@@ -497,16 +545,32 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
   }
 }
 
-// out[t][row] = RN16(sum over slices, in their order, + bias).
+// out[t][row] = RN16(sum over slices, in their order, + bias); four rows per thread.  Launched so that its blocks may
+// start while the products finish; nothing is read before they have.
 template <bool BF16>
-__global__ void w4_reduce_kernel(const float* partial, int split, int T, int rows, long long ld_partial, const uint16_t* bias,
-                                 uint16_t* out, long long ldo) {
-  const int row = blockIdx.x * blockDim.x + threadIdx.x, t = blockIdx.y;
-  if (row >= rows) return;
-  float s = 0.0f;
-  for (int i = 0; i < split; ++i) s += partial[((long long)i * T + t) * ld_partial + row];
-  if (bias != nullptr) s += from16<BF16>(bias[row]);
-  out[(long long)t * ldo + row] = to16<BF16>(s);
+__global__ void __launch_bounds__(256) w4_reduce_kernel(const float* partial, int split, int T, int rows, long long ld_partial,
+                                                        const uint16_t* bias, uint16_t* out, long long ldo) {
+  griddep_wait();
+  const int quads = (int)(ld_partial >> 2);
+  const long long x = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (x >= (long long)T * quads) return;
+  const int t = (int)(x / quads), row = (int)(x - (long long)t * quads) * 4;
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < split; ++i) {
+    const float4 a = __ldcs(reinterpret_cast<const float4*>(partial + ((long long)i * T + t) * ld_partial + row));
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+  }
+  uint16_t* o = out + (long long)t * ldo + row;
+  if (bias != nullptr) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (row + e < rows) v[e] += from16<BF16>(bias[row + e]);
+  }
+  if (row + 4 <= rows && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack16(v[0], v[1], BF16), pack16(v[2], v[3], BF16));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (row + e < rows) o[e] = to16<BF16>(v[e]);
+  }
 }
 
 }  // namespace mp

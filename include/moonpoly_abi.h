@@ -76,9 +76,9 @@ int mp_linear_bias(int dtype, int M, int N, int K, const void* X, const void* W,
 int mp_w4_pack(int N, int K, const uint8_t* q, long long ldq, uint32_t* packed, void* stream);
 
 /* Y[M,N] = X[M,K] * W[N,K]^T (+ bias[N]); dtype MP_FP16 or MP_BF16 is the type of X, scales, bias and Y.  scales: [N, G] and
- * zeros: [N, G] bytes of 0..128 (NULL: 8 everywhere), G = ceil(K / group_size); group_size: a power of two of at least 32
+ * zeros: [N, G] bytes of 0..63 (NULL: 8 everywhere), G = ceil(K / group_size); group_size: a power of two of at least 32
  * (one of at least K gives one scale per row); K a multiple of 32.  X has rows ldx >= K elements apart, Y packed rows.
- * fp32 sums; the bias is added to the sum before the only rounding of the result.  Up to 32 rows of X the scale multiplies
+ * fp32 sums; the bias is added to the sum before the only rounding of the result.  Up to 16 rows of X the scale multiplies
  * fp32 sums; beyond, each weight (q - zero) * scale is rounded once to dtype, so it has to be representable there. */
 int mp_linear_w4(int dtype, int M, int N, int K, const void* X, long long ldx, const uint32_t* packed, const void* scales,
                  const uint8_t* zeros, int group_size, const void* bias, void* Y, void* workspace, size_t workspace_bytes, void* stream);

@@ -17,7 +17,7 @@ using namespace mp;
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-constexpr int kW4StreamMaxTokens = 32;
+constexpr int kW4StreamMaxTokens = 16;
 constexpr int kSmsModel = 148;            // workspace sizes must not depend on the device that is asked
 
 struct Plan {
@@ -83,22 +83,75 @@ W4Weight weight_of(int N, int K, const uint32_t* packed, const void* scales, con
   return w;
 }
 
-template <bool BF16, int RT, int NT>
-int launch_stream(const W4StreamParams& p, cudaStream_t stream) {
-  const int grid = ceil_div(p.w.N, RT * 16);
-  if (p.w.shift >= 2) w4_stream_kernel<BF16, RT, NT, false><<<grid, 256, 0, stream>>>(p);
-  else w4_stream_kernel<BF16, RT, NT, true><<<grid, 256, 0, stream>>>(p);
-  MP_HOST_CUDA_TRY(cudaGetLastError());
+// Scales (and zeros) of a block's fine groups can be read as one 8- or 4-byte word (and one 4- or 2-byte word).
+int vector_groups(const W4Weight& w) {
+  return w.shift < 2 && w.groups % (4 >> w.shift) == 0 && (reinterpret_cast<uintptr_t>(w.scale) & 7) == 0 &&
+         (reinterpret_cast<uintptr_t>(w.zero) & 3) == 0;
+}
+
+// Launch that may begin while the previous kernel of the stream ends; the kernel waits before it reads anything.
+template <typename P>
+int launch_dependent(void (*kern)(P), const P& p, int grid, int threads, size_t smem, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = host_use_pdl() ? 1 : 0;
+  MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
   host_count_launches(1);
   return MP_OK;
 }
 
+template <bool BF16, int NT, int GPB>
+int launch_stream(const HostDevice& d, const W4StreamParams& p, cudaStream_t stream) {
+  const W4Weight& w = p.w;
+  // One CTA per SM; more, in waves, where the parked sums of a share and its group words would leave no room for a ring of
+  // four blocks.  Rows with so many groups that eight waves do not do it read them from global memory.
+  constexpr size_t kBlock = (size_t)kW4StreamWarps * 1024;
+  const int one = std::min(ceil_div(w.N, 16), d.sms);
+  int ctas = one;
+  size_t sums = 0, staged = 0;
+  const auto shape = [&](int c) {
+    const int rows = ceil_div(w.N, c), tiles = ceil_div(rows, 16);
+    // shares are `rows` or `rows` - 1 long, and the shorter may be a single tile, whose sums are parked 16 times
+    sums = (size_t)std::max(tiles * 8, 16) * NT * 512;
+    staged = (size_t)rows * w.groups * 4;
+    ctas = c;
+  };
+  bool stage = false;
+  for (int waves = 1; waves <= 8 && !stage; ++waves) {
+    shape(one * waves);
+    stage = 4 * kBlock + sums + staged <= (size_t)kPairSmem;
+  }
+  if (!stage)
+    for (int waves = 1; shape(one * waves), 4 * kBlock + sums > (size_t)kPairSmem; ++waves) {}
+  const size_t fixed = sums + (stage ? staged : 0);
+  const bool deep = 8 * kBlock + fixed <= (size_t)kPairSmem;
+  auto kern = stage ? (deep ? w4_stream_kernel<BF16, NT, GPB, 8, true> : w4_stream_kernel<BF16, NT, GPB, 4, true>)
+                    : (deep ? w4_stream_kernel<BF16, NT, GPB, 8, false> : w4_stream_kernel<BF16, NT, GPB, 4, false>);
+  static bool ready[64][4] = {};
+  bool& done = ready[d.index & 63][stage * 2 + deep];
+  if (!done) {
+    MP_HOST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    done = true;
+  }
+  return launch_dependent<W4StreamParams>(kern, p, ctas, kW4StreamWarps * 32, (deep ? 8 : 4) * kBlock + fixed, stream);
+}
+
+template <bool BF16, int NT>
+int run_stream_t(const HostDevice& d, const W4StreamParams& p, cudaStream_t stream) {
+  return p.w.shift >= 2 ? launch_stream<BF16, NT, 1>(d, p, stream) : p.w.shift == 1 ? launch_stream<BF16, NT, 2>(d, p, stream)
+                                                                                   : launch_stream<BF16, NT, 4>(d, p, stream);
+}
+
 template <bool BF16>
-int run_stream(const W4StreamParams& p, cudaStream_t stream) {
-  const bool tall = p.w.N >= 32 * 2 * kSmsModel;           // 32 rows per CTA still give two CTAs per SM
-  if (p.T <= 8) return tall ? launch_stream<BF16, 2, 1>(p, stream) : launch_stream<BF16, 1, 1>(p, stream);
-  if (p.T <= 16) return tall ? launch_stream<BF16, 2, 2>(p, stream) : launch_stream<BF16, 1, 2>(p, stream);
-  return tall ? launch_stream<BF16, 2, 4>(p, stream) : launch_stream<BF16, 1, 4>(p, stream);
+int run_stream(const HostDevice& d, const W4StreamParams& p, cudaStream_t stream) {
+  return p.T <= 8 ? run_stream_t<BF16, 1>(d, p, stream) : run_stream_t<BF16, 2>(d, p, stream);
 }
 
 template <bool BF16>
@@ -122,8 +175,7 @@ int run_pair(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, i
   // three stages, and the rest of the shared memory for packed bytes on their way from HBM
   p.stages = 3;
   p.raw_slots = std::min(kW4MaxRawSlots, (kPairSmem - 1024 - 512 - p.stages * p.stage_bytes) / kW4RawBytes);
-  p.vec = w.shift < 2 && w.groups % (4 >> w.shift) == 0 && (reinterpret_cast<uintptr_t>(w.scale) & 7) == 0 &&
-          (reinterpret_cast<uintptr_t>(w.zero) & 3) == 0;
+  p.vec = vector_groups(w);
   const int contraction = grad ? w.N : w.K, hb = l.bn / 2;
   CUtensorMap tmB, tmW;
   p.b_wide = contraction % 64 == 0;
@@ -192,7 +244,7 @@ int run_w4(const char* op, bool grad, int dtype, int M, int N, int K, const void
     p.Y = reinterpret_cast<uint16_t*>(out); p.ldy = N;
     p.bias = reinterpret_cast<const uint16_t*>(bias);
     p.T = M;
-    return dtype == MP_BF16 ? run_stream<true>(p, stream) : run_stream<false>(p, stream);
+    return dtype == MP_BF16 ? run_stream<true>(d, p, stream) : run_stream<false>(d, p, stream);
   }
   return dtype == MP_BF16 ? run_pair<true>(d, l, w, grad, M, X, ldx, bias, out, ws, stream)
                           : run_pair<false>(d, l, w, grad, M, X, ldx, bias, out, ws, stream);

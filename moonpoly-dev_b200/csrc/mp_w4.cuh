@@ -9,10 +9,12 @@
 // Unpacking without conversions: for fp16, 0x6400 | q is 1024 + q and 0x6400 | q << 4 is 1024 + 16 q, so that one
 // subtraction (or a multiply-add with 1 / 16) gives q - zero exactly; for bf16, 0x4300 | q is 128 + q.
 //
-// Two kernels.  Up to 32 tokens: w4_stream_kernel, warp-level MMAs on q - zero, exact in 16 bits, with the scale applied to
+// Two kernels.  Up to 16 tokens: w4_stream_kernel, warp-level MMAs on q - zero, exact in 16 bits, with the scale applied to
 // 32-bit sums -- bound by reading the weight.  More tokens, and the gradient of the input: w4_pair_kernel, CTA-pair tcgen05
 // tiles whose weight operand is unpacked into shared memory by eight warps while the tensor cores work on earlier stages.
 #pragma once
+#include <type_traits>
+
 #include "mp_pair_gemm.cuh"
 #include "mp_stream_mma.cuh"
 
@@ -45,32 +47,39 @@ __device__ __forceinline__ uint32_t fma2_f16(uint32_t a, uint32_t b, uint32_t c)
   return d;
 }
 
-// What unpacking needs to know of a zero point z (0..128): 128 + z (bf16) or 1024 + z and -(64 + z) (fp16), in both halves.
-// Whole numbers this small sit in the mantissa: 128 + z is 0x4300 + z up to 255, 1024 + z is 0x6400 + z, and 64 + z is
-// 0x5400 + 16 z while below 128 (z < 64) and 0x5800 + 8 (z - 64) from there.
+// What unpacking needs to know of a zero point z (0..63), in both halves: 128 + z for bf16, where 0x4300 + z is that number;
+// for fp16 1024 + z, which is 0x6400 + z, and -(64 + z), which is 0xd400 + 16 z.
 struct W4Zero { uint32_t a, b; };
 template <bool BF16> __device__ __forceinline__ W4Zero w4_zero(uint32_t z) {
-  if constexpr (BF16) {
-    // 256 (z = 128) is the next binade's first number, 0x4380, where the addition arrives by itself
-    return {(0x4300u + z) * 0x10001u, 0u};
-  } else {
-    const uint32_t b = z < 64u ? 0xd400u + 16u * z : 0xd800u + 8u * (z - 64u);
-    return {(0x6400u + z) * 0x10001u, b * 0x10001u};
-  }
+  if constexpr (BF16) return {z * 0x10001u + 0x43004300u, 0u};
+  else return {z * 0x10001u + 0x64006400u, z * 0x100010u + 0xd400d400u};
+}
+// The exponent pattern, kept in a register: "and" with one constant and "or" with another is one instruction only if one of
+// the two is a register, and the logic pipe is what the unpacking is bound by.
+template <bool BF16> __device__ __forceinline__ uint32_t w4_magic() {
+  uint32_t m;
+  if constexpr (BF16) asm volatile("mov.b32 %0, 0x43004300;" : "=r"(m));
+  else asm volatile("mov.b32 %0, 0x64006400;" : "=r"(m));
+  return m;
+}
+template <uint32_t MASK> __device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(v), "n"(MASK), "r"(bits));
+  return d;
 }
 // The 8 weights of a word as q - zero: out[j] = weights 2 j and 2 j + 1.
-template <bool BF16> __device__ __forceinline__ void w4_unpack(uint32_t w, const W4Zero& z, uint32_t (&out)[4]) {
+template <bool BF16> __device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t magic, const W4Zero& z, uint32_t (&out)[4]) {
   if constexpr (BF16) {
-    out[0] = sub2<true>((w & 0x000f000fu) | 0x43004300u, z.a);
-    out[1] = sub2<true>(((w >> 4) & 0x000f000fu) | 0x43004300u, z.a);
-    out[2] = sub2<true>(((w >> 8) & 0x000f000fu) | 0x43004300u, z.a);
-    out[3] = sub2<true>(((w >> 12) & 0x000f000fu) | 0x43004300u, z.a);
+    out[0] = sub2<true>(and_or<0x000f000fu>(w, magic), z.a);
+    out[1] = sub2<true>(and_or<0x000f000fu>(w >> 4, magic), z.a);
+    out[2] = sub2<true>(and_or<0x000f000fu>(w >> 8, magic), z.a);
+    out[3] = sub2<true>(and_or<0x000f000fu>(w >> 12, magic), z.a);
   } else {
     const uint32_t v = w >> 8;
-    out[0] = sub2<false>((w & 0x000f000fu) | 0x64006400u, z.a);
-    out[1] = fma2_f16((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z.b);      // (1024 + 16 q) / 16 - 64 - z
-    out[2] = sub2<false>((v & 0x000f000fu) | 0x64006400u, z.a);
-    out[3] = fma2_f16((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z.b);
+    out[0] = sub2<false>(and_or<0x000f000fu>(w, magic), z.a);
+    out[1] = fma2_f16(and_or<0x00f000f0u>(w, magic), 0x2c002c00u, z.b);      // (1024 + 16 q) / 16 - 64 - z
+    out[2] = sub2<false>(and_or<0x000f000fu>(v, magic), z.a);
+    out[3] = fma2_f16(and_or<0x00f000f0u>(v, magic), 0x2c002c00u, z.b);
   }
 }
 
@@ -90,9 +99,16 @@ __global__ void w4_pack_kernel(const uint8_t* q, long long ldq, uint32_t* packed
 }
 
 // ------------------------------------------------------------------------------------------------- few tokens: streaming
-// A CTA owns RT * 16 rows of W against up to 8 * NT tokens; its 8 warps take the blocks of 128 k in turn and add up in warp
-// order through shared memory.  A lane loads 16 bytes of its two rows per block straight into the A fragments of the
-// m16n8k16 MMA (the order of k inside a sum is free: X is loaded by the same rule).
+// One CTA of 16 warps per SM owns an equal share of the rows of W, cut into tiles of 16, against up to 8 * NT tokens.  Eight
+// warps side by side take eight neighbouring blocks of 128 k of a tile -- 512 contiguous bytes of each row, which HBM
+// delivers 1.3 times as fast as the 64 bytes of a warp that walks a row by itself -- and walk over the tiles first, so that
+// the tokens of a block stay in registers for all of them.  The other eight warps take every other tile (or, where the share
+// is a single tile, the other half of the blocks).  A (tile, warp) pair's sums wait in shared memory, 16 bytes per thread
+// and eight tokens, and are added in the order of the warps at the end.
+// A lane's 16 bytes of a row are the A fragments of eight m16n8k16 MMAs (the order of k inside a sum is free: X is loaded by
+// the same rule), so a thread only ever uses bytes that it fetched itself: they wait in a ring of asynchronous copies in
+// shared memory that no barrier guards.  Scales and zeros are brought to shared memory once, where they fit.
+// The sums of a group are formed on q - zero, which is exact in 16 bits, and meet their scale in 32 bits.
 struct W4StreamParams {
   W4Weight w;
   const uint16_t* X; long long ldx;      // T rows, 16-byte aligned
@@ -109,119 +125,184 @@ template <bool BF16> __device__ __forceinline__ uint16_t to16(float v) {
   if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
   else return __half_as_ushort(__float2half_rn(v));
 }
+template <int OFF> __device__ __forceinline__ uint4 ld_smem_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4+%5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "n"(OFF) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  // 0 source bytes: the 16 bytes are filled with zeros and nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+template <bool BF16> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&lo)[4], const uint32_t (&hi)[4], int j, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16) mma_m16n8k16_bf16(d, lo[j], hi[j], lo[j + 1], hi[j + 1], b0, b1);
+  else mma_m16n8k16_f16(d, lo[j], hi[j], lo[j + 1], hi[j + 1], b0, b1);
+}
 
-template <bool BF16, int RT, int NT, bool FINE>
-__global__ void __launch_bounds__(256) w4_stream_kernel(const W4StreamParams p) {
-  constexpr int U = 4 / RT;                               // blocks in flight per warp: 8 16-byte loads of W per lane
-  __shared__ float red[8][RT * 16][NT * 8 + 1];
+constexpr int kW4StreamWarps = 16;
+
+// A group's scale (low half) and zero point, as w4_zero's first half (high half), in one word.
+template <bool BF16> __device__ __forceinline__ uint32_t w4_group_word(const W4Weight& w, long long at) {
+  const uint32_t z = w.zero != nullptr ? (uint32_t)__ldg(w.zero + at) : 8u;
+  return (uint32_t)__ldg(w.scale + at) | ((BF16 ? 0x4300u : 0x6400u) + z) << 16;
+}
+template <bool BF16> __device__ __forceinline__ W4Zero w4_zero_of(uint32_t word) {
+  const uint32_t a = __byte_perm(word, word, 0x3232);
+  return {a, BF16 ? 0u : (a & 0x003f003fu) * 16u + 0xd400d400u};
+}
+
+// GPB: groups that a block of a row meets (1, 2 or 4).  STAGED: their words are in shared memory.
+template <bool BF16, int NT, int GPB, int DEPTH, bool STAGED>
+__global__ void __launch_bounds__(kW4StreamWarps * 32, 1) w4_stream_kernel(const W4StreamParams p) {
+  constexpr int kThreads = kW4StreamWarps * 32;
+  constexpr uint32_t kSlot = kThreads * 32;               // ring bytes per block
+  constexpr int G = 4 / GPB;                              // runs of 32 per group
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row0 = blockIdx.x * (RT * 16);
   const W4Weight& w = p.w;
-  float acc[RT][NT][4];
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[r][n][e] = 0.0f;
-  // rows past the end read the last row; their sums are not stored
-  int rows[RT][2];
-  const uint4* src[RT][2];
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      rows[r][h] = min(row0 + r * 16 + h * 8 + g, w.N - 1);
-      src[r][h] = w.packed + (size_t)rows[r][h] * w.blocks * 4 + t;
+  const int cta_lo = (int)((long long)w.N * blockIdx.x / gridDim.x), share = (int)((long long)w.N * (blockIdx.x + 1) / gridDim.x) - cta_lo;
+  const int tiles = (share + 15) >> 4;
+  const int kw = tiles > 1 ? 8 : 16, kpart = warp & (kw - 1), tile0 = warp / kw, tile_step = kW4StreamWarps / kw;
+  const int outer = kpart < w.blocks && tile0 < tiles ? (w.blocks - kpart + kw - 1) / kw : 0;      // blocks of this warp
+  // shared memory: ring | parked sums | group words
+  uint8_t* sums = smem_raw + DEPTH * kSlot;
+  uint32_t* words = reinterpret_cast<uint32_t*>(sums + (size_t)tiles * kw * (NT * 512));
+
+  // rows past the end of the share read its last row; their sums are not stored.  Offsets inside a share fit 32 bits: a
+  // share of 4 GB would make a weight of 600 GB.
+  const auto row_in = [&](int tile, int half) { return min(tile * 16 + half * 8 + g, share - 1); };
+  const uint32_t ring = smem_u32(smem_raw) + threadIdx.x * 16u;       // [slot][row half][thread]
+  const uint32_t pitch = (uint32_t)w.blocks * 64u;
+  const uint8_t* base = reinterpret_cast<const uint8_t*>(w.packed) + (size_t)cta_lo * pitch + t * 16;
+  int b_in = outer > 0 ? kpart : w.blocks, tile_in = tile0;
+  const auto issue = [&](uint32_t slot) {
+    if (b_in < w.blocks) {
+      const uint8_t* src = base + (size_t)b_in * 64;
+      cp_async16(ring + slot * kSlot, src + (uint32_t)row_in(tile_in, 0) * pitch, true);
+      cp_async16(ring + slot * kSlot + kThreads * 16u, src + (uint32_t)row_in(tile_in, 1) * pitch, true);
+      tile_in += tile_step;
+      if (tile_in >= tiles) { tile_in = tile0; b_in += kw; }
     }
-  uint4 cur[U][RT][2];
-  const auto load = [&](uint4 (&dst)[U][RT][2], int b0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int b = b0 + 8 * u;
-          dst[u][r][h] = b < w.blocks ? __ldcs(src[r][h] + (size_t)b * 4) : make_uint4(0, 0, 0, 0);
-        }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  load(cur, warp);
-  for (int b0 = warp; b0 < w.blocks; b0 += 8 * U) {
-    uint4 nxt[U][RT][2];
-    load(nxt, b0 + 8 * U);
+  griddep_wait();
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int b = b0 + 8 * u;
-      if (b >= w.blocks) break;
-      const int valid = min(4, (w.K - b * 128) >> 5);     // 32-weight runs of this block that exist
-      float part[RT][NT][4];
+  for (uint32_t d = 0; d < DEPTH; ++d) issue(d);
+  const long long group_base = (long long)cta_lo * w.groups;
+  if constexpr (STAGED) {
+    const int num = share * w.groups;
+    const uint16_t* sc = w.scale + group_base;
+    const uint8_t* zr = w.zero + group_base;
+    if (((reinterpret_cast<uintptr_t>(sc) & 15) | (w.zero != nullptr ? reinterpret_cast<uintptr_t>(zr) & 7 : 0) | (num & 7)) == 0) {
+      for (int i = threadIdx.x * 8; i < num; i += kThreads * 8) {     // 8 groups per thread
+        const uint4 s8 = __ldg(reinterpret_cast<const uint4*>(sc + i));
+        const uint2 z8 = w.zero != nullptr ? __ldg(reinterpret_cast<const uint2*>(zr + i)) : make_uint2(0x08080808u, 0x08080808u);
+        const uint32_t sv[4] = {s8.x, s8.y, s8.z, s8.w}, zv[2] = {z8.x, z8.y};
+        uint32_t o[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (FINE && i >= valid) break;
-        uint4 x[NT];
+        for (int e = 0; e < 8; ++e)
+          o[e] = __byte_perm(sv[e >> 1], (BF16 ? 0x4300u : 0x6400u) + ((zv[e >> 2] >> (8 * (e & 3))) & 0xffu), e & 1 ? 0x5432 : 0x5410);
+        reinterpret_cast<uint4*>(words + i)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        reinterpret_cast<uint4*>(words + i)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+    } else {
+      for (int i = threadIdx.x; i < num; i += kThreads) words[i] = w4_group_word<BF16>(w, group_base + i);
+    }
+  }
+
+  const uint16_t* xp[NT];                                 // columns past T repeat the last token; they are not stored
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int tok = n * 8 + g;
-          x[n] = (tok < p.T && i < valid) ? *reinterpret_cast<const uint4*>(p.X + (long long)tok * p.ldx + b * 128 + 32 * i + 8 * t)
-                                          : make_uint4(0, 0, 0, 0);
-        }
-        const int gi = ((b << 2) + i) >> w.shift;         // the group of this run
+  for (int n = 0; n < NT; ++n) xp[n] = p.X + (long long)min(n * 8 + g, p.T - 1) * p.ldx + 8 * t;
+  uint4 x[4][NT];
+  const auto load_x = [&](uint4 (&v)[4][NT], int b) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          uint32_t a[2][4];
+    for (int i = 0; i < 4; ++i) {
+      const int k = min(b * 128 + 32 * i, w.K - 32);      // a run past K is not used
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t z = w.zero != nullptr ? (uint32_t)__ldg(w.zero + (size_t)rows[r][h] * w.groups + gi) : 8u;
-            const uint4 q = cur[u][r][h];
-            w4_unpack<BF16>(i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w, w4_zero<BF16>(z), a[h]);
-          }
-          float sc[2];
-          if (FINE || i == 3) {
+      for (int n = 0; n < NT; ++n) v[i][n] = *reinterpret_cast<const uint4*>(xp[n] + k);
+    }
+  };
+  if (outer > 0) load_x(x, kpart);
+  if constexpr (STAGED) __syncthreads();
+
+  const uint32_t magic = w4_magic<BF16>();
+  uint32_t slot = 0;
+  for (int o = 0; o < outer; ++o) {
+    const int b = kpart + o * kw;
+    const int valid = (w.K - b * 128) >> 5;               // runs of this block that exist, if fewer than 4
+    const int group0 = GPB == 1 ? (b * 4) >> w.shift : b * GPB;
+    uint4 xn[4][NT];
+    if constexpr (NT == 1) load_x(xn, min(b + kw, w.blocks - 1));
+    else if (o > 0) load_x(x, b);
+    // one tile's 16 rows against this block; WHOLE: all four runs exist
+    const auto tile_block = [&](int tile, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      uint4* park = reinterpret_cast<uint4*>(sums) + (size_t)(tile * kw + kpart) * (NT * 32) + lane;
+      const int at_lo = row_in(tile, 0) * w.groups + group0, at_hi = row_in(tile, 1) * w.groups + group0;
+      float acc[NT][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) sc[h] = from16<BF16>(__ldg(w.scale + (size_t)rows[r][h] * w.groups + gi));
-          }
+      for (int n = 0; n < NT; ++n) {
+        const uint4 v = o > 0 ? park[n * 32] : make_uint4(0, 0, 0, 0);
+        acc[n][0] = __uint_as_float(v.x); acc[n][1] = __uint_as_float(v.y); acc[n][2] = __uint_as_float(v.z); acc[n][3] = __uint_as_float(v.w);
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+      const uint4 q_lo = ld_smem_v4<0>(ring + slot * kSlot), q_hi = ld_smem_v4<kThreads * 16>(ring + slot * kSlot);
+#pragma unroll
+      for (int gi = 0; gi < GPB; ++gi) {
+        if (!WHOLE && gi * G >= valid) break;
+        uint32_t word_lo, word_hi;
+        if constexpr (STAGED) { word_lo = words[at_lo + gi]; word_hi = words[at_hi + gi]; }
+        else { word_lo = w4_group_word<BF16>(w, group_base + at_lo + gi); word_hi = w4_group_word<BF16>(w, group_base + at_hi + gi); }
+        const W4Zero z_lo = w4_zero_of<BF16>(word_lo), z_hi = w4_zero_of<BF16>(word_hi);
+        float part[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.0f;
+#pragma unroll
+        for (int i = gi * G; i < gi * G + G; ++i) {
+          if (!WHOLE && i >= valid) break;
+          uint32_t a_lo[4], a_hi[4];
+          w4_unpack<BF16>(i == 0 ? q_lo.x : i == 1 ? q_lo.y : i == 2 ? q_lo.z : q_lo.w, magic, z_lo, a_lo);
+          w4_unpack<BF16>(i == 0 ? q_hi.x : i == 1 ? q_hi.y : i == 2 ? q_hi.z : q_hi.w, magic, z_hi, a_hi);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            if (FINE || i == 0) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) part[r][n][e] = 0.0f;
-            }
-            if constexpr (BF16) {
-              mma_m16n8k16_bf16(part[r][n], a[0][0], a[1][0], a[0][1], a[1][1], x[n].x, x[n].y);
-              mma_m16n8k16_bf16(part[r][n], a[0][2], a[1][2], a[0][3], a[1][3], x[n].z, x[n].w);
-            } else {
-              mma_m16n8k16_f16(part[r][n], a[0][0], a[1][0], a[0][1], a[1][1], x[n].x, x[n].y);
-              mma_m16n8k16_f16(part[r][n], a[0][2], a[1][2], a[0][3], a[1][3], x[n].z, x[n].w);
-            }
-            if (FINE || i == 3) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[r][n][e] = fmaf(sc[e >> 1], part[r][n][e], acc[r][n][e]);
-            }
+            mma16<BF16>(part[n], a_lo, a_hi, 0, x[i][n].x, x[i][n].y);
+            mma16<BF16>(part[n], a_lo, a_hi, 2, x[i][n].z, x[i][n].w);
           }
         }
+        const float s_lo = from16<BF16>((uint16_t)word_lo), s_hi = from16<BF16>((uint16_t)word_hi);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[n][0] = fmaf(s_lo, part[n][0], acc[n][0]);
+          acc[n][1] = fmaf(s_lo, part[n][1], acc[n][1]);
+          acc[n][2] = fmaf(s_hi, part[n][2], acc[n][2]);
+          acc[n][3] = fmaf(s_hi, part[n][3], acc[n][3]);
+        }
       }
+      issue(slot);                                         // the slot's bytes have been read by their only reader
+      slot = (slot + 1) & (DEPTH - 1);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        park[n * 32] = make_uint4(__float_as_uint(acc[n][0]), __float_as_uint(acc[n][1]), __float_as_uint(acc[n][2]), __float_as_uint(acc[n][3]));
+    };
+    if (valid >= 4) for (int tile = tile0; tile < tiles; tile += tile_step) tile_block(tile, std::true_type{});
+    else for (int tile = tile0; tile < tiles; tile += tile_step) tile_block(tile, std::false_type{});
+    if constexpr (NT == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i][0] = xn[i][0];
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) cur[u][r][h] = nxt[u][r][h];
   }
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) red[warp][r * 16 + (e >> 1) * 8 + g][n * 8 + 2 * t + (e & 1)] = acc[r][n][e];
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  for (int x = threadIdx.x; x < RT * 16 * NT * 8; x += 256) {
-    const int row = x % (RT * 16), tok = x / (RT * 16), n = row0 + row;
-    if (n >= w.N || tok >= p.T) continue;
+  const int rows = tiles * 16, parts = min(kw, w.blocks);  // warps beyond the blocks parked nothing
+  const float* parked = reinterpret_cast<const float*>(sums);
+  const int toks = min(p.T, NT * 8);
+  for (int i = threadIdx.x; i < rows * toks; i += kThreads) {
+    const int row = i % rows, tok = i / rows, n = cta_lo + row, rr = row & 15;
+    if (row >= share) continue;
+    const float* q = parked + (size_t)(row >> 4) * kw * (NT * 128) + (tok >> 3) * 128 + ((rr & 7) * 4 + ((tok & 7) >> 1)) * 4 + (rr >> 3) * 2 + (tok & 1);
     float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += red[i][row][tok];
+    for (int k = 0; k < parts; ++k) s += q[k * (NT * 128)];
     if (p.bias != nullptr) s += from16<BF16>(p.bias[n]);
     p.Y[(long long)tok * p.ldy + n] = to16<BF16>(s);
   }
@@ -268,18 +349,13 @@ __device__ __forceinline__ W4Unit w4_unit(const W4PairParams& p, int unit) {
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-template <int OFF> __device__ __forceinline__ uint4 ld_smem_v4(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4+%5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "n"(OFF) : "memory");
-  return v;
-}
 template <int OFF> __device__ __forceinline__ void st_smem_v4(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0+%5], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "n"(OFF) : "memory");
 }
 // The 8 weights of a word.
-template <bool BF16> __device__ __forceinline__ uint4 w4_weights(uint32_t word, const W4Zero& zero, uint32_t scale) {
+template <bool BF16> __device__ __forceinline__ uint4 w4_weights(uint32_t word, uint32_t magic, const W4Zero& zero, uint32_t scale) {
   uint32_t v[4];
-  w4_unpack<BF16>(word, zero, v);
+  w4_unpack<BF16>(word, magic, zero, v);
   return make_uint4(mul2<BF16>(v[0], scale), mul2<BF16>(v[1], scale), mul2<BF16>(v[2], scale), mul2<BF16>(v[3], scale));
 }
 
@@ -407,6 +483,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
     const int group = (warp - 8) >> 3, r0 = ((warp - 8) & 7) * 16 + (lane & 7), t = lane >> 3;
     const uint32_t raw_off = raw_base + (uint32_t)(r0 * 64 + ((t ^ ((r0 >> 1) & 3)) << 4));
     const uint32_t even_off = smem_base + (uint32_t)(r0 * 128 + ((t ^ (r0 & 7)) << 4)), odd_off = even_off ^ 64u;   // runs 0, 2 and 1, 3
+    const uint32_t magic = w4_magic<BF16>();
     int s = group, rs = group;                          // the host gives at least two of each
     uint32_t ph = 0, rph = 0;
     const W4Weight& w = p.w;
@@ -484,14 +561,14 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
       if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) break;
       const uint32_t ev = even_off + (uint32_t)s * (uint32_t)p.stage_bytes, od = odd_off + (uint32_t)s * (uint32_t)p.stage_bytes;
       // the weight in the operand type: one rounding of the exact product (q - zero) * scale
-      st_smem_v4<0>(ev, w4_weights<BF16>(q0.x, zero[0][0], scale[0][0]));
-      st_smem_v4<0>(od, w4_weights<BF16>(q0.y, zero[0][1 % R], scale[0][1 % R]));
-      st_smem_v4<16384>(ev, w4_weights<BF16>(q0.z, zero[0][2 % R], scale[0][2 % R]));
-      st_smem_v4<16384>(od, w4_weights<BF16>(q0.w, zero[0][3 % R], scale[0][3 % R]));
-      st_smem_v4<1024>(ev, w4_weights<BF16>(q1.x, zero[1][0], scale[1][0]));
-      st_smem_v4<1024>(od, w4_weights<BF16>(q1.y, zero[1][1 % R], scale[1][1 % R]));
-      st_smem_v4<17408>(ev, w4_weights<BF16>(q1.z, zero[1][2 % R], scale[1][2 % R]));
-      st_smem_v4<17408>(od, w4_weights<BF16>(q1.w, zero[1][3 % R], scale[1][3 % R]));
+      st_smem_v4<0>(ev, w4_weights<BF16>(q0.x, magic, zero[0][0], scale[0][0]));
+      st_smem_v4<0>(od, w4_weights<BF16>(q0.y, magic, zero[0][1 % R], scale[0][1 % R]));
+      st_smem_v4<16384>(ev, w4_weights<BF16>(q0.z, magic, zero[0][2 % R], scale[0][2 % R]));
+      st_smem_v4<16384>(od, w4_weights<BF16>(q0.w, magic, zero[0][3 % R], scale[0][3 % R]));
+      st_smem_v4<1024>(ev, w4_weights<BF16>(q1.x, magic, zero[1][0], scale[1][0]));
+      st_smem_v4<1024>(od, w4_weights<BF16>(q1.y, magic, zero[1][1 % R], scale[1][1 % R]));
+      st_smem_v4<17408>(ev, w4_weights<BF16>(q1.z, magic, zero[1][2 % R], scale[1][2 % R]));
+      st_smem_v4<17408>(od, w4_weights<BF16>(q1.w, magic, zero[1][3 % R], scale[1][3 % R]));
       fence_async_smem();                              // the tensor cores read through the async proxy
       __syncwarp();
       if (lane == 0) mbar_arrive_pair(mapa_shared(full_bar(s), 0));

@@ -8,6 +8,7 @@ when the CUDA library cannot be loaded, importing the compute entry points raise
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Optional
@@ -427,69 +428,80 @@ def pack_w4(q: torch.Tensor) -> torch.Tensor:
     if q.dim() != 2 or q.dtype != torch.uint8 or not q.is_cuda:
         raise ValueError("q must be a 2-D CUDA uint8 tensor [N, K]")
     N, K = q.shape
-    with torch.cuda.device(q.device):
+    with _device_of(q):
         q, ldq = _rows(q)
         out = torch.empty((N, (K + 127) // 128 * 16), dtype=torch.int32, device=q.device)
         _check(lib().mp_w4_pack(N, K, _ptr(q), ldq, _ptr(out), _stream(q)))
     return out
 
 
-def _w4_checks(op: str, x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros, group_size: int, width: str, K: int):
+_W4_CODES = {torch.float16: MP_FP16, torch.bfloat16: MP_BF16}
+
+
+def _w4_checks(op: str, x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros, group_size: int, grad: bool, K: int):
     if x.dim() != 2 or qweight.dim() != 2:
         raise ValueError(f"{op}: input and packed weight must be 2-D tensors")
-    code = _dtype16(x, op)
-    N = qweight.shape[0]
-    if qweight.dtype != torch.int32 or qweight.shape[1] != (K + 127) // 128 * 16 or N == 0 or K == 0:
+    code = _W4_CODES.get(x.dtype)
+    if code is None:
+        raise ValueError(f"{op} serves fp16 and bf16")
+    N, words = qweight.shape
+    if qweight.dtype != torch.int32 or words != (K + 127) // 128 * 16 or N == 0 or K == 0:
         raise ValueError(f"{op}: the packed weight must be int32 [N, 16 * ceil(K / 128)]")
-    if x.shape[1] != (K if width == "K" else N):
-        raise ValueError(f"{op}: input must be [M, {width}]")
+    if x.shape[1] != (N if grad else K):
+        raise ValueError(f"{op}: input must be [M, {'N' if grad else 'K'}]")
     if K % 32:
         raise ValueError(f"{op}: K = {K} must be a multiple of 32")
     if group_size == -1:                                   # one group per row
-        group_size = 32
-        while group_size < K:
-            group_size *= 2
-    if group_size < 32 or group_size & (group_size - 1):
+        group_size = max(32, 1 << (K - 1).bit_length())
+    elif group_size < 32 or group_size & (group_size - 1):
         raise ValueError(f"{op}: group_size must be a power of two of at least 32, or -1")
     shape = (N, (K + group_size - 1) // group_size)
-    if scales.dtype != x.dtype or tuple(scales.shape) != shape:
+    if scales.dtype != x.dtype or scales.shape != shape:
         raise ValueError(f"{op}: scales must be {list(shape)} in the input dtype")
-    if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != shape):
-        raise ValueError(f"{op}: zeros must be {list(shape)} uint8")
-    for t in (x, qweight, scales, zeros):
-        if t is not None and (not t.is_cuda or t.device != x.device):
-            raise ValueError(f"{op}: all tensors must be CUDA tensors on one device")
+    device = x.get_device()
+    if device < 0 or qweight.get_device() != device or scales.get_device() != device:
+        raise ValueError(f"{op}: all tensors must be CUDA tensors on one device")
+    if zeros is not None:
+        if zeros.dtype != torch.uint8 or zeros.shape != shape or zeros.get_device() != device:
+            raise ValueError(f"{op}: zeros must be {list(shape)} uint8 on the input's device")
+        zeros = zeros.contiguous()
     qweight = qweight.contiguous()
     if qweight.data_ptr() & 15:                            # a view off the 16 bytes the loads want
         qweight = qweight.clone()
-    return code, N, group_size, qweight, scales.contiguous(), None if zeros is None else zeros.contiguous()
+    return code, N, group_size, qweight, scales.contiguous(), zeros
 
 
-def _w4_workspace(M, N, K, x, ldx, grad) -> torch.Tensor:
+def _w4_workspace(M, N, K, x, ldx, grad):
+    """(tensor or None, address, bytes).  A fresh tensor per call: calls on other streams and captured graphs never share it."""
     need = ctypes.c_size_t()
-    _check(lib().mp_linear_w4_workspace(M, N, K, _ptr(x), ldx, grad, ctypes.byref(need)))
-    return torch.empty((need.value,), dtype=torch.uint8, device=x.device) if need.value else None
+    _check(lib().mp_linear_w4_workspace(M, N, K, x.data_ptr(), ldx, grad, ctypes.byref(need)))
+    if need.value == 0:
+        return None, 0, 0
+    ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device)
+    return ws, ws.data_ptr(), need.value
 
 
 def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
               group_size: int = 128, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Y[M,N] = x[M,K] @ W[N,K]^T (+ bias[N]) with W[n,k] = (q[n,k] - zero[n, k // group_size]) * scale[n, k // group_size],
     qweight from `pack_w4`, scales [N, ceil(K / group_size)] in the type of x (fp16 or bf16), zeros the same shape in uint8
-    (values 0..128; None: 8 everywhere).  group_size is a power of two of at least 32, or -1 for one group per row.  The
+    (values 0..63; None: 8 everywhere).  group_size is a power of two of at least 32, or -1 for one group per row.  The
     bias is added before the only rounding of the result."""
     K = x.shape[1] if x.dim() == 2 else 0
-    code, N, group_size, qweight, scales, zeros = _w4_checks("linear_w4", x, qweight, scales, zeros, group_size, "K", K)
+    code, N, group_size, qweight, scales, zeros = _w4_checks("linear_w4", x, qweight, scales, zeros, group_size, False, K)
     M = x.shape[0]
     if bias is not None:
         if bias.dtype != x.dtype or bias.numel() != N or bias.device != x.device:
             raise ValueError("bias must be a CUDA tensor of N elements in the input dtype")
         bias = bias.contiguous()
-    with torch.cuda.device(x.device):
+    with _device_of(x):
         y = torch.empty((M, N), dtype=x.dtype, device=x.device)
         x, ldx = _rows(x)
-        ws = _w4_workspace(M, N, K, x, ldx, 0)
-        _check(lib().mp_linear_w4(code, M, N, K, _ptr(x), ldx, _ptr(qweight), _ptr(scales), _ptr(zeros), group_size, _ptr(bias),
-                                  _ptr(y), _ptr(ws), 0 if ws is None else ws.numel(), _stream(x)))
+        ws, at, size = _w4_workspace(M, N, K, x, ldx, 0)
+        rc = lib().mp_linear_w4(code, M, N, K, x.data_ptr(), ldx, qweight.data_ptr(), scales.data_ptr(), _addr(zeros), group_size,
+                                _addr(bias), y.data_ptr(), at, size, _raw_stream(x))
+    if rc:
+        _check(rc)
     return y
 
 
@@ -497,15 +509,17 @@ def linear_w4_grad_input(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.
                          group_size: int = 128, in_features: Optional[int] = None) -> torch.Tensor:
     """dX[M,K] = dy[M,N] @ W[N,K], the gradient that `linear_w4` with a frozen weight hands back.  in_features is K where it
     is not a multiple of 128 (the packed rows are padded to 128)."""
-    K = qweight.shape[1] * 8 if in_features is None else int(in_features)
-    code, N, group_size, qweight, scales, zeros = _w4_checks("linear_w4_grad_input", dy, qweight, scales, zeros, group_size, "N", K)
+    K = qweight.shape[-1] * 8 if in_features is None else int(in_features)
+    code, N, group_size, qweight, scales, zeros = _w4_checks("linear_w4_grad_input", dy, qweight, scales, zeros, group_size, True, K)
     M = dy.shape[0]
-    with torch.cuda.device(dy.device):
+    with _device_of(dy):
         dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
         dy, ld = _rows(dy)
-        ws = _w4_workspace(M, N, K, dy, ld, 1)
-        _check(lib().mp_linear_w4_grad_input(code, M, N, K, _ptr(dy), ld, _ptr(qweight), _ptr(scales), _ptr(zeros), group_size,
-                                             _ptr(dx), _ptr(ws), 0 if ws is None else ws.numel(), _stream(dy)))
+        ws, at, size = _w4_workspace(M, N, K, dy, ld, 1)
+        rc = lib().mp_linear_w4_grad_input(code, M, N, K, dy.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(), _addr(zeros),
+                                           group_size, dx.data_ptr(), at, size, _raw_stream(dy))
+    if rc:
+        _check(rc)
     return dx
 
 
@@ -522,9 +536,29 @@ def _dtype16(t: torch.Tensor, op: str) -> int:
 
 def _rows(t: torch.Tensor):
     """(tensor, row stride) of a 2-D operand whose rows are packed; anything else is copied."""
-    if t.stride(1) != 1 and t.shape[1] > 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    rows, width = t.shape
+    if t.is_contiguous():
+        return t, width
+    ld, step = t.stride()
+    if step != 1 and width > 1 or (rows > 1 and ld < width):
+        return t.contiguous(), width
+    return t, (ld if rows > 1 else width)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _device_of(t: torch.Tensor):
+    """Makes the tensor's device current for the launches inside, at no cost when it already is."""
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _raw_stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _xent_checks(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor) -> None:
@@ -541,7 +575,7 @@ def _xent_checks(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor) -> None
 def _xent_workspace(code, M, V, H, x, ldx, w, ldw, backward) -> torch.Tensor:
     # a fresh tensor per call: calls on other streams and captured graphs never share it
     need = ctypes.c_size_t()
-    _check(lib().mp_linear_xent_workspace(code, M, V, H, _ptr(x), ldx, _ptr(w), ldw, backward, ctypes.byref(need)))
+    _check(lib().mp_linear_xent_workspace(code, M, V, H, x.data_ptr(), ldx, w.data_ptr(), ldw, backward, ctypes.byref(need)))
     return torch.empty((need.value,), dtype=torch.uint8, device=x.device)
 
 
@@ -553,15 +587,15 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor,
     _xent_checks(x, w, target)
     code = _dtype16(x, "linear_cross_entropy")
     (M, H), V = x.shape, w.shape[0]
-    with torch.cuda.device(x.device):
+    with _device_of(x):
         x, ldx = _rows(x)
         w, ldw = _rows(w)
         target = target.contiguous()
         loss = torch.empty((M,), dtype=torch.float32, device=x.device)
         lse = torch.empty_like(loss)
         ws = _xent_workspace(code, M, V, H, x, ldx, w, ldw, 0)
-        _check(lib().mp_linear_xent(code, M, V, H, _ptr(x), ldx, _ptr(w), ldw, _ptr(target), target.element_size(), ignore_index,
-                                    _ptr(loss), _ptr(lse), _ptr(ws), ws.numel(), _stream(x)))
+        _check(lib().mp_linear_xent(code, M, V, H, x.data_ptr(), ldx, w.data_ptr(), ldw, target.data_ptr(), target.element_size(),
+                                    ignore_index, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(x)))
     return loss, lse
 
 
@@ -576,16 +610,16 @@ def linear_cross_entropy_grad(x: torch.Tensor, w: torch.Tensor, target: torch.Te
     for name, t in (("lse", lse), ("grad_loss", grad_loss)):
         if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != M or t.device != x.device:
             raise ValueError(f"{name} must be M fp32 values on the operands' device")
-    with torch.cuda.device(x.device):
+    with _device_of(x):
         dx = torch.empty((M, H), dtype=x.dtype, device=x.device) if need_dx else None
         dw = torch.empty((V, H), dtype=x.dtype, device=x.device) if need_dw else None
         x, ldx = _rows(x)
         w, ldw = _rows(w)
         target, lse, grad_loss = target.contiguous(), lse.contiguous(), grad_loss.contiguous()
         ws = _xent_workspace(code, M, V, H, x, ldx, w, ldw, 1)
-        _check(lib().mp_linear_xent_grad(code, M, V, H, _ptr(x), ldx, _ptr(w), ldw, _ptr(target), target.element_size(),
-                                         ignore_index, _ptr(lse), _ptr(grad_loss), _ptr(dx), _ptr(dw), _ptr(ws), ws.numel(),
-                                         _stream(x)))
+        _check(lib().mp_linear_xent_grad(code, M, V, H, x.data_ptr(), ldx, w.data_ptr(), ldw, target.data_ptr(), target.element_size(),
+                                         ignore_index, lse.data_ptr(), grad_loss.data_ptr(), _addr(dx), _addr(dw), ws.data_ptr(),
+                                         ws.numel(), _raw_stream(x)))
     return dx, dw
 
 

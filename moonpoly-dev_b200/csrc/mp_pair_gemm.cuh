@@ -40,12 +40,13 @@ struct PairProblem {
   int a_mn, b_mn;                // 1: MN-major operand
   int a_wide, b_wide;            // 1: the operand's tensor map is 3-D and one box brings 256 contiguous bytes per line
   int group_m;                   // raster: tiles are walked in groups of `group_m` row tiles
-  int tile0;                     // index of the problem's first tile in the launch
-  // PAIR_STORE: out16 = scale * acc (+ acc32 before scaling), or acc32 (+)= acc when out16 is null
+  int tile0;                     // index of the problem's first unit in the launch
+  int split, kb_per_split;       // PAIR_STORE: the contraction in `split` slices of kb_per_split blocks, a unit each
+  // PAIR_STORE: out16 = scale * acc (+ acc32 before scaling), or acc32[slice] (+)= acc when out16 is null
   void* out16;
   float* acc32;
   long long ld_out;              // row stride of out16 in elements
-  long long ld_acc;
+  long long ld_acc, acc_slice;   // row stride of acc32, and elements from slice to slice
   int add_acc32;                 // 1: acc32 holds earlier contributions
   const float* scale;            // device scalar, may be null (1.0)
 };
@@ -53,7 +54,8 @@ struct PairProblem {
 struct PairParams {
   int num_problems;
   PairProblem prob[2];
-  int total_tiles;
+  int total_tiles;               // units of the launch
+  unsigned* next_unit;           // PAIR_STORE: counter that hands out units, zero before the launch
   int stages, stage_bytes;
   int kc;                        // 64-element blocks of the contraction per stage (1 or 2)
   int bf16;                      // operand and output type: 1 = bf16, 0 = fp16
@@ -185,13 +187,23 @@ __device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap* tm, u
   }
 }
 
-struct PairUnit { int prob, tm, tn; };
+struct PairUnit { int prob, tm, tn, slice, kb0, kb1; };
 
 __host__ __device__ __forceinline__ PairUnit pair_unit(const PairParams& p, int unit) {
   PairUnit u;
   u.prob = (p.num_problems == 2 && unit >= p.prob[1].tile0) ? 1 : 0;
   const PairProblem& q = p.prob[u.prob];
-  const int t = unit - q.tile0;
+  int t = unit - q.tile0;
+  u.slice = 0;
+  u.kb0 = 0;
+  u.kb1 = q.kblocks;
+  if (q.split > 1) {                                     // slice by slice: neighbours share the operands of a slice
+    const int tiles = q.tiles_m * q.tiles_n;
+    u.slice = t / tiles;
+    t -= u.slice * tiles;
+    u.kb0 = u.slice * q.kb_per_split;
+    u.kb1 = u.kb0 + q.kb_per_split < q.kblocks ? u.kb0 + q.kb_per_split : q.kblocks;
+  }
   const int group = q.group_m * q.tiles_n;
   const int g = t / group, first = g * q.group_m;
   const int height = q.tiles_m - first < q.group_m ? q.tiles_m - first : q.group_m;
@@ -200,6 +212,47 @@ __host__ __device__ __forceinline__ PairUnit pair_unit(const PairParams& p, int 
   u.tm = first + (in - u.tn * height);
   return u;
 }
+
+// Where the roles of a CTA get their units from.  Static: pair, pair + pairs, ...  Dynamic (units of different lengths):
+// the first unit is the pair's own number, further ones come from a counter in global memory; warp 2 of rank 0 fetches them
+// and posts them in a two-slot box in the shared memory of both CTAs, which every role reads and hands back.  Which pair
+// computes a unit has no influence on its result.
+template <bool DYNAMIC>
+struct PairUnits {
+  const PairParams& p;
+  uint32_t box, bars;            // slots (4 bytes each) and barriers (box_full[2], box_empty[2], 8 bytes each)
+  int unit, step;
+  uint32_t n = 0;
+  __device__ PairUnits(const PairParams& p_, uint32_t box_, uint32_t bars_, int pair, int pairs) : p(p_), box(box_), bars(bars_), unit(pair - pairs), step(pairs) {}
+  // The next unit, or -1.  Called by one lane.
+  __device__ __forceinline__ int next() {
+    if constexpr (!DYNAMIC) {
+      unit += step;
+      return unit < p.total_tiles ? unit : -1;
+    } else {
+      const uint32_t slot = n & 1u, ph = (n >> 1) & 1u;
+      ++n;
+      if (!mbar_wait_cluster(bars + 8u * slot, ph, p.status, MP_DEV_TIMEOUT_CLUSTER)) return -1;
+      int v;
+      asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(box + 4u * slot) : "memory");
+      mbar_arrive_cluster(mapa_shared(bars + 16u + 8u * slot, 0));
+      return v < p.total_tiles ? v : -1;
+    }
+  }
+  // Warp 2 of rank 0, one lane: posts units until the roles have been told that there are none left.
+  __device__ __forceinline__ void post(int pair, int pairs) {
+    for (uint32_t i = 0;; ++i) {
+      const uint32_t slot = i & 1u, ph = (i >> 1) & 1u;
+      if (!mbar_wait_cluster(bars + 16u + 8u * slot, ph ^ 1u, p.status, MP_DEV_TIMEOUT_CLUSTER)) return;
+      const int v = i == 0 ? pair : (int)atomicAdd(p.next_unit, 1u) + pairs;
+      for (uint32_t r = 0; r < 2; ++r) {
+        asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(mapa_shared(box + 4u * slot, r)), "r"(v) : "memory");
+        mbar_arrive_cluster(mapa_shared(bars + 8u * slot, r));
+      }
+      if (v >= p.total_tiles) return;
+    }
+  }
+};
 
 // ------------------------------------------------------------------------------------------------------ the epilogues
 // Softmax statistics of this warp's half (128 columns) of a 256-column tile, one row per lane.  The tensor cores drop the
@@ -279,7 +332,7 @@ __device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const
 }
 
 __device__ __forceinline__ void pair_epilogue_store(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
-                                                    int ncols, int half_cols) {
+                                                    int ncols, int half_cols, int slice) {
   const bool live = row < q.rows;
   const float scale = (q.out16 != nullptr && q.scale != nullptr) ? *q.scale : 1.0f;
   for (int c0 = 0; c0 < half_cols; c0 += 32) {
@@ -292,7 +345,7 @@ __device__ __forceinline__ void pair_epilogue_store(const PairParams& p, const P
     float v[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-    float* a = q.acc32 + (long long)row * q.ld_acc + c_begin + c0;
+    float* a = q.acc32 + (long long)slice * q.acc_slice + (long long)row * q.ld_acc + c_begin + c0;
     if (q.add_acc32) {                                  // ld_acc is a multiple of 32: rows of the scratch are padded
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -326,16 +379,23 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
   auto empty_bar = [&](int s) { return bar_base + 8u * (uint32_t)(stages + s); };
   auto tfull_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + b); };
   auto tempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 2 + b); };
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4));
+  const uint32_t unit_bars = bar_base + 8u * (uint32_t)(2 * stages + 4), unit_box = unit_bars + 32u;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 40);
+  constexpr bool DYNAMIC = EPI == PAIR_STORE;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
   int* status = p.status;
+  PairUnits<DYNAMIC> units(p, unit_box, unit_bars, pair, pairs);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), 16); }
+    for (uint32_t b = 0; b < 2; ++b) {
+      mbar_init(unit_bars + 8u * b, 1);
+      mbar_init(unit_bars + 16u + 8u * b, 19);          // two producers, the MMA issuer, sixteen epilogue warps
+    }
     mbar_fence_init();
     tma_prefetch_desc(&tmA0);
     tma_prefetch_desc(&tmB0);
@@ -355,7 +415,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int unit = pair; ok && unit < p.total_tiles; unit += pairs) {
+      for (int unit; ok && (unit = units.next()) >= 0;) {
         const PairUnit u = pair_unit(p, unit);
         const PairProblem& q = p.prob[u.prob];
         const CUtensorMap* tmA = u.prob ? &tmA1 : &tmA0;
@@ -363,7 +423,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         const int hb = q.bn >> 1;
         const int a0 = u.tm * kPairRows + (int)rank * 128, b0 = u.tn * q.bn + (int)rank * hb;
         const uint32_t a_bytes = (uint32_t)(p.kc * kPairABytes), tx = 2u * (a_bytes + (uint32_t)(p.kc * hb * 128));   // both CTAs
-        for (int kb = 0; kb < q.kblocks; kb += p.kc) {
+        for (int kb = u.kb0; kb < u.kb1; kb += p.kc) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
           const uint32_t dst = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), tx);
@@ -385,7 +445,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
       int s = 0;
       uint32_t ph = 0, ui = 0;
       bool ok = true;
-      for (int unit = pair; ok && unit < p.total_tiles; unit += pairs) {
+      for (int unit; ok && (unit = units.next()) >= 0;) {
         const PairUnit u = pair_unit(p, unit);
         const PairProblem& q = p.prob[u.prob];
         const uint32_t idesc = umma_idesc(1u, p.bf16 ? 1u : 0u, kPairRows, (uint32_t)q.bn) | ((uint32_t)q.a_mn << 15) | ((uint32_t)q.b_mn << 16);
@@ -400,12 +460,12 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4;
         // an accumulator takes the whole contraction, or a chunk of it (PAIR_LSE)
         const int chunk = EPI == PAIR_LSE ? kLseChunk : q.kblocks;
-        for (int k0 = 0; ok && k0 < q.kblocks; k0 += chunk, ++ui) {
+        for (int k0 = u.kb0; ok && k0 < u.kb1; k0 += chunk, ++ui) {
         const uint32_t buf = ui & 1u, use = ui >> 1;
         if (!mbar_wait(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * (uint32_t)kPairMaxBN;
-        const int k1 = min(q.kblocks, k0 + chunk);
+        const int k1 = min(u.kb1, k0 + chunk);
         uint32_t first = 0u;
         for (int kb = k0; kb < k1; kb += p.kc) {
           if (!mbar_wait(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
@@ -424,13 +484,24 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         }
       }
     }
+    if constexpr (DYNAMIC) {
+      if (warp == 2 && lane == 0 && rank == 0) units.post(pair, pairs);
+    }
   } else {
     // -------------------------------------------------------------------------------------------------- epilogue warps
     if constexpr (EPI == PAIR_LSE) regs_more_208();
     const int quad = warp & 3, half = (warp - 4) >> 2;
     uint32_t ui = 0;
     bool ok = true;
-    for (int unit = pair; ok && unit < p.total_tiles; unit += pairs) {
+    while (ok) {
+      int unit = 0;
+      if constexpr (DYNAMIC) {
+        if (lane == 0) unit = units.next();
+        unit = __shfl_sync(0xffffffffu, unit, 0);
+      } else {
+        unit = units.next();
+      }
+      if (unit < 0) break;
       const PairUnit u = pair_unit(p, unit);
       const PairProblem& q = p.prob[u.prob];
       const int half_cols = q.bn >> 1;
@@ -466,7 +537,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         tc_fence_after();
         const uint32_t t_addr = t_half + buf * (uint32_t)kPairMaxBN;
         if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols);
-        else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols);
+        else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols, u.slice);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));

@@ -62,10 +62,13 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const float2* partial, 
 
 // Row factors of d and the scale of the products.  d is parked in 16 bits, so the largest |g| is divided out (a mean over
 // the tokens then rounds exactly: the factors are 1) and, for fp16, replaced by 2^15: a probability of 2e-9 is still a
-// normal fp16 number beside a one.  One block: the rows of a training batch are a few kilobytes.
+// normal fp16 number beside a one.  One block: the rows of a training batch are a few kilobytes.  It also
+// clears the counters that hand out the units of the products' launches.
 __global__ void __launch_bounds__(1024) xent_coef_kernel(const float* grad_loss, const void* target, int target64,
-                                                         long long ignore_index, int vocab, int rows, int bf16, float* coef, float* scale) {
+                                                         long long ignore_index, int vocab, int rows, int bf16, float* coef, float* scale,
+                                                         unsigned* counters, int num_counters) {
   __shared__ float red[32];
+  for (int i = threadIdx.x; i < num_counters; i += 1024) counters[i] = 0u;
   float g = 0.0f;
   for (int i = threadIdx.x; i < rows; i += 1024) {
     const long long t = target64 ? reinterpret_cast<const long long*>(target)[i] : reinterpret_cast<const int*>(target)[i];
@@ -91,6 +94,31 @@ __global__ void __launch_bounds__(1024) xent_coef_kernel(const float* grad_loss,
   if (threadIdx.x == 0) *scale = g / up;
 }
 
+// dX = scale * sum of the slices' 32-bit sums, in their order; four columns per thread.
+__global__ void __launch_bounds__(256) xent_dx_kernel(const float* acc, int slices, long long slice_words, long long ld_acc, int rows, int cols,
+                                                      const float* scale, uint16_t* out, int bf16) {
+  const int quads = (int)(ld_acc >> 2);
+  const long long x = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (x >= (long long)rows * quads) return;
+  const int row = (int)(x / quads), col = (int)(x - (long long)row * quads) * 4;
+  const int n = cols - col < 4 ? cols - col : 4;
+  if (n <= 0) return;
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < slices; ++i) {
+    const float4 a = *reinterpret_cast<const float4*>(acc + i * slice_words + row * ld_acc + col);
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+  }
+  const float k = *scale;
+  const uint32_t lo = pack16(v[0] * k, v[1] * k, bf16), hi = pack16(v[2] * k, v[3] * k, bf16);
+  uint16_t* o = out + (long long)row * cols + col;
+  if (n == 4 && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+  } else {
+    const uint16_t w[4] = {(uint16_t)lo, (uint16_t)(lo >> 16), (uint16_t)hi, (uint16_t)(hi >> 16)};
+    for (int e = 0; e < n; ++e) o[e] = w[e];
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------ problem
 struct Xent {
   int dtype, M, V, H;
@@ -104,9 +132,10 @@ struct Xent {
 struct Layout {
   size_t x_copy, w_copy;                  // aligned copies of operands whose rows miss TMA's 16 bytes
   size_t partial, target_logit;           // forward
-  size_t coef, dl, acc;                   // gradients
+  size_t coef, counters, dl, acc;         // gradients
   int hp, piece, pieces;
-  long long ld_acc, ld_dl;
+  int max_split;                          // slices that `acc` has room for
+  long long ld_acc, ld_dl, acc_slice;
   size_t total;
 };
 
@@ -116,6 +145,28 @@ int xent_piece(int M, int V) {
   long long piece = (256ll << 20) / (2 * rows) / 256 * 256;
   piece = std::max<long long>(piece, 4096);
   return (int)std::min<long long>(piece, (long long)round_up((size_t)V, 256));
+}
+
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+constexpr int kPairsModel = 74;          // workspace sizes must not depend on the device that is asked
+
+// Slices of the vocabulary in the product dX = d W of one piece.  It has few, long tiles (M / 256 x H / 256, cols / 64 blocks
+// each), so whole tiles leave SMs idle: 300 x 2040 are 16 tiles for 74 pairs.  The slices' sums are joined by a kernel of
+// its own; its traffic, in units of a block's time (a third of a microsecond), is weighed against the shorter critical path.
+// dW's many short tiles fill the gaps where there is a dW.
+int dx_split(int M, int H, int cols, bool with_dw) {
+  const int tiles = ceil_div(M, kPairRows) * ceil_div(H, kPairMaxBN), blocks = ceil_div(cols, 64);
+  const double even = (with_dw ? 2.0 : 1.0) * tiles * blocks / kPairsModel;          // dW is as much work as dX
+  const long long slice_bytes = (long long)M * (long long)round_up((size_t)H, 32) * 4;
+  double best = 0.0;
+  int split = 1;
+  for (int s = 1; s <= 16 && (s == 1 || s * slice_bytes <= (512ll << 20)) && blocks / s >= 16; ++s) {
+    const double longest = (double)ceil_div(tiles * s, kPairsModel) * (ceil_div(blocks, s) + 8);
+    const double cost = std::max(longest, even) + (s > 1 ? 10.0 + 2.0 * s * slice_bytes / 1.7e6 : 0.0);
+    if (s == 1 || cost < 0.97 * best) { best = cost; split = s; }
+  }
+  return split;
 }
 
 Layout xent_layout(int M, int V, int H, bool copies, bool backward) {
@@ -138,7 +189,11 @@ Layout xent_layout(int M, int V, int H, bool copies, bool backward) {
     l.ld_acc = (long long)round_up((size_t)H, 32);
     l.coef = take(((size_t)M + 64) * sizeof(float));
     l.dl = take((size_t)M * l.piece * 2);
-    if (l.pieces > 1) l.acc = take((size_t)M * l.ld_acc * sizeof(float));
+    l.counters = take((size_t)l.pieces * sizeof(unsigned));
+    const int first = std::min(V, l.piece);
+    l.max_split = std::max(dx_split(M, H, first, false), dx_split(M, H, first, true));
+    l.acc_slice = (long long)M * l.ld_acc;
+    if (l.pieces > 1 || l.max_split > 1) l.acc = take((size_t)l.max_split * l.acc_slice * sizeof(float));
   }
   l.total = at;
   return l;
@@ -178,8 +233,6 @@ int operand_map(CUtensorMap* tm, const void* ptr, long long inner, long long row
   return host_tmap(tm, kTmap16, ptr, inner, rows, ld * 2, 64, mn ? kc * 64 : rows_cta, 128);
 }
 
-int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
 void shape_problem(PairProblem* q, int rows, int cols, int contraction, int bn, int a_mn, int b_mn, int group_m, int tile0) {
   q->rows = rows; q->cols = cols;
   q->kblocks = ceil_div(contraction, 64);
@@ -189,6 +242,8 @@ void shape_problem(PairProblem* q, int rows, int cols, int contraction, int bn, 
   q->a_mn = a_mn; q->b_mn = b_mn;
   q->group_m = std::max(1, std::min(group_m, q->tiles_m));
   q->tile0 = tile0;
+  q->split = 1;
+  q->kb_per_split = q->kblocks;
 }
 
 template <int EPI>
@@ -295,12 +350,17 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
   }
   float* coef = reinterpret_cast<float*>(ws + l.coef);
   float* scale = coef + M;
+  unsigned* counters = reinterpret_cast<unsigned*>(ws + l.counters);
   uint16_t* dl = reinterpret_cast<uint16_t*>(ws + l.dl);
+  // the same slices in every piece (a short last piece may leave the last ones without work): sums stay in their order
+  const int split = dX == nullptr ? 1 : dx_split(M, H, std::min(V, l.piece), dW != nullptr);
   const int bf16 = dtype == MP_BF16, target64 = target_bytes == 8;
-  xent_coef_kernel<<<1, 1024, 0, stream>>>(grad_loss, target, target64, ignore_index, V, M, bf16, coef, scale);
+  xent_coef_kernel<<<1, 1024, 0, stream>>>(grad_loss, target, target64, ignore_index, V, M, bf16, coef, scale,
+                                           counters, l.pieces);
   MP_HOST_CUDA_TRY(cudaGetLastError());
   host_count_launches(1);
 
+  int slices = 0;                                     // of dX, waiting to be joined
   for (int i = 0; i < l.pieces; ++i) {
     const int col0 = i * l.piece, cols = std::min(l.piece, V - col0);
     const uint16_t* Wp = reinterpret_cast<const uint16_t*>(W) + (long long)col0 * ldw;
@@ -320,17 +380,25 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
     }
     PairParams p{};
     p.bf16 = bf16;
+    p.next_unit = counters + i;
     int n = 0;
     if (dX != nullptr) {                              // dX[M, H] (+)= d[M, cols] W[cols, H]
       PairProblem& q = p.prob[n];
       shape_problem(&q, M, H, cols, kPairMaxBN, 0, 1, 8, p.total_tiles);
       q.acc32 = reinterpret_cast<float*>(ws + l.acc);
       q.ld_acc = l.ld_acc;
+      q.acc_slice = l.acc_slice;
       q.add_acc32 = i > 0;
-      if (i == l.pieces - 1) { q.out16 = dX; q.ld_out = H; q.scale = scale; }
+      if (split > 1) {
+        q.kb_per_split = (int)round_up((size_t)ceil_div(q.kblocks, split), kStageBlocks);
+        q.split = ceil_div(q.kblocks, q.kb_per_split);
+        if (i == 0) slices = q.split;
+      } else if (i == l.pieces - 1) {
+        q.out16 = dX; q.ld_out = H; q.scale = scale;
+      }
       if (int rc = operand_map(&tm[2 * n], dl, cols, M, l.ld_dl, false, 128, &q.a_wide)) return rc;
       if (int rc = operand_map(&tm[2 * n + 1], Wp, H, cols, ldw, true, q.bn / 2, &q.b_wide)) return rc;
-      p.total_tiles += q.tiles_m * q.tiles_n;
+      p.total_tiles += q.tiles_m * q.tiles_n * q.split;
       ++n;
     }
     if (dW != nullptr) {                              // dW[cols, H] = d^T[cols, M] X[M, H]
@@ -347,6 +415,13 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
     p.num_problems = n;
     if (n == 1) { tm[2] = tm[0]; tm[3] = tm[1]; }
     if (int rc = launch_pair<PAIR_STORE>(d, p, tm, stream)) return rc;
+  }
+  if (slices > 0) {
+    const long long threads = (long long)M * (l.ld_acc / 4);
+    xent_dx_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(reinterpret_cast<const float*>(ws + l.acc), slices, l.acc_slice,
+                                                                           l.ld_acc, M, H, scale, reinterpret_cast<uint16_t*>(dX), bf16);
+    MP_HOST_CUDA_TRY(cudaGetLastError());
+    host_count_launches(1);
   }
   return MP_OK;
 }

@@ -137,6 +137,10 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
 // Registers per thread of a warpgroup from here on.  The launch has 384 x 168; 128 x 88 + 256 x 208 is just that.
 __device__ __forceinline__ void regs_fewer_88() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 __device__ __forceinline__ void regs_more_208() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+// mbar_wait by a whole warp, with one answer for it.
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code)) != 0;
+}
 __device__ __forceinline__ float exp2_approx(float x) {        // 2^x, 2 ulp, subnormal results flushed to zero
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -177,13 +181,23 @@ __device__ __forceinline__ void store_row32(uint16_t* o, const float (&v)[32], i
 // One stage of one operand: `rows` row indices from r0, contraction blocks kb ... kb + kc - 1.  K-major: [block][row][128 B];
 // MN-major: [64 row indices][kc * 64 contraction indices][128 B].  Blocks past the end of the contraction are filled with
 // zeros and count their bytes like the others.
+template <bool PAIR = true>
 __device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int mn, int wide, int rows, int r0, int kb, int kc) {
+  const auto load2 = [&](uint32_t d, int x, int y) {
+    if constexpr (PAIR) tma_load_2d_pair(d, tm, bar, x, y);
+    else tma_load_2d(d, tm, bar, x, y);
+  };
+  const auto load3 = [&](uint32_t d, int x, int y, int z) {
+    if constexpr (PAIR) tma_load_3d_pair(d, tm, bar, x, y, z);
+    else tma_load_3d(d, tm, bar, x, y, z);
+  };
   if (mn) {
-    if (wide) tma_load_3d_pair(dst, tm, bar, 0, kb * 64, r0 >> 6);
-    else for (int j = 0; j < rows; j += 64) tma_load_2d_pair(dst + (uint32_t)(j * kc * 128), tm, bar, r0 + j, kb * 64);
+    if (wide) load3(dst, 0, kb * 64, r0 >> 6);
+    else for (int j = 0; j < rows; j += 64) load2(dst + (uint32_t)(j * kc * 128), r0 + j, kb * 64);
+  } else if (wide) {
+    load3(dst, 0, r0, kb);
   } else {
-    if (wide) tma_load_3d_pair(dst, tm, bar, 0, r0, kb);
-    else for (int c = 0; c < kc; ++c) tma_load_2d_pair(dst + (uint32_t)(c * rows * 128), tm, bar, (kb + c) * 64, r0);
+    for (int c = 0; c < kc; ++c) load2(dst + (uint32_t)(c * rows * 128), (kb + c) * 64, r0);
   }
 }
 
@@ -383,7 +397,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 40);
   constexpr bool DYNAMIC = EPI == PAIR_STORE;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
   int* status = p.status;
@@ -441,11 +455,22 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
       if (!ok) settle_copies();
     }
     // ---------------------------------------------------------------------------- MMA issuer (one lane of rank 0's warp)
-    if (warp == 1 && lane == 0 && rank == 0) {
+    // The whole warp walks the loop and one elected lane issues: the operands of the instructions are then uniform values,
+    // which the compiler keeps where the instruction takes them from; a loop inside one lane's branch moves every descriptor
+    // there first (46 cycles per instruction).
+    if (warp == 1 && rank == 0) {
       int s = 0;
       uint32_t ph = 0, ui = 0;
       bool ok = true;
-      for (int unit; ok && (unit = units.next()) >= 0;) {
+      while (ok) {
+        int unit;
+        if constexpr (DYNAMIC) {
+          unit = lane == 0 ? units.next() : 0;
+          unit = __shfl_sync(0xffffffffu, unit, 0);
+        } else {
+          unit = units.next();
+        }
+        if (unit < 0) break;
         const PairUnit u = pair_unit(p, unit);
         const PairProblem& q = p.prob[u.prob];
         const uint32_t idesc = umma_idesc(1u, p.bf16 ? 1u : 0u, kPairRows, (uint32_t)q.bn) | ((uint32_t)q.a_mn << 15) | ((uint32_t)q.b_mn << 16);
@@ -461,26 +486,31 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         // an accumulator takes the whole contraction, or a chunk of it (PAIR_LSE)
         const int chunk = EPI == PAIR_LSE ? kLseChunk : q.kblocks;
         for (int k0 = u.kb0; ok && k0 < u.kb1; k0 += chunk, ++ui) {
-        const uint32_t buf = ui & 1u, use = ui >> 1;
-        if (!mbar_wait(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + buf * (uint32_t)kPairMaxBN;
-        const int k1 = min(u.kb1, k0 + chunk);
-        uint32_t first = 0u;
-        for (int kb = k0; kb < k1; kb += p.kc) {
-          if (!mbar_wait(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+          const uint32_t buf = ui & 1u, use = ui >> 1;
+          if (!wait_all(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
           tc_fence_after();
-          uint64_t ad = a_base + (uint64_t)((uint32_t)s * stage16), bd = b_base + (uint64_t)((uint32_t)s * stage16);
-          const int nc = min(p.kc, k1 - kb);
-          for (int c = 0; c < nc; ++c, ad += a_blk, bd += b_blk) {
+          const uint32_t d_tmem = tmem_base + buf * (uint32_t)kPairMaxBN;
+          const int k1 = min(u.kb1, k0 + chunk);
+          uint32_t more = 0u;
+          for (int kb = k0; kb < k1; kb += p.kc) {
+            if (!wait_all(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+            tc_fence_after();
+            uint64_t ad = a_base + (uint64_t)((uint32_t)s * stage16), bd = b_base + (uint64_t)((uint32_t)s * stage16);
+            const int nc = min(p.kc, k1 - kb);
+            if (elect_one()) {
+              for (int c = 0; c < nc; ++c, ad += a_blk, bd += b_blk) {
 #pragma unroll
-            for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_pair(d_tmem, ad + kk * a_step, bd + kk * b_step, idesc, kk > 0 ? 1u : first);
-            first = 1u;
+                for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_pair(d_tmem, ad + kk * a_step, bd + kk * b_step, idesc, kk > 0 ? 1u : more);
+                more = 1u;
+              }
+              tc_commit_pair(empty_bar(s));
+            }
+            __syncwarp();
+            more = 1u;
+            if (++s == stages) { s = 0; ph ^= 1u; }
           }
-          tc_commit_pair(empty_bar(s));
-          if (++s == stages) { s = 0; ph ^= 1u; }
-        }
-        if (ok) tc_commit_pair(tfull_bar((int)buf));
+          if (ok && elect_one()) tc_commit_pair(tfull_bar((int)buf));
+          __syncwarp();
         }
       }
     }

@@ -21,7 +21,7 @@ constexpr int kW4StreamMaxTokens = 16;
 constexpr int kSmsModel = 148;            // workspace sizes must not depend on the device that is asked
 
 struct Plan {
-  bool stream;
+  bool stream, pair;
   int bn, tiles_m, tiles_n, steps, split, steps_per_split;
   size_t copy, partial, total;            // workspace: aligned copy of the tokens, partial sums
   long long ld_copy, ld_partial;
@@ -41,12 +41,13 @@ Plan w4_plan(int T, int N, int K, bool grad, bool copy_tokens) {
   }
   if (p.stream) return p;
   p.bn = T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
-  p.tiles_m = ceil_div(rows, kPairRows);
+  p.pair = p.bn == 256;
+  p.tiles_m = ceil_div(rows, p.pair ? 256 : 128);
   p.tiles_n = ceil_div(T, p.bn);
   p.steps = ceil_div(contraction, 128);
-  // few tiles: cut the contraction so that every pair of SMs has work, in pieces of at least four steps
-  const int tiles = p.tiles_m * p.tiles_n, pairs = kSmsModel / 2;
-  int split = std::max(1, std::min(pairs / std::max(tiles, 1), p.steps / 4));
+  // few tiles: cut the contraction so that every SM (pair) has work, in pieces of at least four steps
+  const int tiles = p.tiles_m * p.tiles_n, slots = p.pair ? kSmsModel / 2 : kSmsModel;
+  int split = std::max(1, std::min(slots / std::max(tiles, 1), p.steps / 4));
   p.steps_per_split = ceil_div(p.steps, split);
   p.split = ceil_div(p.steps, p.steps_per_split);
   if (p.split > 1) {
@@ -155,7 +156,7 @@ int run_stream(const HostDevice& d, const W4StreamParams& p, cudaStream_t stream
 }
 
 template <bool BF16>
-int run_pair(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, int T, const void* x, long long ldx, const void* bias,
+int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, int T, const void* x, long long ldx, const void* bias,
              void* out, uint8_t* ws, cudaStream_t stream) {
   W4PairParams p{};
   p.w = w;
@@ -171,12 +172,13 @@ int run_pair(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, i
   p.partial = reinterpret_cast<float*>(ws + l.partial);
   p.ld_partial = l.ld_partial;
   p.status = d.status;
-  p.stage_bytes = kW4ABytes + l.bn / 2 * 256;
+  const int hb = l.pair ? l.bn / 2 : l.bn;
+  p.stage_bytes = kW4ABytes + hb * 256;
   // three stages, and the rest of the shared memory for packed bytes on their way from HBM
   p.stages = 3;
-  p.raw_slots = std::min(kW4MaxRawSlots, (kPairSmem - 1024 - 512 - p.stages * p.stage_bytes) / kW4RawBytes);
+  p.raw_slots = std::min(kW4MaxRawSlots, (kPairSmem - 1024 - 256 - p.stages * p.stage_bytes) / kW4RawBytes);
   p.vec = vector_groups(w);
-  const int contraction = grad ? w.N : w.K, hb = l.bn / 2;
+  const int contraction = grad ? w.N : w.K;
   CUtensorMap tmB, tmW;
   p.b_wide = contraction % 64 == 0;
   if (p.b_wide) {
@@ -184,17 +186,39 @@ int run_pair(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, i
   } else {
     if (int rc = host_tmap(&tmB, kTmap16, x, contraction, T, ldx * 2, 64, hb, 128)) return rc;
   }
-  if (int rc = host_tmap(&tmW, kTmapByte, w.packed, (long long)w.blocks * 64, w.N, (long long)w.blocks * 64, 64, 128, 64)) return rc;
+  const int line = grad ? 64 : 128;                      // packed bytes per row and box
+  if (int rc = host_tmap(&tmW, kTmapByte, w.packed, (long long)w.blocks * 64, w.N, (long long)w.blocks * 64, line, 128, line)) return rc;
   const bool fine = w.shift < 2;
-  auto kern = fine ? w4_pair_kernel<BF16, true> : w4_pair_kernel<BF16, false>;
-  static bool ready[64][2] = {};
-  if (!ready[d.index & 63][fine]) {
+  auto kern = l.pair ? (fine ? w4_mma_kernel<BF16, true, true> : w4_mma_kernel<BF16, false, true>)
+                     : (fine ? w4_mma_kernel<BF16, true, false> : w4_mma_kernel<BF16, false, false>);
+  static bool ready[64][4] = {};
+  bool& done = ready[d.index & 63][l.pair * 2 + fine];
+  if (!done) {
     MP_HOST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-    ready[d.index & 63][fine] = true;
+    done = true;
   }
-  const int pairs = std::max(1, std::min(p.tiles_m * p.tiles_n * p.split, d.sms / 2));
-  kern<<<2 * pairs, kW4Threads, kPairSmem, stream>>>(tmB, tmW, p);
-  MP_HOST_CUDA_TRY(cudaGetLastError());
+  const int ctas = l.pair ? 2 : 1;
+  cudaLaunchConfig_t run = {};
+  run.gridDim = dim3((unsigned)(ctas * std::max(1, std::min(p.tiles_m * p.tiles_n * p.split, d.sms / ctas))));
+  run.blockDim = dim3(kW4Threads);
+  run.dynamicSmemBytes = kPairSmem;
+  run.stream = stream;
+  cudaLaunchAttribute early[2];
+  int num = 0;
+  if (l.pair) {
+    early[num].id = cudaLaunchAttributeClusterDimension;
+    early[num].val.clusterDim.x = 2;
+    early[num].val.clusterDim.y = early[num].val.clusterDim.z = 1;
+    ++num;
+  }
+  if (host_use_pdl()) {
+    early[num].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early[num].val.programmaticStreamSerializationAllowed = 1;
+    ++num;
+  }
+  run.attrs = early;
+  run.numAttrs = num;
+  MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&run, kern, tmB, tmW, p));
   host_count_launches(1);
   if (p.split > 1) {
     const long long threads = (long long)T * (l.ld_partial / 4);
@@ -246,8 +270,8 @@ int run_w4(const char* op, bool grad, int dtype, int M, int N, int K, const void
     p.T = M;
     return dtype == MP_BF16 ? run_stream<true>(d, p, stream) : run_stream<false>(d, p, stream);
   }
-  return dtype == MP_BF16 ? run_pair<true>(d, l, w, grad, M, X, ldx, bias, out, ws, stream)
-                          : run_pair<false>(d, l, w, grad, M, X, ldx, bias, out, ws, stream);
+  return dtype == MP_BF16 ? run_mma<true>(d, l, w, grad, M, X, ldx, bias, out, ws, stream)
+                          : run_mma<false>(d, l, w, grad, M, X, ldx, bias, out, ws, stream);
 }
 
 }  // namespace

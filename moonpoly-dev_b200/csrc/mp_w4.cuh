@@ -10,8 +10,8 @@
 // subtraction (or a multiply-add with 1 / 16) gives q - zero exactly; for bf16, 0x4300 | q is 128 + q.
 //
 // Two kernels.  Up to 16 tokens: w4_stream_kernel, warp-level MMAs on q - zero, exact in 16 bits, with the scale applied to
-// 32-bit sums -- bound by reading the weight.  More tokens, and the gradient of the input: w4_pair_kernel, CTA-pair tcgen05
-// tiles whose weight operand is unpacked into shared memory by eight warps while the tensor cores work on earlier stages.
+// 32-bit sums -- bound by reading the weight.  More tokens, and the gradient of the input: w4_mma_kernel, tcgen05 tiles whose
+// weight operand is unpacked into shared memory by sixteen warps while the tensor cores work on earlier stages.
 #pragma once
 #include <type_traits>
 
@@ -308,17 +308,20 @@ __global__ void __launch_bounds__(kW4StreamWarps * 32, 1) w4_stream_kernel(const
   }
 }
 
-// ----------------------------------------------------------------------------------------- more tokens: CTA-pair tiles
-// D[256 rows x bn tokens], rows = output channels (forward, contraction K) or input features (gradient, contraction N).
-// A stage is 128 contraction elements: 32 KB of unpacked weight and bn / 2 token rows per CTA.  Both directions unpack the
+// ------------------------------------------------------------------------------------------------ more tokens: tcgen05
+// D[rows x bn tokens], rows = output channels (forward, contraction K) or input features (gradient, contraction N): 128 rows
+// per CTA.  PAIR: two CTAs share a 256 x 256 tile (cta_group::2, each loads half of the tokens), which halves the token
+// traffic where the tensor cores are the bound.  Alone: 128 x bn tiles with bn <= 128; with so few tokens a step is
+// over in 300 cycles, and the hand-over between two CTAs (550 cycles a step measured with four stages) and the pair's
+// 78 cycles per instruction at 64 tokens would be the bound.
+// A step is 128 contraction elements: 32 KB of unpacked weight and the tokens' 256 bytes each.  Both directions unpack the
 // same thing -- 128 rows of W by one block of 128 k -- into the same swizzled lines of 64 k; forward, the lines are a K-major
 // operand (line = row of D), in the gradient an MN-major one (line = contraction index).
 // Warps: 0 = TMA of the tokens, 1 = MMA, 2 = TMA of the packed weight, 4..7 = epilogue, 8..15 and 16..23 = unpacking, two
-// groups that take alternate stages: a stage's chain (packed bytes, conversion, stores, proxy fence, arrival) lasts about
-// 1600 cycles and its MMAs 1024.
+// groups that take turns of two steps.
 constexpr int kW4Threads = 768;
-constexpr int kW4RawBytes = 128 * 64;         // packed bytes per stage and CTA
-constexpr int kW4MaxRawSlots = 12;
+constexpr int kW4RawBytes = 2 * 128 * 64;     // packed bytes per turn and CTA
+constexpr int kW4MaxRawSlots = 6;
 constexpr int kW4ABytes = 128 * 256;
 
 struct W4PairParams {
@@ -339,7 +342,7 @@ struct W4PairParams {
 struct W4Unit { int tm, tn, s0, s1, slice; };
 __device__ __forceinline__ W4Unit w4_unit(const W4PairParams& p, int unit) {
   W4Unit u;
-  u.tn = unit % p.tiles_n;                    // neighbouring pairs share the weight's tile
+  u.tn = unit % p.tiles_n;                    // neighbours share the weight's tile
   const int r = unit / p.tiles_n;
   u.slice = r % p.split;
   u.tm = r / p.split;
@@ -360,15 +363,14 @@ template <bool BF16> __device__ __forceinline__ uint4 w4_weights(uint32_t word, 
 }
 
 // FINE: groups of 32 or 64, so the runs of a block have scales of their own.
-template <bool BF16, bool FINE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
-w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmW, const W4PairParams p) {
+template <bool BF16, bool FINE, bool PAIR>
+__global__ void __launch_bounds__(kW4Threads, 1)
+w4_mma_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmW, const W4PairParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t smem_base = smem_u32(smem);
-  const int stages = p.stages;
+  const int stages = p.stages, raw_slots = p.raw_slots;
   const uint32_t raw_base = smem_base + (uint32_t)stages * (uint32_t)p.stage_bytes;
-  const int raw_slots = p.raw_slots;
   const uint32_t bar_base = raw_base + (uint32_t)raw_slots * kW4RawBytes;
   auto full_bar = [&](int s) { return bar_base + 8u * (uint32_t)s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (uint32_t)(stages + s); };
@@ -376,45 +378,60 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
   auto tempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 2 + b); };
   auto rfull_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 4 + b); };
   auto rempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 4 + raw_slots + b); };
-  const uint32_t slot_off = bar_base - smem_base + 8u * (uint32_t)(2 * stages + 4 + 2 * raw_slots);
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + slot_off);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (bar_base - smem_base) + 8u * (uint32_t)(2 * stages + 4 + 2 * raw_slots));
+  // barriers that the MMA issuer waits on live in rank 0 of a pair
+  auto at_leader = [&](uint32_t bar) { return PAIR ? mapa_shared(bar, 0) : bar; };
+  auto arrive = [&](uint32_t bar) {
+    if constexpr (PAIR) mbar_arrive_pair(mapa_shared(bar, 0));
+    else mbar_arrive(bar);
+  };
+  auto commit = [&](uint32_t bar) {
+    if constexpr (PAIR) tc_commit_pair(bar);
+    else tc_commit(bar);
+  };
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
-  const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+  constexpr int kCtas = PAIR ? 2 : 1, kRows = 128 * kCtas;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const int first = (int)blockIdx.x / kCtas, stride = (int)gridDim.x / kCtas;       // units of this CTA (pair)
   const int units = p.tiles_m * p.tiles_n * p.split;
   int* status = p.status;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 17); mbar_init(empty_bar(s), 1); }   // 1 + 8 unpacking warps per CTA
-    for (int b = 0; b < 2; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), 8); }
+    for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 1 + 8 * kCtas); mbar_init(empty_bar(s), 1); }   // TMA + unpacking warps
+    for (int b = 0; b < 2; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), 4 * kCtas); }
     for (int b = 0; b < raw_slots; ++b) { mbar_init(rfull_bar(b), 1); mbar_init(rempty_bar(b), 8); }
     mbar_fence_init();
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmW);
   }
-  if (warp == 1) tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+  if (warp == 1) {
+    if constexpr (PAIR) tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    else { tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512); tmem_relinquish(); }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  cluster_sync_all();
+  if constexpr (PAIR) cluster_sync_all();
+  // Everything above may overlap the previous kernel of the stream; nothing of it is read or overwritten before it is done.
   griddep_launch_dependents();
+  griddep_wait();
 
-  const int hb = p.bn >> 1;
+  const int hb = p.bn / kCtas;                          // token rows per CTA
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------------------ TMA: tokens
     if (lane == 0) {
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int unit = pair; ok && unit < units; unit += pairs) {
+      for (int unit = first; ok && unit < units; unit += stride) {
         const W4Unit u = w4_unit(p, unit);
         const int b0 = u.tn * p.bn + (int)rank * hb;
         for (int st = u.s0; st < u.s1; ++st) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
-          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2u * (uint32_t)(hb * 256));
-          pair_load(smem_base + (uint32_t)s * (uint32_t)p.stage_bytes + kW4ABytes, &tmB, mapa_shared(full_bar(s), 0), 0, p.b_wide, hb, b0, st * 2, 2);
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), (uint32_t)(kCtas * hb * 256));
+          pair_load<PAIR>(smem_base + (uint32_t)s * (uint32_t)p.stage_bytes + kW4ABytes, &tmB, at_leader(full_bar(s)), 0, p.b_wide, hb, b0, st * 2, 2);
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
       }
@@ -426,35 +443,45 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------------------------------------------ MMA (rank 0)
-    if (lane == 0 && rank == 0) {
+    // The whole warp walks the loop and one elected lane issues: the operands of the instructions are then uniform values,
+    // which the compiler keeps where the instruction takes them from; a loop inside one lane's branch moves every descriptor
+    // there first (46 cycles per instruction).
+    if (rank == 0) {
       int s = 0;
       uint32_t ph = 0, ui = 0;
       bool ok = true;
-      const uint32_t idesc = umma_idesc(1u, BF16 ? 1u : 0u, kPairRows, (uint32_t)p.bn) | ((uint32_t)p.grad << 15);
+      const uint32_t idesc = umma_idesc(1u, BF16 ? 1u : 0u, kRows, (uint32_t)p.bn) | ((uint32_t)p.grad << 15);
       const uint64_t a_base = p.grad ? umma_smem_desc_mn(smem_base, 16384u) : umma_smem_desc_sw128(smem_base);
       const uint64_t b_base = umma_smem_desc_sw128(smem_base) + (kW4ABytes >> 4);
       const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4;
-      for (int unit = pair; ok && unit < units; unit += pairs, ++ui) {
+      // 64 contraction elements further: the next block of K-major lines, or 64 MN-major lines; 16: 32 bytes, or 16 lines
+      const uint32_t a_step = p.grad ? 2048u >> 4 : 2u, a_blk = p.grad ? 8192u >> 4 : 16384u >> 4, b_blk = (uint32_t)hb * 128u >> 4;
+      for (int unit = first; ok && unit < units; unit += stride, ++ui) {
         const W4Unit u = w4_unit(p, unit);
         const uint32_t buf = ui & 1u, use = ui >> 1;
-        if (!mbar_wait(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
+        if (!wait_all(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * (uint32_t)kPairMaxBN;
+        uint32_t more = 0u;
         for (int st = u.s0; st < u.s1; ++st) {
-          if (!mbar_wait(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
+          if (!wait_all(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
           tc_fence_after();
           const uint64_t ad = a_base + (uint64_t)((uint32_t)s * stage16), bd = b_base + (uint64_t)((uint32_t)s * stage16);
+          if (elect_one()) {
 #pragma unroll
-          for (uint32_t kk = 0; kk < 8; ++kk) {
-            // 16 contraction elements further: 32 bytes of a K-major line (the next 16 KB block after four), 16 MN-major lines
-            const uint32_t a_off = p.grad ? kk * (2048u >> 4) : (kk >> 2) * (16384u >> 4) + (kk & 3u) * 2u;
-            const uint32_t b_off = (kk >> 2) * ((uint32_t)hb * 128u >> 4) + (kk & 3u) * 2u;
-            umma_f16_pair(d_tmem, ad + a_off, bd + b_off, idesc, (st > u.s0 || kk > 0) ? 1u : 0u);
+            for (uint32_t kk = 0; kk < 8; ++kk) {
+              const uint64_t da = ad + (kk >> 2) * a_blk + (kk & 3u) * a_step, db = bd + (kk >> 2) * b_blk + (kk & 3u) * 2u;
+              if constexpr (PAIR) umma_f16_pair(d_tmem, da, db, idesc, kk > 0 ? 1u : more);
+              else umma_f16(d_tmem, da, db, idesc, kk > 0 ? 1u : more);
+            }
+            commit(empty_bar(s));
           }
-          tc_commit_pair(empty_bar(s));
+          __syncwarp();
+          more = 1u;
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
-        if (ok) tc_commit_pair(tfull_bar((int)buf));
+        if (ok && elect_one()) commit(tfull_bar((int)buf));
+        __syncwarp();
       }
     }
   } else if (warp == 2) {
@@ -463,14 +490,18 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
       int rs = 0;
       uint32_t rph = 0;
       bool ok = true;
-      for (int unit = pair; ok && unit < units; unit += pairs) {
+      for (int unit = first; ok && unit < units; unit += stride) {
         const W4Unit u = w4_unit(p, unit);
-        for (int st = u.s0; st < u.s1; ++st) {
+        for (int st = u.s0; st < u.s1; st += 2) {
           if (!mbar_wait(rempty_bar(rs), rph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
           mbar_arrive_expect_tx(rfull_bar(rs), kW4RawBytes);
-          const int blk = p.grad ? u.tm * 2 + (int)rank : st;
-          const int row = p.grad ? st * 128 : u.tm * kPairRows + (int)rank * 128;
-          tma_load_2d(raw_base + (uint32_t)rs * kW4RawBytes, &tmW, rfull_bar(rs), blk * 64, row);
+          const uint32_t dst = raw_base + (uint32_t)rs * kW4RawBytes;
+          if (p.grad) {                                  // two tiles of 128 rows, one block wide
+            tma_load_2d(dst, &tmW, rfull_bar(rs), (u.tm * kCtas + (int)rank) * 64, st * 128);
+            tma_load_2d(dst + kW4RawBytes / 2, &tmW, rfull_bar(rs), (u.tm * kCtas + (int)rank) * 64, st * 128 + 128);
+          } else {                                       // one tile, two blocks wide
+            tma_load_2d(dst, &tmW, rfull_bar(rs), st * 64, u.tm * kRows + (int)rank * 128);
+          }
           if (++rs == raw_slots) { rs = 0; rph ^= 1u; }
         }
       }
@@ -478,29 +509,22 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
     }
   } else if (warp >= 8) {
     // -------------------------------------------------------------------------------------------------------- unpacking
-    // a lane takes the 16-byte chunk t of two rows 8 apart: eight neighbouring lanes are eight rows, which the 64-byte
-    // swizzle of the packed tile and the 128-byte swizzle of the operand both spread over all banks
+    // A lane takes the 16-byte chunk t of two rows 8 apart: eight neighbouring lanes are eight rows, which the swizzles of the
+    // packed tile (64 or 128 bytes) and of the operand (128 bytes) all spread over the banks.
     const int group = (warp - 8) >> 3, r0 = ((warp - 8) & 7) * 16 + (lane & 7), t = lane >> 3;
-    const uint32_t raw_off = raw_base + (uint32_t)(r0 * 64 + ((t ^ ((r0 >> 1) & 3)) << 4));
-    const uint32_t even_off = smem_base + (uint32_t)(r0 * 128 + ((t ^ (r0 & 7)) << 4)), odd_off = even_off ^ 64u;   // runs 0, 2 and 1, 3
+    const uint32_t raw0 = raw_base + (uint32_t)(p.grad ? r0 * 64 + ((t ^ ((r0 >> 1) & 3)) << 4) : r0 * 128 + ((t ^ (r0 & 7)) << 4));
+    const uint32_t raw1 = p.grad ? raw0 + kW4RawBytes / 2 : raw0 ^ 64u;              // second step of the turn
+    const uint32_t rows8 = p.grad ? 512u : 1024u;                                    // eight rows further
+    const uint32_t even_at = smem_base + (uint32_t)(r0 * 128 + ((t ^ (r0 & 7)) << 4)), odd_at = even_at ^ 64u;   // runs 0, 2 and 1, 3
     const uint32_t magic = w4_magic<BF16>();
-    int s = group, rs = group;                          // the host gives at least two of each
-    uint32_t ph = 0, rph = 0;
     const W4Weight& w = p.w;
     constexpr int R = FINE ? 4 : 1;                     // groups that a block of a row meets
-    // This CTA pair's steps, one after the other across its units.
-    struct Step { int unit, st; W4Unit u; };
-    const auto advance = [&](Step& x) {
-      if (++x.st < x.u.s1) return;
-      x.unit += pairs;
-      if (x.unit < units) { x.u = w4_unit(p, x.unit); x.st = x.u.s0; }
-    };
     uint32_t sz[2][R];                                  // scale | zero << 16
     // Scales and zeros of the lane's two rows, a step ahead of their use.  Weights that do not exist (rows past N, runs past
     // K) get scale 0: they are zero whatever their bits say.
-    const auto fetch = [&](const Step& x) {
-      const int blk = p.grad ? x.u.tm * 2 + (int)rank : x.st;
-      const int row = (p.grad ? x.st * 128 : x.u.tm * kPairRows + (int)rank * 128) + r0;
+    const auto fetch = [&](int tm, int st) {
+      const int blk = p.grad ? tm * kCtas + (int)rank : st;
+      const int row = (p.grad ? st * 128 : tm * kRows + (int)rank * 128) + r0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const long long line = (long long)(row + 8 * h) * w.groups;
@@ -535,54 +559,84 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
         }
       }
     };
-    Step cur{pair, 0, {}};
-    if (pair < units) {
-      cur.u = w4_unit(p, pair);
-      cur.st = cur.u.s0;
-      if (group) advance(cur);
-      if (cur.unit < units) fetch(cur);
-    }
-    while (cur.unit < units) {
-      uint32_t scale[2][R];
-      W4Zero zero[2][R];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < R; ++i) { scale[h][i] = (sz[h][i] & 0xffffu) * 0x10001u; zero[h][i] = w4_zero<BF16>(sz[h][i] >> 16); }
-      Step nxt = cur;
-      advance(nxt);
-      if (nxt.unit < units) advance(nxt);
-      if (nxt.unit < units) fetch(nxt);
+    // This CTA's turns (two steps, or the odd last one of a unit), dealt to the two groups alternately across the units.
+    struct Turn { int unit, st, s1, tm; };
+    const auto open_unit = [&](Turn& x) {
+      if (x.unit < units) { const W4Unit u = w4_unit(p, x.unit); x.st = u.s0; x.s1 = u.s1; x.tm = u.tm; }
+    };
+    // To the next turn; returns the steps of this one that a stage counter has to pass over.
+    const auto advance = [&](Turn& x) {
+      const int n = min(2, x.s1 - x.st);
+      x.st += 2;
+      if (x.st >= x.s1) { x.unit += stride; open_unit(x); }
+      return n;
+    };
+    int s = 0, rs = 0;
+    uint32_t ph = 0, rph = 0;
+    const auto pass = [&](int n) {                       // n stages and one slot further
+      s += n;
+      if (s >= stages) { s -= stages; ph ^= 1u; }
+      if (++rs == raw_slots) { rs = 0; rph ^= 1u; }
+    };
+    Turn cur{first, 0, 0, 0};
+    open_unit(cur);
+    if (group == 1 && cur.unit < units) pass(advance(cur));
+    if (cur.unit < units) fetch(cur.tm, cur.st);
+    bool ok = true;
+    while (ok && cur.unit < units) {
+      Turn nxt = cur;
+      const int mine = advance(nxt);
+      int theirs = 0;
+      if (nxt.unit < units) theirs = advance(nxt);
       if (!mbar_wait(rfull_bar(rs), rph, status, MP_DEV_TIMEOUT_MMA_FULL)) break;
-      const uint4 q0 = ld_smem_v4<0>(raw_off + (uint32_t)rs * kW4RawBytes), q1 = ld_smem_v4<512>(raw_off + (uint32_t)rs * kW4RawBytes);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(rempty_bar(rs));
-      if ((rs += 2) >= raw_slots) { rs -= raw_slots; rph ^= 1u; }
-      if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) break;
-      const uint32_t ev = even_off + (uint32_t)s * (uint32_t)p.stage_bytes, od = odd_off + (uint32_t)s * (uint32_t)p.stage_bytes;
-      // the weight in the operand type: one rounding of the exact product (q - zero) * scale
-      st_smem_v4<0>(ev, w4_weights<BF16>(q0.x, magic, zero[0][0], scale[0][0]));
-      st_smem_v4<0>(od, w4_weights<BF16>(q0.y, magic, zero[0][1 % R], scale[0][1 % R]));
-      st_smem_v4<16384>(ev, w4_weights<BF16>(q0.z, magic, zero[0][2 % R], scale[0][2 % R]));
-      st_smem_v4<16384>(od, w4_weights<BF16>(q0.w, magic, zero[0][3 % R], scale[0][3 % R]));
-      st_smem_v4<1024>(ev, w4_weights<BF16>(q1.x, magic, zero[1][0], scale[1][0]));
-      st_smem_v4<1024>(od, w4_weights<BF16>(q1.y, magic, zero[1][1 % R], scale[1][1 % R]));
-      st_smem_v4<17408>(ev, w4_weights<BF16>(q1.z, magic, zero[1][2 % R], scale[1][2 % R]));
-      st_smem_v4<17408>(od, w4_weights<BF16>(q1.w, magic, zero[1][3 % R], scale[1][3 % R]));
-      fence_async_smem();                              // the tensor cores read through the async proxy
-      __syncwarp();
-      if (lane == 0) mbar_arrive_pair(mapa_shared(full_bar(s), 0));
-      if ((s += 2) >= stages) { s -= stages; ph ^= 1u; }
+      const uint32_t slot = (uint32_t)rs * kW4RawBytes;
+      int sh = s;
+      uint32_t phh = ph;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (half >= mine) break;
+        uint32_t scale[2][R];
+        W4Zero zero[2][R];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < R; ++i) { scale[h][i] = (sz[h][i] & 0xffffu) * 0x10001u; zero[h][i] = w4_zero<BF16>(sz[h][i] >> 16); }
+        if (half + 1 < mine) fetch(cur.tm, cur.st + 1);
+        else if (nxt.unit < units) fetch(nxt.tm, nxt.st);
+        const uint32_t from = (half == 0 ? raw0 : raw1) + slot;
+        const uint4 q0 = ld_smem_v4<0>(from), q1 = ld_smem_v4<0>(from + rows8);
+        if (half + 1 == mine) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(rempty_bar(rs));
+        }
+        if (!mbar_wait(empty_bar(sh), phh ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
+        const uint32_t ev = even_at + (uint32_t)sh * (uint32_t)p.stage_bytes, od = odd_at + (uint32_t)sh * (uint32_t)p.stage_bytes;
+        // the weight in the operand type: one rounding of the exact product (q - zero) * scale
+        st_smem_v4<0>(ev, w4_weights<BF16>(q0.x, magic, zero[0][0], scale[0][0]));
+        st_smem_v4<0>(od, w4_weights<BF16>(q0.y, magic, zero[0][1 % R], scale[0][1 % R]));
+        st_smem_v4<16384>(ev, w4_weights<BF16>(q0.z, magic, zero[0][2 % R], scale[0][2 % R]));
+        st_smem_v4<16384>(od, w4_weights<BF16>(q0.w, magic, zero[0][3 % R], scale[0][3 % R]));
+        st_smem_v4<1024>(ev, w4_weights<BF16>(q1.x, magic, zero[1][0], scale[1][0]));
+        st_smem_v4<1024>(od, w4_weights<BF16>(q1.y, magic, zero[1][1 % R], scale[1][1 % R]));
+        st_smem_v4<17408>(ev, w4_weights<BF16>(q1.z, magic, zero[1][2 % R], scale[1][2 % R]));
+        st_smem_v4<17408>(od, w4_weights<BF16>(q1.w, magic, zero[1][3 % R], scale[1][3 % R]));
+        fence_async_smem();                              // the tensor cores read through the async proxy
+        __syncwarp();
+        if (lane == 0) arrive(full_bar(sh));
+        if (++sh == stages) { sh = 0; phh ^= 1u; }
+      }
+      pass(mine);
+      if (theirs) pass(theirs);
       cur = nxt;
     }
   } else if (warp >= 4) {
     // --------------------------------------------------------------------------------------------------------- epilogue
     const int quad = warp & 3;
     uint32_t ui = 0;
-    for (int unit = pair; unit < units; unit += pairs, ++ui) {
+    for (int unit = first; unit < units; unit += stride, ++ui) {
       const W4Unit u = w4_unit(p, unit);
       const uint32_t buf = ui & 1u, use = ui >> 1;
-      const int row = u.tm * kPairRows + (int)rank * 128 + quad * 32 + lane;
+      const int row = u.tm * kRows + (int)rank * 128 + quad * 32 + lane;
       const bool live = row < p.rows;
       const float bias = live && p.bias != nullptr ? from16<BF16>(p.bias[row]) : 0.0f;
       if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
@@ -608,17 +662,18 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ 
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));
+      if (lane == 0) arrive(tempty_bar((int)buf));
     }
   }
 
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  if constexpr (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem_base, 512);
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
   }
 }
 

@@ -89,7 +89,7 @@ int mp_linear_w4_grad_input(int dtype, int M, int N, int K, const void* dY, long
 
 /* Bytes of workspace that mp_linear_w4 (grad_input = 0) or mp_linear_w4_grad_input (1) needs; X (or dY) is only looked at for
  * its alignment.  256-byte aligned device memory, not initialised, not shared by calls or graph replays that can overlap. */
-int mp_linear_w4_workspace(int M, int N, int K, const void* X, long long ldx, int grad_input, size_t* bytes);
+int mp_linear_w4_workspace(int M, int N, int K, int group_size, const void* X, long long ldx, int grad_input, size_t* bytes);
 
 /* Linear with softmax cross entropy (no counterpart in the reference): the output layer of a language model and its
  * loss, without holding the logits.  z[M,V] = X[M,H] * W[V,H]^T with fp32 accumulation; for every row

@@ -23,14 +23,14 @@ constexpr int kSmsModel = 148;            // workspace sizes must not depend on 
 struct Plan {
   bool stream, pair;
   int bn, tiles_m, tiles_n, steps, split, steps_per_split;
-  size_t copy, partial, total;            // workspace: aligned copy of the tokens, partial sums
+  size_t copy, partial, table, total;     // workspace: aligned copy of the tokens, partial sums, group words
   long long ld_copy, ld_partial;
 };
 
 bool tokens_aligned(const void* x, long long ld) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld % 8 == 0; }
 
 // rows = output features of this direction, contraction = input features.
-Plan w4_plan(int T, int N, int K, bool grad, bool copy_tokens) {
+Plan w4_plan(int T, int N, int K, int group_size, bool grad, bool copy_tokens) {
   Plan p{};
   const int rows = grad ? K : N, contraction = grad ? N : K;
   p.stream = !grad && T <= kW4StreamMaxTokens;
@@ -40,16 +40,30 @@ Plan w4_plan(int T, int N, int K, bool grad, bool copy_tokens) {
     p.total += round_up((size_t)T * p.ld_copy * 2, 256);
   }
   if (p.stream) return p;
-  p.bn = T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
-  p.pair = p.bn == 256;
-  p.tiles_m = ceil_div(rows, p.pair ? 256 : 128);
-  p.tiles_n = ceil_div(T, p.bn);
   p.steps = ceil_div(contraction, 128);
-  // few tiles: cut the contraction so that every SM (pair) has work, in pieces of at least four steps
-  const int tiles = p.tiles_m * p.tiles_n, slots = p.pair ? kSmsModel / 2 : kSmsModel;
-  int split = std::max(1, std::min(slots / std::max(tiles, 1), p.steps / 4));
-  p.steps_per_split = ceil_div(p.steps, split);
+  p.pair = T > 128;
+  const int slots = p.pair ? kSmsModel / 2 : kSmsModel;
+  p.tiles_m = ceil_div(rows, p.pair ? 256 : 128);
+  // Tokens per tile (a multiple of 32) and slices of the contraction: the choice whose longest SM (pair) is done first.  A step
+  // of a tile costs four cycles per token on the tensor cores, or the 900 of the unpacking; a slice at least four steps, and
+  // eight for its sums to be written and joined.
+  double best = 0.0;
+  const int widest = p.pair ? 256 : 128, whole = (int)round_up((size_t)T, 32);
+  for (int bn = std::min(widest, whole); bn >= (p.pair ? 160 : std::min(widest, whole)); bn -= 32) {
+    const int tiles = p.tiles_m * ceil_div(T, bn);
+    for (int split = 1; split <= 16 && (split == 1 || p.steps / split >= 4) && (split == 1 || tiles * split <= slots); ++split) {
+      const int each = ceil_div(p.steps, split);
+      const double cost = (double)ceil_div(tiles * ceil_div(p.steps, each), slots) * (each + (split > 1 ? 8 : 0)) * std::max(4 * bn + 100, 900);
+      if (best == 0.0 || cost < best) { best = cost; p.bn = bn; p.split = split; }
+    }
+  }
+  p.tiles_n = ceil_div(T, p.bn);
+  p.steps_per_split = ceil_div(p.steps, p.split);
   p.split = ceil_div(p.steps, p.steps_per_split);
+  if (p.pair) {
+    p.table = p.total;
+    p.total += round_up((size_t)ceil_div(K, group_size) * N * 4, 256);
+  }
   if (p.split > 1) {
     p.ld_partial = (long long)round_up((size_t)rows, 32);
     p.partial = p.total;
@@ -186,6 +200,21 @@ int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, in
   } else {
     if (int rc = host_tmap(&tmB, kTmap16, x, contraction, T, ldx * 2, 64, hb, 128)) return rc;
   }
+  if (l.pair) {
+    p.table = reinterpret_cast<const uint32_t*>(ws + l.table);
+    p.ld_table = w.N;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ceil_div(w.N, 32), (unsigned)ceil_div(w.groups, 32));
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = host_use_pdl() ? 1 : 0;
+    MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&cfg, w4_table_kernel, w.scale, w.zero, w.N, w.groups, reinterpret_cast<uint32_t*>(ws + l.table), w.N));
+    host_count_launches(1);
+  }
   const int line = grad ? 64 : 128;                      // packed bytes per row and box
   if (int rc = host_tmap(&tmW, kTmapByte, w.packed, (long long)w.blocks * 64, w.N, (long long)w.blocks * 64, line, 128, line)) return rc;
   const bool fine = w.shift < 2;
@@ -245,7 +274,7 @@ int run_w4(const char* op, bool grad, int dtype, int M, int N, int K, const void
   if (M == 0) return MP_OK;
   if (out == nullptr) return host_fail(MP_ERR_INVALID_ARG, "%s: null output", op);
   const bool copy = !tokens_aligned(X, ldx);
-  const Plan l = w4_plan(M, N, K, grad, copy);
+  const Plan l = w4_plan(M, N, K, group_size, grad, copy);
   if (l.total > 0) {
     if (workspace == nullptr || workspace_bytes < l.total)
       return host_fail(MP_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", op, workspace ? workspace_bytes : (size_t)0, l.total);
@@ -293,9 +322,10 @@ int mp_w4_pack(int N, int K, const uint8_t* q, long long ldq, uint32_t* packed, 
   return MP_OK;
 }
 
-int mp_linear_w4_workspace(int M, int N, int K, const void* X, long long ldx, int grad_input, size_t* bytes) {
-  if (bytes == nullptr || M < 0 || N <= 0 || K <= 0) return host_fail(MP_ERR_INVALID_ARG, "mp_linear_w4_workspace: needs M >= 0, N > 0, K > 0 and a result pointer");
-  *bytes = M == 0 ? 0 : w4_plan(M, N, K, grad_input != 0, !tokens_aligned(X, ldx)).total;
+int mp_linear_w4_workspace(int M, int N, int K, int group_size, const void* X, long long ldx, int grad_input, size_t* bytes) {
+  if (bytes == nullptr || M < 0 || N <= 0 || K <= 0 || group_size <= 0)
+    return host_fail(MP_ERR_INVALID_ARG, "mp_linear_w4_workspace: needs M >= 0, N > 0, K > 0, group_size > 0 and a result pointer");
+  *bytes = M == 0 ? 0 : w4_plan(M, N, K, group_size, grad_input != 0, !tokens_aligned(X, ldx)).total;
   return MP_OK;
 }
 

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -86,7 +87,7 @@ def lib() -> ctypes.CDLL:
         L.mp_linear_xent.argtypes = xent + [vp, ci, ll, vp, vp, vp, sz, vp]
         L.mp_linear_xent_grad.argtypes = xent + [vp, ci, ll, vp, vp, vp, vp, vp, sz, vp]
         L.mp_w4_pack.argtypes = [ci, ci, vp, ll, vp, vp]
-        L.mp_linear_w4_workspace.argtypes = [ci, ci, ci, vp, ll, ci, ctypes.POINTER(sz)]
+        L.mp_linear_w4_workspace.argtypes = [ci, ci, ci, ci, vp, ll, ci, ctypes.POINTER(sz)]
         L.mp_linear_w4.argtypes = [ci, ci, ci, ci, vp, ll, vp, vp, vp, ci, vp, vp, vp, sz, vp]
         L.mp_linear_w4_grad_input.argtypes = [ci, ci, ci, ci, vp, ll, vp, vp, vp, ci, vp, vp, sz, vp]
         _lib = L
@@ -471,14 +472,21 @@ def _w4_checks(op: str, x: torch.Tensor, qweight: torch.Tensor, scales: torch.Te
     return code, N, group_size, qweight, scales.contiguous(), zeros
 
 
-def _w4_workspace(M, N, K, x, ldx, grad):
-    """(tensor or None, address, bytes).  A fresh tensor per call: calls on other streams and captured graphs never share it."""
+@functools.lru_cache(maxsize=4096)
+def _w4_workspace_bytes(M: int, N: int, K: int, group_size: int, aligned: bool, grad: int) -> int:
+    # an address and a row stride that are 16-byte aligned or not: the library looks at nothing else
     need = ctypes.c_size_t()
-    _check(lib().mp_linear_w4_workspace(M, N, K, x.data_ptr(), ldx, grad, ctypes.byref(need)))
-    if need.value == 0:
+    _check(lib().mp_linear_w4_workspace(M, N, K, group_size, 0 if aligned else 1, 8, grad, ctypes.byref(need)))
+    return need.value
+
+
+def _w4_workspace(M, N, K, group_size, x, ldx, grad):
+    """(tensor or None, address, bytes).  A fresh tensor per call: calls on other streams and captured graphs never share it."""
+    need = _w4_workspace_bytes(M, N, K, group_size, x.data_ptr() & 15 == 0 and ldx & 7 == 0, grad)
+    if need == 0:
         return None, 0, 0
-    ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device)
-    return ws, ws.data_ptr(), need.value
+    ws = torch.empty((need,), dtype=torch.uint8, device=x.device)
+    return ws, ws.data_ptr(), need
 
 
 def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
@@ -497,7 +505,7 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zero
     with _device_of(x):
         y = torch.empty((M, N), dtype=x.dtype, device=x.device)
         x, ldx = _rows(x)
-        ws, at, size = _w4_workspace(M, N, K, x, ldx, 0)
+        ws, at, size = _w4_workspace(M, N, K, group_size, x, ldx, 0)
         rc = lib().mp_linear_w4(code, M, N, K, x.data_ptr(), ldx, qweight.data_ptr(), scales.data_ptr(), _addr(zeros), group_size,
                                 _addr(bias), y.data_ptr(), at, size, _raw_stream(x))
     if rc:
@@ -515,7 +523,7 @@ def linear_w4_grad_input(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.
     with _device_of(dy):
         dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
         dy, ld = _rows(dy)
-        ws, at, size = _w4_workspace(M, N, K, dy, ld, 1)
+        ws, at, size = _w4_workspace(M, N, K, group_size, dy, ld, 1)
         rc = lib().mp_linear_w4_grad_input(code, M, N, K, dy.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(), _addr(zeros),
                                            group_size, dx.data_ptr(), at, size, _raw_stream(dy))
     if rc:

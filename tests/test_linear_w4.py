@@ -58,11 +58,11 @@ def test_refusals_need_no_gpu(api):
     assert fwd(K=48) == 3                                                 # not a multiple of 32
     assert fwd(M=0) == 0
     assert fwd(M=40, K=4096, ldx=4096, ws=z, size=0) == 5                 # split sums need room
-    assert L.mp_linear_w4_workspace(40, 64, 4096, p, 4096, 0, ctypes.byref(n)) == 0 and n.value > 0
+    assert L.mp_linear_w4_workspace(40, 64, 4096, 32, p, 4096, 0, ctypes.byref(n)) == 0 and n.value > 0
     assert fwd(M=40, K=4096, ldx=4096, size=n.value - 1) == 5 and fwd(M=40, K=4096, ldx=4096, ws=ctypes.c_void_p(4096 + 64)) == 5
-    assert L.mp_linear_w4_workspace(1, 64, 4096, p, 4096, 0, ctypes.byref(n)) == 0 and n.value == 0
-    assert L.mp_linear_w4_workspace(1, 64, 4096, p, 4097, 0, ctypes.byref(n)) == 0 and n.value > 0      # an aligned copy
-    assert L.mp_linear_w4_workspace(1, 64, 4096, p, 4096, 0, None) == 1
+    assert L.mp_linear_w4_workspace(1, 64, 4096, 32, p, 4096, 0, ctypes.byref(n)) == 0 and n.value == 0
+    assert L.mp_linear_w4_workspace(1, 64, 4096, 32, p, 4097, 0, ctypes.byref(n)) == 0 and n.value > 0      # an aligned copy
+    assert L.mp_linear_w4_workspace(1, 64, 4096, 32, p, 4096, 0, None) == 1
     assert L.mp_w4_pack(4, 64, z, 64, p, z) == 1 and L.mp_w4_pack(4, 64, p, 63, p, z) == 1 and L.mp_w4_pack(0, 64, z, 64, z, z) == 0
 
 
@@ -187,7 +187,7 @@ def test_padding_bits_and_rows_behind_the_end(api, m):
     assert torch.equal(api.linear_w4(big[:m, :160], pw, s, z, group_size=32), want)
     out = torch.full((m + 2, 33), 7.0, device="cuda", dtype=torch.float16)
     L, n = api.lib(), ctypes.c_size_t()
-    assert L.mp_linear_w4_workspace(m, 33, 160, ctypes.c_void_p(x.data_ptr()), 160, 0, ctypes.byref(n)) == 0
+    assert L.mp_linear_w4_workspace(m, 33, 160, 32, ctypes.c_void_p(x.data_ptr()), 160, 0, ctypes.byref(n)) == 0
     ws = torch.empty(n.value + 256, dtype=torch.uint8, device="cuda")
     api._check(L.mp_linear_w4(api.MP_FP16, m, 33, 160, x.data_ptr(), 160, pw.data_ptr(), s.data_ptr(), z.data_ptr(), 32, None, out.data_ptr(),
                               ws.data_ptr(), n.value, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))

@@ -19,6 +19,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "mp_host.h"
 #include "mp_ptx.cuh"
 
 namespace mp {
@@ -38,7 +39,7 @@ struct PairProblem {
   int rows, cols, kblocks;       // extents of D, 64-element blocks of the contraction
   int tiles_m, tiles_n, bn;
   int a_mn, b_mn;                // 1: MN-major operand
-  int a_wide, b_wide;            // 1: the operand's tensor map is 3-D and one box brings 256 contiguous bytes per line
+  int a_wide, b_wide;            // whole blocks of 64 along the operand's lines (see OperandMaps)
   int group_m;                   // raster: tiles are walked in groups of `group_m` row tiles
   int tile0;                     // index of the problem's first unit in the launch
   int split, kb_per_split;       // PAIR_STORE: the contraction in `split` slices of kb_per_split blocks, a unit each
@@ -178,23 +179,42 @@ __device__ __forceinline__ void store_row32(uint16_t* o, const float (&v)[32], i
   }
 }
 
+// The tensor maps of an operand.  `wide` is 3-D and one box brings 256 contiguous bytes per line, two blocks of 64 (1.07 times
+// as fast a main loop as 128-byte boxes); it covers whole blocks only.  `narrow` covers the lines to their last element and is
+// there for the boxes that would reach past the last whole block.
+struct alignas(64) OperandMaps { CUtensorMap wide, narrow; };
+struct PairMaps { OperandMaps a[2], b[2]; };          // of the launch's problems
+
+// Maps of a row-major 16-bit matrix of `rows` lines of `inner` elements, `ld` apart, for boxes of `box_lines` lines and
+// `box_blocks` blocks of 64 elements.
+inline int operand_maps(OperandMaps* m, const void* ptr, long long inner, long long rows, long long ld, int box_lines, int box_blocks, int* whole) {
+  *whole = inner % 64 == 0 ? 1 << 24 : (int)(inner / 64);      // a line of whole blocks: the fill beyond it does the rest
+  if (inner >= 64) {
+    if (int rc = host_tmap_blocks(&m->wide, ptr, inner / 64 * 64, rows, ld * 2, box_lines, box_blocks)) return rc;
+  }
+  if (inner % 64 != 0) {
+    if (int rc = host_tmap(&m->narrow, kTmap16, ptr, inner, rows, ld * 2, 64, box_lines, 128)) return rc;
+  }
+  return 0;
+}
+
 // One stage of one operand: `rows` row indices from r0, contraction blocks kb ... kb + kc - 1.  K-major: [block][row][128 B];
-// MN-major: [64 row indices][kc * 64 contraction indices][128 B].  Blocks past the end of the contraction are filled with
-// zeros and count their bytes like the others.
+// MN-major: [64 row indices][kc * 64 contraction indices][128 B].  `blocks` whole blocks of 64 along the lines may be read
+// through the wide map.  Blocks past the end of the contraction are filled with zeros and count their bytes like the others.
 template <bool PAIR = true>
-__device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int mn, int wide, int rows, int r0, int kb, int kc) {
+__device__ __forceinline__ void pair_load(uint32_t dst, const OperandMaps& maps, uint32_t bar, int mn, int blocks, int rows, int r0, int kb, int kc) {
   const auto load2 = [&](uint32_t d, int x, int y) {
-    if constexpr (PAIR) tma_load_2d_pair(d, tm, bar, x, y);
-    else tma_load_2d(d, tm, bar, x, y);
+    if constexpr (PAIR) tma_load_2d_pair(d, &maps.narrow, bar, x, y);
+    else tma_load_2d(d, &maps.narrow, bar, x, y);
   };
   const auto load3 = [&](uint32_t d, int x, int y, int z) {
-    if constexpr (PAIR) tma_load_3d_pair(d, tm, bar, x, y, z);
-    else tma_load_3d(d, tm, bar, x, y, z);
+    if constexpr (PAIR) tma_load_3d_pair(d, &maps.wide, bar, x, y, z);
+    else tma_load_3d(d, &maps.wide, bar, x, y, z);
   };
   if (mn) {
-    if (wide) load3(dst, 0, kb * 64, r0 >> 6);
+    if (r0 + rows <= blocks * 64) load3(dst, 0, kb * 64, r0 >> 6);
     else for (int j = 0; j < rows; j += 64) load2(dst + (uint32_t)(j * kc * 128), r0 + j, kb * 64);
-  } else if (wide) {
+  } else if (kb + kc <= blocks) {
     load3(dst, 0, r0, kb);
   } else {
     for (int c = 0; c < kc; ++c) load2(dst + (uint32_t)(c * rows * 128), (kb + c) * 64, r0);
@@ -381,8 +401,7 @@ __device__ __forceinline__ void pair_epilogue_store(const PairParams& p, const P
 // ---------------------------------------------------------------------------------------------------------- the kernel
 template <int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0,
-                 const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB1, const PairParams p) {
+pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
   extern __shared__ uint8_t smem_raw[];
   // both CTAs of the pair see the same dynamic shared-memory offset, so the rounding agrees
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -411,9 +430,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
       mbar_init(unit_bars + 16u + 8u * b, 19);          // two producers, the MMA issuer, sixteen epilogue warps
     }
     mbar_fence_init();
-    tma_prefetch_desc(&tmA0);
-    tma_prefetch_desc(&tmB0);
-    if (p.num_problems == 2) { tma_prefetch_desc(&tmA1); tma_prefetch_desc(&tmB1); }
+    for (int i = 0; i < p.num_problems; ++i) { tma_prefetch_desc(&maps.a[i].wide); tma_prefetch_desc(&maps.b[i].wide); }
   }
   if (warp == 1) tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
   tc_fence_before();
@@ -432,8 +449,6 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
       for (int unit; ok && (unit = units.next()) >= 0;) {
         const PairUnit u = pair_unit(p, unit);
         const PairProblem& q = p.prob[u.prob];
-        const CUtensorMap* tmA = u.prob ? &tmA1 : &tmA0;
-        const CUtensorMap* tmB = u.prob ? &tmB1 : &tmB0;
         const int hb = q.bn >> 1;
         const int a0 = u.tm * kPairRows + (int)rank * 128, b0 = u.tn * q.bn + (int)rank * hb;
         const uint32_t a_bytes = (uint32_t)(p.kc * kPairABytes), tx = 2u * (a_bytes + (uint32_t)(p.kc * hb * 128));   // both CTAs
@@ -442,8 +457,8 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
           const uint32_t dst = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), tx);
           const uint32_t bar = mapa_shared(full_bar(s), 0);
-          pair_load(dst, tmA, bar, q.a_mn, q.a_wide, 128, a0, kb, p.kc);
-          pair_load(dst + a_bytes, tmB, bar, q.b_mn, q.b_wide, hb, b0, kb, p.kc);
+          pair_load(dst, maps.a[u.prob], bar, q.a_mn, q.a_wide, 128, a0, kb, p.kc);
+          pair_load(dst + a_bytes, maps.b[u.prob], bar, q.b_mn, q.b_wide, hb, b0, kb, p.kc);
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
       }

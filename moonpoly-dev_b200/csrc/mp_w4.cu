@@ -35,7 +35,7 @@ Plan w4_plan(int T, int N, int K, int group_size, bool grad, bool copy_tokens) {
   const int rows = grad ? K : N, contraction = grad ? N : K;
   p.stream = !grad && T <= kW4StreamMaxTokens;
   if (copy_tokens) {
-    p.ld_copy = (long long)round_up((size_t)contraction, 8);
+    p.ld_copy = (long long)round_up((size_t)contraction, 64);      // whole blocks: every box is a wide one
     p.copy = p.total;
     p.total += round_up((size_t)T * p.ld_copy * 2, 256);
   }
@@ -170,7 +170,7 @@ int run_stream(const HostDevice& d, const W4StreamParams& p, cudaStream_t stream
 }
 
 template <bool BF16>
-int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, int T, const void* x, long long ldx, const void* bias,
+int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, int T, const void* x, long long ldx, int inner, const void* bias,
              void* out, uint8_t* ws, cudaStream_t stream) {
   W4PairParams p{};
   p.w = w;
@@ -192,14 +192,9 @@ int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, in
   p.stages = 3;
   p.raw_slots = std::min(kW4MaxRawSlots, (kPairSmem - 1024 - 256 - p.stages * p.stage_bytes) / kW4RawBytes);
   p.vec = vector_groups(w);
-  const int contraction = grad ? w.N : w.K;
-  CUtensorMap tmB, tmW;
-  p.b_wide = contraction % 64 == 0;
-  if (p.b_wide) {
-    if (int rc = host_tmap_blocks(&tmB, x, contraction, T, ldx * 2, hb, 2)) return rc;
-  } else {
-    if (int rc = host_tmap(&tmB, kTmap16, x, contraction, T, ldx * 2, 64, hb, 128)) return rc;
-  }
+  OperandMaps tokens;
+  CUtensorMap tmW;
+  if (int rc = operand_maps(&tokens, x, inner, T, ldx, hb, 2, &p.b_wide)) return rc;
   if (l.pair) {
     p.table = reinterpret_cast<const uint32_t*>(ws + l.table);
     p.ld_table = w.N;
@@ -247,7 +242,7 @@ int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, in
   }
   run.attrs = early;
   run.numAttrs = num;
-  MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&run, kern, tmB, tmW, p));
+  MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&run, kern, tokens, tmW, p));
   host_count_launches(1);
   if (p.split > 1) {
     const long long threads = (long long)T * (l.ld_partial / 4);
@@ -270,6 +265,7 @@ int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, in
 int run_w4(const char* op, bool grad, int dtype, int M, int N, int K, const void* X, long long ldx, const uint32_t* packed, const void* scales,
            const uint8_t* zeros, int group_size, const void* bias, void* out, void* workspace, size_t workspace_bytes, void* stream_) {
   const int width = grad ? N : K;
+  int inner = width;
   if (int rc = check_args(op, dtype, M, N, K, X, ldx, width, packed, scales, group_size)) return rc;
   if (M == 0) return MP_OK;
   if (out == nullptr) return host_fail(MP_ERR_INVALID_ARG, "%s: null output", op);
@@ -288,6 +284,7 @@ int run_w4(const char* op, bool grad, int dtype, int M, int N, int K, const void
     if (int rc = host_pad_rows16(X, ldx, ws + l.copy, M, width, (int)l.ld_copy, stream)) return rc;
     X = ws + l.copy;
     ldx = l.ld_copy;
+    inner = (int)l.ld_copy;                              // its lines end in zeros
   }
   const W4Weight w = weight_of(N, K, packed, scales, zeros, group_size);
   if (l.stream) {
@@ -299,8 +296,8 @@ int run_w4(const char* op, bool grad, int dtype, int M, int N, int K, const void
     p.T = M;
     return dtype == MP_BF16 ? run_stream<true>(d, p, stream) : run_stream<false>(d, p, stream);
   }
-  return dtype == MP_BF16 ? run_mma<true>(d, l, w, grad, M, X, ldx, bias, out, ws, stream)
-                          : run_mma<false>(d, l, w, grad, M, X, ldx, bias, out, ws, stream);
+  return dtype == MP_BF16 ? run_mma<true>(d, l, w, grad, M, X, ldx, inner, bias, out, ws, stream)
+                          : run_mma<false>(d, l, w, grad, M, X, ldx, inner, bias, out, ws, stream);
 }
 
 }  // namespace

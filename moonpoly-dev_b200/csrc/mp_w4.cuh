@@ -329,7 +329,7 @@ struct W4PairParams {
   int grad;                     // 0: Y = X W^T, 1: dX = dY W
   int rows, T, steps;           // rows of D, tokens, contraction steps of 128
   int tiles_m, tiles_n, bn, split, steps_per_split;
-  int b_wide;
+  int b_wide;                   // whole blocks of 64 along the tokens' lines
   int stages, stage_bytes, raw_slots;
   const uint32_t* table; int ld_table;   // PAIR: group words [groups][rows of W] (w4_table_kernel)
   int vec;                      // the scales (and zeros) of a block's runs are read in one load each
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(256) w4_table_kernel(const uint16_t* scale, co
 // FINE: groups of 32 or 64, so the runs of a block have scales of their own.
 template <bool BF16, bool FINE, bool PAIR>
 __global__ void __launch_bounds__(kW4Threads, 1)
-w4_mma_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmW, const W4PairParams p) {
+w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant__ CUtensorMap tmW, const W4PairParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t smem_base = smem_u32(smem);
@@ -421,7 +421,7 @@ w4_mma_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ C
     for (int b = 0; b < 2; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), 4 * kCtas); }
     for (int b = 0; b < raw_slots; ++b) { mbar_init(rfull_bar(b), 1); mbar_init(rempty_bar(b), 8); }
     mbar_fence_init();
-    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tokens.wide);
     tma_prefetch_desc(&tmW);
   }
   if (warp == 1) {
@@ -450,7 +450,7 @@ w4_mma_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ C
         for (int st = u.s0; st < u.s1; ++st) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), (uint32_t)(kCtas * hb * 256));
-          pair_load<PAIR>(smem_base + (uint32_t)s * (uint32_t)p.stage_bytes + kW4ABytes, &tmB, at_leader(full_bar(s)), 0, p.b_wide, hb, b0, st * 2, 2);
+          pair_load<PAIR>(smem_base + (uint32_t)s * (uint32_t)p.stage_bytes + kW4ABytes, tokens, at_leader(full_bar(s)), 0, p.b_wide, hb, b0, st * 2, 2);
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
       }

@@ -149,6 +149,9 @@ int xent_piece(int M, int V) {
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
+// 64-element contraction blocks per pipeline stage.
+constexpr int kStageBlocks = 2;
+
 constexpr int kPairsModel = 74;          // workspace sizes must not depend on the device that is asked
 
 // Slices of the vocabulary in the product dX = d W of one piece.  It has few, long tiles (M / 256 x H / 256, cols / 64 blocks
@@ -173,7 +176,7 @@ Layout xent_layout(int M, int V, int H, bool copies, bool backward) {
   Layout l{};
   size_t at = 0;
   const auto take = [&](size_t bytes) { const size_t p = at; at += round_up(bytes, 256); return p; };
-  l.hp = (int)round_up((size_t)H, 8);
+  l.hp = (int)round_up((size_t)H, 64);     // whole blocks: every box is a wide one
   if (copies) {
     l.x_copy = take((size_t)M * l.hp * 2);
     l.w_copy = take((size_t)V * l.hp * 2);
@@ -221,17 +224,6 @@ int check_workspace(const char* op, void* ws, size_t have, size_t need) {
   return MP_OK;
 }
 
-// 64-element contraction blocks per pipeline stage.
-constexpr int kStageBlocks = 2;
-
-// TMA view of a row-major 16-bit matrix as a K-major operand of which a CTA takes `rows_cta` rows, or as an MN-major one of
-// which it takes `rows_cta` columns.
-int operand_map(CUtensorMap* tm, const void* ptr, long long inner, long long rows, long long ld, bool mn, int rows_cta, int* wide) {
-  const int kc = kStageBlocks;
-  *wide = inner % 64 == 0 && kc > 1;
-  if (*wide) return host_tmap_blocks(tm, ptr, inner, rows, ld * 2, mn ? kc * 64 : rows_cta, mn ? rows_cta / 64 : kc);
-  return host_tmap(tm, kTmap16, ptr, inner, rows, ld * 2, 64, mn ? kc * 64 : rows_cta, 128);
-}
 
 void shape_problem(PairProblem* q, int rows, int cols, int contraction, int bn, int a_mn, int b_mn, int group_m, int tile0) {
   q->rows = rows; q->cols = cols;
@@ -247,7 +239,7 @@ void shape_problem(PairProblem* q, int rows, int cols, int contraction, int bn, 
 }
 
 template <int EPI>
-int launch_pair(const HostDevice& d, PairParams& p, const CUtensorMap (&tm)[4], cudaStream_t stream) {
+int launch_pair(const HostDevice& d, PairParams& p, const PairMaps& maps, cudaStream_t stream) {
   auto kern = pair_gemm_kernel<EPI>;
   static bool ready[64] = {};
   if (!ready[d.index & 63]) {
@@ -260,7 +252,7 @@ int launch_pair(const HostDevice& d, PairParams& p, const CUtensorMap (&tm)[4], 
   p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - 256) / p.stage_bytes);
   p.status = d.status;
   const int pairs = std::max(1, std::min(p.total_tiles, d.sms / 2));
-  kern<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(tm[0], tm[1], tm[2], tm[3], p);
+  kern<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(maps, p);
   MP_HOST_CUDA_TRY(cudaGetLastError());
   host_count_launches(1);
   return MP_OK;
@@ -303,6 +295,7 @@ int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx,
     if (int rc = host_pad_rows16(W, ldw, ws + l.w_copy, V, H, l.hp, stream)) return rc;
     X = ws + l.x_copy; W = ws + l.w_copy; ldx = ldw = l.hp;
   }
+  const int inner = copies ? l.hp : H;               // a copy's lines end in zeros
   PairParams p{};
   p.num_problems = 1;
   shape_problem(&p.prob[0], M, V, H, kPairMaxBN, 0, 0, group_rows((long long)H * 2), 0);
@@ -311,11 +304,10 @@ int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx,
   p.target = target; p.target64 = target_bytes == 8; p.ignore_index = ignore_index;
   p.partial = reinterpret_cast<float2*>(ws + l.partial);
   p.target_logit = reinterpret_cast<float*>(ws + l.target_logit);
-  CUtensorMap tm[4];
-  if (int rc = operand_map(&tm[0], X, H, M, ldx, false, 128, &p.prob[0].a_wide)) return rc;
-  if (int rc = operand_map(&tm[1], W, H, V, ldw, false, p.prob[0].bn / 2, &p.prob[0].b_wide)) return rc;
-  tm[2] = tm[0]; tm[3] = tm[1];
-  if (int rc = launch_pair<PAIR_LSE>(d, p, tm, stream)) return rc;
+  PairMaps maps{};
+  if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, 128, kStageBlocks, &p.prob[0].a_wide)) return rc;
+  if (int rc = operand_maps(&maps.b[0], W, inner, V, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
+  if (int rc = launch_pair<PAIR_LSE>(d, p, maps, stream)) return rc;
   xent_join_kernel<<<ceil_div(M, 32), 1024, 0, stream>>>(p.partial, 2 * p.prob[0].tiles_n, M, p.target_logit, target, p.target64,
                                                          ignore_index, V, loss, lse);
   MP_HOST_CUDA_TRY(cudaGetLastError());
@@ -348,6 +340,7 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
     if (int rc = host_pad_rows16(W, ldw, ws + l.w_copy, V, H, l.hp, stream)) return rc;
     X = ws + l.x_copy; W = ws + l.w_copy; ldx = ldw = l.hp;
   }
+  const int inner = copies ? l.hp : H;               // a copy's lines end in zeros
   float* coef = reinterpret_cast<float*>(ws + l.coef);
   float* scale = coef + M;
   unsigned* counters = reinterpret_cast<unsigned*>(ws + l.counters);
@@ -364,7 +357,7 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
   for (int i = 0; i < l.pieces; ++i) {
     const int col0 = i * l.piece, cols = std::min(l.piece, V - col0);
     const uint16_t* Wp = reinterpret_cast<const uint16_t*>(W) + (long long)col0 * ldw;
-    CUtensorMap tm[4];
+    PairMaps maps{};
     {
       PairParams p{};
       p.num_problems = 1;
@@ -373,10 +366,9 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       p.bf16 = bf16;
       p.target = target; p.target64 = target64; p.ignore_index = ignore_index;
       p.col0 = col0; p.lse = lse; p.coef = coef; p.dlogits = dl; p.ld_dl = l.ld_dl;
-      if (int rc = operand_map(&tm[0], X, H, M, ldx, false, 128, &p.prob[0].a_wide)) return rc;
-      if (int rc = operand_map(&tm[1], Wp, H, cols, ldw, false, p.prob[0].bn / 2, &p.prob[0].b_wide)) return rc;
-      tm[2] = tm[0]; tm[3] = tm[1];
-      if (int rc = launch_pair<PAIR_DLOGITS>(d, p, tm, stream)) return rc;
+      if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, 128, kStageBlocks, &p.prob[0].a_wide)) return rc;
+      if (int rc = operand_maps(&maps.b[0], Wp, inner, cols, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
+          if (int rc = launch_pair<PAIR_DLOGITS>(d, p, maps, stream)) return rc;
     }
     PairParams p{};
     p.bf16 = bf16;
@@ -396,8 +388,8 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       } else if (i == l.pieces - 1) {
         q.out16 = dX; q.ld_out = H; q.scale = scale;
       }
-      if (int rc = operand_map(&tm[2 * n], dl, cols, M, l.ld_dl, false, 128, &q.a_wide)) return rc;
-      if (int rc = operand_map(&tm[2 * n + 1], Wp, H, cols, ldw, true, q.bn / 2, &q.b_wide)) return rc;
+      if (int rc = operand_maps(&maps.a[n], dl, cols, M, l.ld_dl, 128, kStageBlocks, &q.a_wide)) return rc;
+      if (int rc = operand_maps(&maps.b[n], Wp, inner, cols, ldw, kStageBlocks * 64, q.bn / 2 / 64, &q.b_wide)) return rc;
       p.total_tiles += q.tiles_m * q.tiles_n * q.split;
       ++n;
     }
@@ -407,14 +399,13 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       q.out16 = reinterpret_cast<uint16_t*>(dW) + (long long)col0 * H;
       q.ld_out = H;
       q.scale = scale;
-      if (int rc = operand_map(&tm[2 * n], dl, cols, M, l.ld_dl, true, 128, &q.a_wide)) return rc;
-      if (int rc = operand_map(&tm[2 * n + 1], X, H, M, ldx, true, q.bn / 2, &q.b_wide)) return rc;
+      if (int rc = operand_maps(&maps.a[n], dl, cols, M, l.ld_dl, kStageBlocks * 64, 128 / 64, &q.a_wide)) return rc;
+      if (int rc = operand_maps(&maps.b[n], X, inner, M, ldx, kStageBlocks * 64, q.bn / 2 / 64, &q.b_wide)) return rc;
       p.total_tiles += q.tiles_m * q.tiles_n;
       ++n;
     }
     p.num_problems = n;
-    if (n == 1) { tm[2] = tm[0]; tm[3] = tm[1]; }
-    if (int rc = launch_pair<PAIR_STORE>(d, p, tm, stream)) return rc;
+    if (int rc = launch_pair<PAIR_STORE>(d, p, maps, stream)) return rc;
   }
   if (slices > 0) {
     const long long threads = (long long)M * (l.ld_acc / 4);

@@ -27,7 +27,6 @@ namespace mp {
 constexpr int kPairRows = 256;               // rows of D per tile
 constexpr int kPairMaxBN = 256;
 constexpr int kPairThreads = 384;             // warps 2 and 3 only fill the first warpgroup up
-constexpr int kPairABytes = 128 * 128;       // one CTA's share of A per 64 contraction elements
 constexpr int kPairMaxStages = 8;
 constexpr int kPairSmem = 232448;            // 227 KB opt-in limit per CTA
 
@@ -39,6 +38,8 @@ struct PairProblem {
   int rows, cols, kblocks;       // extents of D, 64-element blocks of the contraction
   int tiles_m, tiles_n, bn;
   int a_mn, b_mn;                // 1: MN-major operand
+  int a_rows;                    // rows of A that a CTA loads: 128, or fewer (a multiple of 8) where D has fewer altogether; the
+                                 // rest of the tile is whatever lies behind them, and so are its sums, which nobody stores
   int a_wide, b_wide;            // whole blocks of 64 along the operand's lines (see OperandMaps)
   int group_m;                   // raster: tiles are walked in groups of `group_m` row tiles
   int tile0;                     // index of the problem's first unit in the launch
@@ -56,7 +57,7 @@ struct PairParams {
   int num_problems;
   PairProblem prob[2];
   int total_tiles;               // units of the launch
-  unsigned* next_unit;           // PAIR_STORE: counter that hands out units, zero before the launch
+  unsigned* next_unit;           // counter that hands out the units of PAIR_STORE; PAIR_DLOGITS, which goes before, clears it
   int stages, stage_bytes;
   int kc;                        // 64-element blocks of the contraction per stage (1 or 2)
   int bf16;                      // operand and output type: 1 = bf16, 0 = fp16
@@ -68,7 +69,9 @@ struct PairParams {
   float2* partial;               // PAIR_LSE: [2 * tiles_n][rows] (max, sum of exp(z - max))
   float* target_logit;           // PAIR_LSE: [rows]
   const float* lse;              // PAIR_DLOGITS
-  const float* coef;             // PAIR_DLOGITS: row factor
+  const float* grad_loss;        // PAIR_DLOGITS: [rows], the gradient with respect to the rows' losses
+  int vocab;                     // PAIR_DLOGITS: targets are below it
+  float* scale_out;              // PAIR_DLOGITS: what the products of d are to be multiplied by
   uint16_t* dlogits; long long ld_dl;
 };
 
@@ -332,9 +335,31 @@ __device__ __forceinline__ void pair_epilogue_lse(const PairParams& p, const Pai
   if (live) p.partial[(size_t)(2 * tn + half) * q.rows + row] = make_float2(mm, s0 + s1);
 }
 
-// d = coef[row] * (softmax - onehot), rounded once to the operand type and parked for the two gradient products.
+// The largest finite |grad_loss| of the rows that have a loss (1 if there is none), by the eight epilogue warps while the
+// first tile is being multiplied; `slots` are 8 floats of shared memory.
+__device__ __forceinline__ float pair_grad_max(const PairParams& p, int rows, float* slots) {
+  const int e = (int)threadIdx.x - 128;
+  float g = 0.0f;
+  for (int i = e; i < rows; i += 256) {
+    const long long t = p.target64 ? reinterpret_cast<const long long*>(p.target)[i] : reinterpret_cast<const int*>(p.target)[i];
+    const float a = fabsf(p.grad_loss[i]);
+    if (t != p.ignore_index && a < INFINITY) g = fmaxf(g, a);          // infinities and NaN go through as they are
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if ((e & 31) == 0) slots[e >> 5] = g;
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  g = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) g = fmaxf(g, slots[i]);
+  return g == 0.0f ? 1.0f : g;
+}
+
+// d = grad_loss[row] * (softmax - onehot), rounded once to the operand type and parked for the two gradient products.  The
+// largest |grad_loss| is divided out (a mean over the tokens then rounds exactly: the factors are 1) and, for fp16, replaced
+// by 2^15: a probability of 2e-9 is still a normal fp16 number beside a one.  The products are multiplied by *scale_out.
 __device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
-                                                      int ncols, int half_cols) {
+                                                      int ncols, int half_cols, float grad_max) {
   const bool live = row < q.rows;
   long long target = -1;
   float lse = 0.0f, coef = 0.0f;
@@ -344,7 +369,7 @@ __device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const
     kept = t != p.ignore_index;
     target = t - p.col0 - c_begin;
     lse = p.lse[row];
-    coef = p.coef[row];
+    coef = t < 0 || t >= p.vocab ? NAN : p.grad_loss[row] / grad_max * (p.bf16 ? 1.0f : 32768.0f);
   }
   uint16_t* o = p.dlogits + (long long)row * p.ld_dl + c_begin;
   for (int c0 = 0; c0 < half_cols; c0 += 32) {
@@ -438,6 +463,9 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   cluster_sync_all();                       // the peer's barriers are initialised, its TMEM is allocated
+  // Everything above may overlap the previous kernel of the stream; nothing of it is read or overwritten before it is done.
+  griddep_launch_dependents();
+  griddep_wait();
 
   if (warp < 4) {
     if constexpr (EPI == PAIR_LSE) regs_fewer_88();      // its epilogue holds 128 sums per thread
@@ -451,14 +479,18 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         const PairProblem& q = p.prob[u.prob];
         const int hb = q.bn >> 1;
         const int a0 = u.tm * kPairRows + (int)rank * 128, b0 = u.tn * q.bn + (int)rank * hb;
-        const uint32_t a_bytes = (uint32_t)(p.kc * kPairABytes), tx = 2u * (a_bytes + (uint32_t)(p.kc * hb * 128));   // both CTAs
+        // A CTA whose share of an operand lies wholly behind its end loads nothing: boxes of zeros take the TMA unit longer
+        // than data (a single row of 4096 against 50021: 116 us with them).
+        const uint32_t a_bytes = (uint32_t)(p.kc * q.a_rows * 128), b_bytes = (uint32_t)(p.kc * hb * 128);
+        const bool has_a = a0 < q.rows, has_b = b0 < q.cols;
+        const uint32_t tx = a_bytes * (u.tm * kPairRows + 128 < q.rows ? 2u : 1u) + b_bytes * (u.tn * q.bn + hb < q.cols ? 2u : 1u);   // both CTAs
         for (int kb = u.kb0; kb < u.kb1; kb += p.kc) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
           const uint32_t dst = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), tx);
           const uint32_t bar = mapa_shared(full_bar(s), 0);
-          pair_load(dst, maps.a[u.prob], bar, q.a_mn, q.a_wide, 128, a0, kb, p.kc);
-          pair_load(dst + a_bytes, maps.b[u.prob], bar, q.b_mn, q.b_wide, hb, b0, kb, p.kc);
+          if (has_a) pair_load(dst, maps.a[u.prob], bar, q.a_mn, q.a_wide, q.a_rows, a0, kb, p.kc);
+          if (has_b) pair_load(dst + a_bytes, maps.b[u.prob], bar, q.b_mn, q.b_wide, hb, b0, kb, p.kc);
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
       }
@@ -492,11 +524,11 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         const uint32_t mn_block = (uint32_t)p.kc * 8192u;
         const uint64_t a_base = q.a_mn ? umma_smem_desc_mn(smem_base, mn_block) : umma_smem_desc_sw128(smem_base);
         const uint64_t b_base = (q.b_mn ? umma_smem_desc_mn(smem_base, mn_block) : umma_smem_desc_sw128(smem_base)) +
-                                (uint64_t)((uint32_t)(p.kc * kPairABytes) >> 4);
+                                (uint64_t)((uint32_t)(p.kc * q.a_rows * 128) >> 4);
         // 16 contraction elements further: 32 bytes along a K-major line, or 16 lines of an MN-major tile; 64 further: the
         // next K-major block, or 64 lines
         const uint32_t a_step = q.a_mn ? 2048u >> 4 : 2u, b_step = q.b_mn ? 2048u >> 4 : 2u;
-        const uint32_t a_blk = q.a_mn ? 8192u >> 4 : kPairABytes >> 4, b_blk = q.b_mn ? 8192u >> 4 : (uint32_t)(q.bn >> 1) * 128u >> 4;
+        const uint32_t a_blk = q.a_mn ? 8192u >> 4 : (uint32_t)q.a_rows * 128u >> 4, b_blk = q.b_mn ? 8192u >> 4 : (uint32_t)(q.bn >> 1) * 128u >> 4;
         const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4;
         // an accumulator takes the whole contraction, or a chunk of it (PAIR_LSE)
         const int chunk = EPI == PAIR_LSE ? kLseChunk : q.kblocks;
@@ -538,6 +570,14 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
     const int quad = warp & 3, half = (warp - 4) >> 2;
     uint32_t ui = 0;
     bool ok = true;
+    float grad_max = 1.0f;
+    if constexpr (EPI == PAIR_DLOGITS) {
+      grad_max = pair_grad_max(p, p.prob[0].rows, reinterpret_cast<float*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 48));
+      if (blockIdx.x == 0 && threadIdx.x == 128) {
+        *p.scale_out = grad_max / (p.bf16 ? 1.0f : 32768.0f);
+        *p.next_unit = 0u;                               // of the products' launch
+      }
+    }
     while (ok) {
       int unit = 0;
       if constexpr (DYNAMIC) {
@@ -581,7 +621,7 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
         tc_fence_after();
         const uint32_t t_addr = t_half + buf * (uint32_t)kPairMaxBN;
-        if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols);
+        if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols, grad_max);
         else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols, u.slice);
         tc_fence_before();
         __syncwarp();

@@ -27,6 +27,8 @@ size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 __global__ void __launch_bounds__(1024) xent_join_kernel(const float2* partial, int num, int rows, const float* target_logit,
                                                          const void* target, int target64, long long ignore_index, int vocab,
                                                          float* loss, float* lse) {
+  griddep_launch_dependents();
+  griddep_wait();
   __shared__ float sm[32][33], ss[32][33];
   const int rx = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + rx;
@@ -60,43 +62,11 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const float2* partial, 
   else loss[row] = logsum + (base - target_logit[row]);   // small losses keep their digits: no large lse is formed
 }
 
-// Row factors of d and the scale of the products.  d is parked in 16 bits, so the largest |g| is divided out (a mean over
-// the tokens then rounds exactly: the factors are 1) and, for fp16, replaced by 2^15: a probability of 2e-9 is still a
-// normal fp16 number beside a one.  One block: the rows of a training batch are a few kilobytes.  It also
-// clears the counters that hand out the units of the products' launches.
-__global__ void __launch_bounds__(1024) xent_coef_kernel(const float* grad_loss, const void* target, int target64,
-                                                         long long ignore_index, int vocab, int rows, int bf16, float* coef, float* scale,
-                                                         unsigned* counters, int num_counters) {
-  __shared__ float red[32];
-  for (int i = threadIdx.x; i < num_counters; i += 1024) counters[i] = 0u;
-  float g = 0.0f;
-  for (int i = threadIdx.x; i < rows; i += 1024) {
-    const long long t = target64 ? reinterpret_cast<const long long*>(target)[i] : reinterpret_cast<const int*>(target)[i];
-    if (t != ignore_index) {
-      const float a = fabsf(grad_loss[i]);
-      if (a < INFINITY) g = fmaxf(g, a);           // infinities and NaN go through as they are
-    }
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = g;
-  __syncthreads();
-  g = red[threadIdx.x & 31];
-#pragma unroll
-  for (int o = 16; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-  if (g == 0.0f) g = 1.0f;
-  const float up = bf16 ? 1.0f : 32768.0f;
-  for (int i = threadIdx.x; i < rows; i += 1024) {
-    const long long t = target64 ? reinterpret_cast<const long long*>(target)[i] : reinterpret_cast<const int*>(target)[i];
-    const bool bad = t < 0 || t >= vocab;
-    coef[i] = t == ignore_index ? 0.0f : bad ? NAN : grad_loss[i] / g * up;
-  }
-  if (threadIdx.x == 0) *scale = g / up;
-}
-
 // dX = scale * sum of the slices' 32-bit sums, in their order; four columns per thread.
 __global__ void __launch_bounds__(256) xent_dx_kernel(const float* acc, int slices, long long slice_words, long long ld_acc, int rows, int cols,
                                                       const float* scale, uint16_t* out, int bf16) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int quads = (int)(ld_acc >> 2);
   const long long x = (long long)blockIdx.x * 256 + threadIdx.x;
   if (x >= (long long)rows * quads) return;
@@ -132,7 +102,7 @@ struct Xent {
 struct Layout {
   size_t x_copy, w_copy;                  // aligned copies of operands whose rows miss TMA's 16 bytes
   size_t partial, target_logit;           // forward
-  size_t coef, counters, dl, acc;         // gradients
+  size_t scale, dl, acc;                  // gradients (scale: and the unit counter)
   int hp, piece, pieces;
   int max_split;                          // slices that `acc` has room for
   long long ld_acc, ld_dl, acc_slice;
@@ -190,9 +160,8 @@ Layout xent_layout(int M, int V, int H, bool copies, bool backward) {
     l.pieces = (V + l.piece - 1) / l.piece;
     l.ld_dl = l.piece;
     l.ld_acc = (long long)round_up((size_t)H, 32);
-    l.coef = take(((size_t)M + 64) * sizeof(float));
+    l.scale = take(2 * sizeof(float));
     l.dl = take((size_t)M * l.piece * 2);
-    l.counters = take((size_t)l.pieces * sizeof(unsigned));
     const int first = std::min(V, l.piece);
     l.max_split = std::max(dx_split(M, H, first, false), dx_split(M, H, first, true));
     l.acc_slice = (long long)M * l.ld_acc;
@@ -232,10 +201,29 @@ void shape_problem(PairProblem* q, int rows, int cols, int contraction, int bn, 
   q->tiles_m = ceil_div(rows, kPairRows);
   q->tiles_n = ceil_div(cols, bn);
   q->a_mn = a_mn; q->b_mn = b_mn;
+  q->a_rows = a_mn ? 128 : std::min(128, (int)round_up((size_t)rows, 8));
   q->group_m = std::max(1, std::min(group_m, q->tiles_m));
   q->tile0 = tile0;
   q->split = 1;
   q->kb_per_split = q->kblocks;
+}
+
+// A launch that may begin while the previous kernel of the stream ends; every kernel here waits before it touches memory.
+template <typename... P, typename... A>
+int launch(void (*kern)(P...), int grid, int threads, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = host_use_pdl() ? 1 : 0;
+  MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, P(args)...));
+  host_count_launches(1);
+  return MP_OK;
 }
 
 template <int EPI>
@@ -248,14 +236,12 @@ int launch_pair(const HostDevice& d, PairParams& p, const PairMaps& maps, cudaSt
   }
   const int bn = p.num_problems == 2 ? std::max(p.prob[0].bn, p.prob[1].bn) : p.prob[0].bn;
   p.kc = kStageBlocks;
-  p.stage_bytes = p.kc * (kPairABytes + bn / 2 * 128);
+  const int a_rows = p.num_problems == 2 ? 128 : p.prob[0].a_rows;
+  p.stage_bytes = p.kc * (a_rows * 128 + bn / 2 * 128);
   p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - 256) / p.stage_bytes);
   p.status = d.status;
   const int pairs = std::max(1, std::min(p.total_tiles, d.sms / 2));
-  kern<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(maps, p);
-  MP_HOST_CUDA_TRY(cudaGetLastError());
-  host_count_launches(1);
-  return MP_OK;
+  return launch(kern, 2 * pairs, kPairThreads, kPairSmem, stream, maps, p);
 }
 
 // Row tiles that run side by side against one column tile: their operand rows should stay in L2 while the columns pass.
@@ -305,14 +291,11 @@ int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx,
   p.partial = reinterpret_cast<float2*>(ws + l.partial);
   p.target_logit = reinterpret_cast<float*>(ws + l.target_logit);
   PairMaps maps{};
-  if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, 128, kStageBlocks, &p.prob[0].a_wide)) return rc;
+  if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, p.prob[0].a_rows, kStageBlocks, &p.prob[0].a_wide)) return rc;
   if (int rc = operand_maps(&maps.b[0], W, inner, V, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
   if (int rc = launch_pair<PAIR_LSE>(d, p, maps, stream)) return rc;
-  xent_join_kernel<<<ceil_div(M, 32), 1024, 0, stream>>>(p.partial, 2 * p.prob[0].tiles_n, M, p.target_logit, target, p.target64,
-                                                         ignore_index, V, loss, lse);
-  MP_HOST_CUDA_TRY(cudaGetLastError());
-  host_count_launches(1);
-  return MP_OK;
+  return launch(xent_join_kernel, ceil_div(M, 32), 1024, 0, stream, p.partial, 2 * p.prob[0].tiles_n, M, p.target_logit, target, p.target64,
+                ignore_index, V, loss, lse);
 }
 
 int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long ldx, const void* W, long long ldw, const void* target,
@@ -341,17 +324,12 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
     X = ws + l.x_copy; W = ws + l.w_copy; ldx = ldw = l.hp;
   }
   const int inner = copies ? l.hp : H;               // a copy's lines end in zeros
-  float* coef = reinterpret_cast<float*>(ws + l.coef);
-  float* scale = coef + M;
-  unsigned* counters = reinterpret_cast<unsigned*>(ws + l.counters);
+  float* scale = reinterpret_cast<float*>(ws + l.scale);
+  unsigned* counter = reinterpret_cast<unsigned*>(ws + l.scale) + 1;
   uint16_t* dl = reinterpret_cast<uint16_t*>(ws + l.dl);
   // the same slices in every piece (a short last piece may leave the last ones without work): sums stay in their order
   const int split = dX == nullptr ? 1 : dx_split(M, H, std::min(V, l.piece), dW != nullptr);
   const int bf16 = dtype == MP_BF16, target64 = target_bytes == 8;
-  xent_coef_kernel<<<1, 1024, 0, stream>>>(grad_loss, target, target64, ignore_index, V, M, bf16, coef, scale,
-                                           counters, l.pieces);
-  MP_HOST_CUDA_TRY(cudaGetLastError());
-  host_count_launches(1);
 
   int slices = 0;                                     // of dX, waiting to be joined
   for (int i = 0; i < l.pieces; ++i) {
@@ -365,14 +343,14 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       p.total_tiles = p.prob[0].tiles_m * p.prob[0].tiles_n;
       p.bf16 = bf16;
       p.target = target; p.target64 = target64; p.ignore_index = ignore_index;
-      p.col0 = col0; p.lse = lse; p.coef = coef; p.dlogits = dl; p.ld_dl = l.ld_dl;
-      if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, 128, kStageBlocks, &p.prob[0].a_wide)) return rc;
+      p.col0 = col0; p.lse = lse; p.grad_loss = grad_loss; p.vocab = V; p.scale_out = scale; p.next_unit = counter; p.dlogits = dl; p.ld_dl = l.ld_dl;
+      if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, p.prob[0].a_rows, kStageBlocks, &p.prob[0].a_wide)) return rc;
       if (int rc = operand_maps(&maps.b[0], Wp, inner, cols, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
           if (int rc = launch_pair<PAIR_DLOGITS>(d, p, maps, stream)) return rc;
     }
     PairParams p{};
     p.bf16 = bf16;
-    p.next_unit = counters + i;
+    p.next_unit = counter;
     int n = 0;
     if (dX != nullptr) {                              // dX[M, H] (+)= d[M, cols] W[cols, H]
       PairProblem& q = p.prob[n];
@@ -388,7 +366,7 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       } else if (i == l.pieces - 1) {
         q.out16 = dX; q.ld_out = H; q.scale = scale;
       }
-      if (int rc = operand_maps(&maps.a[n], dl, cols, M, l.ld_dl, 128, kStageBlocks, &q.a_wide)) return rc;
+      if (int rc = operand_maps(&maps.a[n], dl, cols, M, l.ld_dl, q.a_rows, kStageBlocks, &q.a_wide)) return rc;
       if (int rc = operand_maps(&maps.b[n], Wp, inner, cols, ldw, kStageBlocks * 64, q.bn / 2 / 64, &q.b_wide)) return rc;
       p.total_tiles += q.tiles_m * q.tiles_n * q.split;
       ++n;
@@ -409,10 +387,8 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
   }
   if (slices > 0) {
     const long long threads = (long long)M * (l.ld_acc / 4);
-    xent_dx_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(reinterpret_cast<const float*>(ws + l.acc), slices, l.acc_slice,
-                                                                           l.ld_acc, M, H, scale, reinterpret_cast<uint16_t*>(dX), bf16);
-    MP_HOST_CUDA_TRY(cudaGetLastError());
-    host_count_launches(1);
+    return launch(xent_dx_kernel, (int)((threads + 255) / 256), 256, 0, stream, reinterpret_cast<const float*>(ws + l.acc), slices, l.acc_slice,
+                  l.ld_acc, M, H, scale, reinterpret_cast<uint16_t*>(dX), bf16);
   }
   return MP_OK;
 }

@@ -21,7 +21,7 @@ constexpr int kW4StreamMaxTokens = 16;
 constexpr int kSmsModel = 148;            // workspace sizes must not depend on the device that is asked
 
 struct Plan {
-  bool stream, pair;
+  bool stream, pair, with_table;
   int bn, tiles_m, tiles_n, steps, split, steps_per_split;
   size_t copy, partial, table, total;     // workspace: aligned copy of the tokens, partial sums, group words
   long long ld_copy, ld_partial;
@@ -60,7 +60,9 @@ Plan w4_plan(int T, int N, int K, int group_size, bool grad, bool copy_tokens) {
   p.tiles_n = ceil_div(T, p.bn);
   p.steps_per_split = ceil_div(p.steps, p.split);
   p.split = ceil_div(p.steps, p.steps_per_split);
-  if (p.pair) {
+  // The transposed group words pay for their kernel (3 us) where the weight is unpacked more than once.
+  p.with_table = p.tiles_n > 1;
+  if (p.with_table) {
     p.table = p.total;
     p.total += round_up((size_t)ceil_div(K, group_size) * N * 4, 256);
   }
@@ -195,7 +197,7 @@ int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, in
   OperandMaps tokens;
   CUtensorMap tmW;
   if (int rc = operand_maps(&tokens, x, inner, T, ldx, hb, 2, &p.b_wide)) return rc;
-  if (l.pair) {
+  if (l.with_table) {
     p.table = reinterpret_cast<const uint32_t*>(ws + l.table);
     p.ld_table = w.N;
     cudaLaunchConfig_t cfg = {};

@@ -331,7 +331,7 @@ struct W4PairParams {
   int tiles_m, tiles_n, bn, split, steps_per_split;
   int b_wide;                   // whole blocks of 64 along the tokens' lines
   int stages, stage_bytes, raw_slots;
-  const uint32_t* table; int ld_table;   // PAIR: group words [groups][rows of W] (w4_table_kernel)
+  const uint32_t* table; int ld_table;   // PAIR: group words [groups][rows of W] (w4_table_kernel); may be null
   int vec;                      // the scales (and zeros) of a block's runs are read in one load each
   uint16_t* out; long long ldo; // out[token][row]
   const uint16_t* bias;
@@ -544,7 +544,7 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
     const auto fetch = [&](int tm, int st) {
       const int blk = p.grad ? tm * kCtas + (int)rank : st;
       const int row = (p.grad ? st * 128 : tm * kRows + (int)rank * 128) + r0;
-      if constexpr (PAIR) {
+      if (PAIR && p.table != nullptr) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           const int run = blk * 4 + i;

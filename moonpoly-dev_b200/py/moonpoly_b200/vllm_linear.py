@@ -39,7 +39,7 @@ _WS_POOL: Dict[Tuple[int, int], torch.Tensor] = {}
 DECODE_SELECTOR: Dict[Tuple[int, int, int], Tuple[int, int]] = {}
 STATS = {"cpp_selector": 0, "whitelist_attempt": 0, "whitelist_hit": 0, "whitelist_fallback": 0,
          "whitelist_unmapped": 0, "streamk_attempt": 0, "streamk_success": 0, "streamk_fallback": 0,
-         "streamk_skipped": 0, "linear": 0, "declined": 0}
+         "streamk_skipped": 0, "linear": 0, "linear_w4": 0, "declined": 0}
 
 
 def _flag(name: str, default: str) -> bool:
@@ -182,11 +182,36 @@ def apply_moonpoly_linear(weight: torch.Tensor, x: torch.Tensor, bias: Optional[
     return out.view(*lead, n)
 
 
+def apply_moonpoly_linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+                             group_size: int = 128, bias: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """x[..., K] @ W[N, K]^T (+ bias) for a layer whose weight is held in 4 bits with a scale (and zero point) per group, through
+    `moonpoly_ops.linear_w4` (qweight from `moonpoly_ops.pack_w4`), or None when this path declines: the switch is off, the
+    tensors are not CUDA or not fp16 / bf16, or the operator refuses them.  Not in the reference, which serves unquantized
+    and INT8 layers only."""
+    if not _flag("VLLM_USE_MOONPOLY_LINEAR", "0"):
+        return None
+    ops = _ops()
+    if (ops is None or not hasattr(ops, "linear_w4") or x.device.type != "cuda" or qweight.device.type != "cuda"
+            or x.dtype not in (torch.float16, torch.bfloat16)):
+        STATS["declined"] += 1
+        return None
+    x2 = x.reshape(-1, x.shape[-1])
+    try:
+        out = ops.linear_w4(x2, qweight, scales, zeros, group_size, bias)
+    except Exception:
+        STATS["declined"] += 1
+        return None
+    STATS["linear_w4"] += 1
+    return out.view(*x.shape[:-1], qweight.shape[0])
+
+
 def apply(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor] = None,
           fallback: Optional[Callable] = None) -> torch.Tensor:
     """Drop-in body of UnquantizedLinearMethod.apply(layer, x, bias): the operators first, `fallback(layer, x, bias)`
-    (default torch.nn.functional.linear on the layer's weight) when they decline."""
-    out = apply_moonpoly_linear(layer.weight, x, bias)
+    (default torch.nn.functional.linear on the layer's weight) when they decline.  A layer that carries `moonpoly_w4 =
+    (qweight, scales, zeros or None, group_size)` runs from its 4-bit weight."""
+    w4 = getattr(layer, "moonpoly_w4", None)
+    out = apply_moonpoly_linear_w4(x, *w4, bias=bias) if w4 is not None else apply_moonpoly_linear(layer.weight, x, bias)
     if out is not None:
         return out
     if fallback is not None:

@@ -212,6 +212,162 @@ std::tuple<int, int, int, int> scaled_mm_config(int id) {
   return {v[0], v[1], v[2], v[3]};
 }
 
+// ------------------------------------------------------------------------------------------ 4-bit Linear (not in the reference)
+int code16(const at::Tensor& t, const char* op) {
+  require(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, std::string(op) + ": fp16 or bf16 only");
+  return t.scalar_type() == at::kHalf ? MP_FP16 : MP_BF16;
+}
+
+// Rows that are packed and do not share memory, as they are; anything else copied.
+at::Tensor packed_rows(const at::Tensor& t, long long* ld) {
+  const bool ok = (t.stride(1) == 1 || t.size(1) <= 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+  at::Tensor r = ok ? t : t.contiguous();
+  *ld = r.size(0) > 1 ? r.stride(0) : r.size(1);
+  return r;
+}
+
+at::Tensor workspace_of(size_t bytes, const at::Tensor& like) {
+  // a tensor per call: calls on other streams and captured graphs never share it
+  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
+at::Tensor pack_w4(const at::Tensor& q) {
+  require(q.is_cuda() && q.dim() == 2 && q.scalar_type() == at::kByte, "pack_w4: q must be a 2D CUDA uint8 tensor [N, K]");
+  c10::cuda::CUDAGuard guard(q.device());
+  long long ld = 0;
+  const at::Tensor qc = packed_rows(q, &ld);
+  at::Tensor out = at::empty({q.size(0), (q.size(1) + 127) / 128 * 16}, q.options().dtype(at::kInt));
+  check(mp_w4_pack((int)q.size(0), (int)q.size(1), qc.data_ptr<uint8_t>(), ld, reinterpret_cast<uint32_t*>(out.data_ptr<int>()), stream_of(q)));
+  return out;
+}
+
+struct W4Args {
+  at::Tensor qweight, scales, zeros;
+  int code = 0, N = 0, K = 0, group = 0;
+  const uint32_t* packed() const { return reinterpret_cast<const uint32_t*>(qweight.data_ptr<int>()); }
+  const uint8_t* zero() const { return zeros.defined() ? zeros.data_ptr<uint8_t>() : nullptr; }
+};
+
+W4Args w4_args(const char* name, const at::Tensor& x, const at::Tensor& qweight, const at::Tensor& scales, const std::optional<at::Tensor>& zeros,
+               int64_t group_size, int64_t K, bool grad) {
+  const std::string op(name);
+  require(x.is_cuda() && qweight.is_cuda() && scales.is_cuda(), op + ": tensors must be CUDA");
+  require(x.dim() == 2 && qweight.dim() == 2, op + ": input and packed weight must be 2D");
+  W4Args a;
+  a.code = code16(x, name);
+  const int64_t N = qweight.size(0);
+  require(qweight.scalar_type() == at::kInt && N > 0 && K > 0 && qweight.size(1) == (K + 127) / 128 * 16, op + ": the packed weight must be int32 [N, 16 * ceil(K / 128)]");
+  require(x.size(1) == (grad ? N : K), op + ": input width does not match the weight");
+  require(K % 32 == 0, op + ": K must be a multiple of 32");
+  if (group_size == -1) for (group_size = 32; group_size < K; group_size *= 2) {}
+  require(group_size >= 32 && (group_size & (group_size - 1)) == 0, op + ": group_size must be a power of two of at least 32, or -1");
+  const int64_t groups = (K + group_size - 1) / group_size;
+  require(scales.scalar_type() == x.scalar_type() && scales.dim() == 2 && scales.size(0) == N && scales.size(1) == groups, op + ": scales must be [N, ceil(K / group_size)] in the input dtype");
+  require(qweight.device() == x.device() && scales.device() == x.device(), op + ": tensors must be on one device");
+  if (zeros.has_value() && zeros->defined()) {
+    require(zeros->device() == x.device() && zeros->scalar_type() == at::kByte && zeros->dim() == 2 && zeros->size(0) == N && zeros->size(1) == groups, op + ": zeros must be uint8 in the shape of the scales");
+    a.zeros = zeros->contiguous();
+  }
+  a.qweight = qweight.contiguous();
+  if (reinterpret_cast<uintptr_t>(a.qweight.data_ptr()) & 15) a.qweight = a.qweight.clone();
+  a.scales = scales.contiguous();
+  a.N = (int)N; a.K = (int)K; a.group = (int)group_size;
+  return a;
+}
+
+at::Tensor linear_w4(const at::Tensor& x, const at::Tensor& qweight, const at::Tensor& scales, const std::optional<at::Tensor>& zeros,
+                     int64_t group_size, const std::optional<at::Tensor>& bias) {
+  const W4Args a = w4_args("linear_w4", x, qweight, scales, zeros, group_size, x.dim() == 2 ? x.size(1) : 0, false);
+  c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor bc;
+  if (bias.has_value() && bias->defined()) {
+    require(bias->device() == x.device() && bias->scalar_type() == x.scalar_type() && bias->numel() == a.N, "linear_w4: bias must be a CUDA tensor of N elements in the input dtype");
+    bc = bias->contiguous();
+  }
+  long long ld = 0;
+  const at::Tensor xc = packed_rows(x, &ld);
+  at::Tensor y = at::empty({x.size(0), a.N}, x.options());
+  size_t need = 0;
+  check(mp_linear_w4_workspace((int)x.size(0), a.N, a.K, a.group, xc.data_ptr(), ld, 0, &need));
+  const at::Tensor ws = workspace_of(need, x);
+  check(mp_linear_w4(a.code, (int)x.size(0), a.N, a.K, xc.data_ptr(), ld, a.packed(), a.scales.data_ptr(), a.zero(), a.group,
+                     bc.defined() ? bc.data_ptr() : nullptr, y.data_ptr(), need ? ws.data_ptr() : nullptr, need, stream_of(x)));
+  return y;
+}
+
+at::Tensor linear_w4_grad_input(const at::Tensor& dy, const at::Tensor& qweight, const at::Tensor& scales, const std::optional<at::Tensor>& zeros,
+                                int64_t group_size, std::optional<int64_t> in_features) {
+  const int64_t K = in_features.has_value() ? *in_features : qweight.dim() == 2 ? qweight.size(1) * 8 : 0;
+  const W4Args a = w4_args("linear_w4_grad_input", dy, qweight, scales, zeros, group_size, K, true);
+  c10::cuda::CUDAGuard guard(dy.device());
+  long long ld = 0;
+  const at::Tensor dyc = packed_rows(dy, &ld);
+  at::Tensor dx = at::empty({dy.size(0), K}, dy.options());
+  size_t need = 0;
+  check(mp_linear_w4_workspace((int)dy.size(0), a.N, a.K, a.group, dyc.data_ptr(), ld, 1, &need));
+  const at::Tensor ws = workspace_of(need, dy);
+  check(mp_linear_w4_grad_input(a.code, (int)dy.size(0), a.N, a.K, dyc.data_ptr(), ld, a.packed(), a.scales.data_ptr(), a.zero(), a.group,
+                                dx.data_ptr(), need ? ws.data_ptr() : nullptr, need, stream_of(dy)));
+  return dx;
+}
+
+// ------------------------------------------------------------------------------------------ Linear with softmax cross entropy
+struct XentArgs {
+  at::Tensor x, w, target;
+  long long ldx = 0, ldw = 0;
+  int code = 0, M = 0, V = 0, H = 0;
+  size_t workspace(int backward) const {
+    size_t need = 0;
+    check(mp_linear_xent_workspace(code, M, V, H, x.data_ptr(), ldx, w.data_ptr(), ldw, backward, &need));
+    return need;
+  }
+};
+
+XentArgs xent_args(const char* name, const at::Tensor& x, const at::Tensor& w, const at::Tensor& target) {
+  const std::string op(name);
+  require(x.is_cuda() && w.is_cuda() && target.is_cuda(), op + ": tensors must be CUDA");
+  require(x.dim() == 2 && w.dim() == 2 && w.size(1) == x.size(1), op + ": hidden states [M, H] and weight [V, H]");
+  require(w.size(0) > 0 && w.size(1) > 0, op + ": the weight must not be empty");
+  require(x.scalar_type() == w.scalar_type(), op + ": hidden states and weight dtypes differ");
+  require(target.dim() == 1 && target.size(0) == x.size(0) && (target.scalar_type() == at::kLong || target.scalar_type() == at::kInt), op + ": target must be M integers (int64 or int32)");
+  require(w.device() == x.device() && target.device() == x.device(), op + ": tensors must be on one device");
+  XentArgs a;
+  a.code = code16(x, name);
+  a.x = packed_rows(x, &a.ldx);
+  a.w = packed_rows(w, &a.ldw);
+  a.target = target.contiguous();
+  a.M = (int)x.size(0); a.V = (int)w.size(0); a.H = (int)x.size(1);
+  return a;
+}
+
+std::tuple<at::Tensor, at::Tensor> linear_cross_entropy(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, int64_t ignore_index) {
+  c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? std::optional<at::Device>(x.device()) : std::nullopt);
+  const XentArgs a = xent_args("linear_cross_entropy", x, w, target);
+  at::Tensor loss = at::empty({a.M}, x.options().dtype(at::kFloat)), lse = at::empty_like(loss);
+  const size_t need = a.workspace(0);
+  const at::Tensor ws = workspace_of(need, x);
+  check(mp_linear_xent(a.code, a.M, a.V, a.H, a.x.data_ptr(), a.ldx, a.w.data_ptr(), a.ldw, a.target.data_ptr(), (int)a.target.element_size(),
+                       ignore_index, loss.data_ptr<float>(), lse.data_ptr<float>(), ws.data_ptr(), need, stream_of(x)));
+  return {loss, lse};
+}
+
+// A gradient that is not needed comes back as an empty tensor.
+std::tuple<at::Tensor, at::Tensor> linear_cross_entropy_grad(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, const at::Tensor& lse,
+                                                             const at::Tensor& grad_loss, int64_t ignore_index, bool need_dx, bool need_dw) {
+  c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? std::optional<at::Device>(x.device()) : std::nullopt);
+  const XentArgs a = xent_args("linear_cross_entropy_grad", x, w, target);
+  for (const at::Tensor* t : {&lse, &grad_loss})
+    require(t->device() == x.device() && t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == a.M, "linear_cross_entropy_grad: lse and grad_loss must be M fp32 values");
+  const at::Tensor lc = lse.contiguous(), gc = grad_loss.contiguous();
+  at::Tensor dx = at::empty({need_dx ? a.M : 0, a.H}, x.options()), dw = at::empty({need_dw ? a.V : 0, a.H}, x.options());
+  const size_t need = a.workspace(1);
+  const at::Tensor ws = workspace_of(need, x);
+  check(mp_linear_xent_grad(a.code, a.M, a.V, a.H, a.x.data_ptr(), a.ldx, a.w.data_ptr(), a.ldw, a.target.data_ptr(), (int)a.target.element_size(),
+                            ignore_index, lc.data_ptr<float>(), gc.data_ptr<float>(), need_dx ? dx.data_ptr() : nullptr,
+                            need_dw ? dw.data_ptr() : nullptr, ws.data_ptr(), need, stream_of(x)));
+  return {dx, dw};
+}
+
 // ------------------------------------------------------------------------------------------ Meta kernels
 at::Tensor linear_meta(const at::Tensor& x, const at::Tensor& w) {
   return at::empty_symint({x.sym_size(0), w.sym_size(0)}, x.options());
@@ -223,6 +379,26 @@ int64_t ws_size_meta(const at::Tensor&, const at::Tensor&, int64_t, int64_t) { r
 at::Tensor linear_ws_meta(const at::Tensor& x, const at::Tensor& w, int64_t, const at::Tensor&, int64_t) {
   return at::empty_symint({x.sym_size(0), w.sym_size(0)}, x.options());
 }
+at::Tensor pack_w4_meta(const at::Tensor& q) {
+  return at::empty_symint({q.sym_size(0), (q.sym_size(1) + 127) / 128 * 16}, q.options().dtype(at::kInt));
+}
+at::Tensor linear_w4_meta(const at::Tensor& x, const at::Tensor& qweight, const at::Tensor&, const std::optional<at::Tensor>&, int64_t,
+                          const std::optional<at::Tensor>&) {
+  return at::empty_symint({x.sym_size(0), qweight.sym_size(0)}, x.options());
+}
+at::Tensor linear_w4_grad_input_meta(const at::Tensor& dy, const at::Tensor& qweight, const at::Tensor&, const std::optional<at::Tensor>&, int64_t,
+                                     std::optional<int64_t> in_features) {
+  return at::empty_symint({dy.sym_size(0), in_features.has_value() ? c10::SymInt(*in_features) : qweight.sym_size(1) * 8}, dy.options());
+}
+std::tuple<at::Tensor, at::Tensor> xent_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, int64_t) {
+  at::Tensor loss = at::empty_symint({x.sym_size(0)}, x.options().dtype(at::kFloat));
+  return {loss, at::empty_like(loss)};
+}
+std::tuple<at::Tensor, at::Tensor> xent_grad_meta(const at::Tensor& x, const at::Tensor& w, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                  int64_t, bool need_dx, bool need_dw) {
+  return {at::empty_symint({need_dx ? x.sym_size(0) : c10::SymInt(0), x.sym_size(1)}, x.options()),
+          at::empty_symint({need_dw ? w.sym_size(0) : c10::SymInt(0), x.sym_size(1)}, w.options())};
+}
 void out_meta(const at::Tensor&, const at::Tensor&, at::Tensor&, int64_t, const at::Tensor&, int64_t) {}
 
 }  // namespace
@@ -231,6 +407,12 @@ TORCH_LIBRARY(moonpoly_ops, m) {
   m.def("linear(Tensor input, Tensor weight) -> Tensor");
   m.def("linear_cpp_selector(Tensor input, Tensor weight) -> Tensor");
   m.def("linear_bias(Tensor input, Tensor weight, Tensor? bias=None) -> Tensor");      // not in the reference's op set
+  // none of the following five is in the reference's op set
+  m.def("pack_w4(Tensor q) -> Tensor");
+  m.def("linear_w4(Tensor input, Tensor qweight, Tensor scales, Tensor? zeros=None, int group_size=128, Tensor? bias=None) -> Tensor");
+  m.def("linear_w4_grad_input(Tensor grad_output, Tensor qweight, Tensor scales, Tensor? zeros=None, int group_size=128, int? in_features=None) -> Tensor");
+  m.def("linear_cross_entropy(Tensor input, Tensor weight, Tensor target, int ignore_index=-100) -> (Tensor loss, Tensor lse)");
+  m.def("linear_cross_entropy_grad(Tensor input, Tensor weight, Tensor target, Tensor lse, Tensor grad_loss, int ignore_index=-100, bool need_dx=True, bool need_dw=True) -> (Tensor, Tensor)");
   m.def("fp16_workspace_size(Tensor input, Tensor weight, int pid, int split_k_slices=2) -> int");
   m.def("fp16_rcc_workspace_size(Tensor a, Tensor b_col, int pid, int split_k_slices=2) -> int");
   m.def("linear_fp16_pid_ws(Tensor input, Tensor weight, int pid, Tensor workspace, int split_k_slices=2) -> Tensor");
@@ -242,6 +424,11 @@ TORCH_LIBRARY_IMPL(moonpoly_ops, CUDA, m) {
   m.impl("linear", &linear_cuda);
   m.impl("linear_cpp_selector", &linear_cpp_selector_cuda);
   m.impl("linear_bias", &linear_bias_cuda);
+  m.impl("pack_w4", &pack_w4);
+  m.impl("linear_w4", &linear_w4);
+  m.impl("linear_w4_grad_input", &linear_w4_grad_input);
+  m.impl("linear_cross_entropy", &linear_cross_entropy);
+  m.impl("linear_cross_entropy_grad", &linear_cross_entropy_grad);
   m.impl("fp16_workspace_size", &fp16_workspace_size);
   m.impl("fp16_rcc_workspace_size", &fp16_rcc_workspace_size);
   m.impl("linear_fp16_pid_ws", &linear_fp16_pid_ws);
@@ -253,6 +440,11 @@ TORCH_LIBRARY_IMPL(moonpoly_ops, Meta, m) {
   m.impl("linear", &linear_meta);
   m.impl("linear_cpp_selector", &linear_meta);
   m.impl("linear_bias", &linear_bias_meta);
+  m.impl("pack_w4", &pack_w4_meta);
+  m.impl("linear_w4", &linear_w4_meta);
+  m.impl("linear_w4_grad_input", &linear_w4_grad_input_meta);
+  m.impl("linear_cross_entropy", &xent_meta);
+  m.impl("linear_cross_entropy_grad", &xent_grad_meta);
   m.impl("fp16_workspace_size", &ws_size_meta);
   m.impl("fp16_rcc_workspace_size", &ws_size_meta);
   m.impl("linear_fp16_pid_ws", &linear_ws_meta);
@@ -265,6 +457,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear_cuda, py::arg("A"), py::arg("B"));
   m.def("linear_cpp_selector", &linear_cpp_selector_cuda, py::arg("A"), py::arg("B"));
   m.def("linear_bias", &linear_bias_cuda, py::arg("A"), py::arg("B"), py::arg("bias") = py::none());
+  m.def("pack_w4", &pack_w4, py::arg("q"));
+  m.def("linear_w4", &linear_w4, py::arg("A"), py::arg("qweight"), py::arg("scales"), py::arg("zeros") = py::none(),
+        py::arg("group_size") = 128, py::arg("bias") = py::none());
+  m.def("linear_w4_grad_input", &linear_w4_grad_input, py::arg("dY"), py::arg("qweight"), py::arg("scales"), py::arg("zeros") = py::none(),
+        py::arg("group_size") = 128, py::arg("in_features") = py::none());
+  m.def("linear_cross_entropy", &linear_cross_entropy, py::arg("A"), py::arg("B"), py::arg("target"), py::arg("ignore_index") = -100);
+  m.def("linear_cross_entropy_grad", &linear_cross_entropy_grad, py::arg("A"), py::arg("B"), py::arg("target"), py::arg("lse"),
+        py::arg("grad_loss"), py::arg("ignore_index") = -100, py::arg("need_dx") = true, py::arg("need_dw") = true);
   m.def("linear_cpp_forced_pid", &linear_cpp_forced_pid, py::arg("A"), py::arg("B"), py::arg("pid"), py::arg("split_k"));
   m.def("fp16_workspace_size", &fp16_workspace_size, py::arg("A"), py::arg("B"), py::arg("pid"), py::arg("split_k_slices") = 2);
   m.def("linear_fp16_pid_ws", &linear_fp16_pid_ws, py::arg("A"), py::arg("B"), py::arg("pid"), py::arg("workspace"),

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stddef.h>
 
+#include "../../include/moonpoly_abi.h"
+
 namespace mp {
 
 // Records the calling thread's error text (mp_last_error_string) and returns `code`.
@@ -34,3 +36,26 @@ int host_pad_rows16(const void* src, long long ld, void* dst, int rows, int k, i
     if (e__ != cudaSuccess)                                                                                           \
       return mp::host_fail(MP_ERR_CUDA, "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e__), __FILE__, __LINE__); \
   } while (0)
+
+namespace mp {
+
+// A launch that may begin while the previous kernel of the stream ends (programmatic dependent launch); its kernel waits
+// (griddepcontrol.wait) before it touches memory.
+template <typename... P, typename... A>
+int host_launch(void (*kern)(P...), int grid, int threads, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = host_use_pdl() ? 1 : 0;
+  MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, P(args)...));
+  host_count_launches(1);
+  return MP_OK;
+}
+
+}  // namespace mp

@@ -204,23 +204,14 @@ inline int operand_maps(OperandMaps* m, const void* ptr, long long inner, long l
 // One stage of one operand: `rows` row indices from r0, contraction blocks kb ... kb + kc - 1.  K-major: [block][row][128 B];
 // MN-major: [64 row indices][kc * 64 contraction indices][128 B].  `blocks` whole blocks of 64 along the lines may be read
 // through the wide map.  Blocks past the end of the contraction are filled with zeros and count their bytes like the others.
-template <bool PAIR = true>
 __device__ __forceinline__ void pair_load(uint32_t dst, const OperandMaps& maps, uint32_t bar, int mn, int blocks, int rows, int r0, int kb, int kc) {
-  const auto load2 = [&](uint32_t d, int x, int y) {
-    if constexpr (PAIR) tma_load_2d_pair(d, &maps.narrow, bar, x, y);
-    else tma_load_2d(d, &maps.narrow, bar, x, y);
-  };
-  const auto load3 = [&](uint32_t d, int x, int y, int z) {
-    if constexpr (PAIR) tma_load_3d_pair(d, &maps.wide, bar, x, y, z);
-    else tma_load_3d(d, &maps.wide, bar, x, y, z);
-  };
   if (mn) {
-    if (r0 + rows <= blocks * 64) load3(dst, 0, kb * 64, r0 >> 6);
-    else for (int j = 0; j < rows; j += 64) load2(dst + (uint32_t)(j * kc * 128), r0 + j, kb * 64);
+    if (r0 + rows <= blocks * 64) tma_load_3d_pair(dst, &maps.wide, bar, 0, kb * 64, r0 >> 6);
+    else for (int j = 0; j < rows; j += 64) tma_load_2d_pair(dst + (uint32_t)(j * kc * 128), &maps.narrow, bar, r0 + j, kb * 64);
   } else if (kb + kc <= blocks) {
-    load3(dst, 0, r0, kb);
+    tma_load_3d_pair(dst, &maps.wide, bar, 0, r0, kb);
   } else {
-    for (int c = 0; c < kc; ++c) load2(dst + (uint32_t)(c * rows * 128), (kb + c) * 64, r0);
+    for (int c = 0; c < kc; ++c) tma_load_2d_pair(dst + (uint32_t)(c * rows * 128), &maps.narrow, bar, (kb + c) * 64, r0);
   }
 }
 

@@ -21,7 +21,7 @@ constexpr int kW4StreamMaxTokens = 16;
 constexpr int kSmsModel = 148;            // workspace sizes must not depend on the device that is asked
 
 struct Plan {
-  bool stream, pair, with_table;
+  bool stream, with_table;
   int bn, tiles_m, tiles_n, steps, split, steps_per_split;
   size_t copy, partial, table, total;     // workspace: aligned copy of the tokens, partial sums, group words
   long long ld_copy, ld_partial;
@@ -41,15 +41,14 @@ Plan w4_plan(int T, int N, int K, int group_size, bool grad, bool copy_tokens) {
   }
   if (p.stream) return p;
   p.steps = ceil_div(contraction, 128);
-  p.pair = T > 128;
-  const int slots = p.pair ? kSmsModel / 2 : kSmsModel;
-  p.tiles_m = ceil_div(rows, p.pair ? 256 : 128);
-  // Tokens per tile (a multiple of 32) and slices of the contraction: the choice whose longest SM (pair) is done first.  A step
+  const int slots = kSmsModel / 2;
+  p.tiles_m = ceil_div(rows, kPairRows);
+  // Tokens per tile (a multiple of 32) and slices of the contraction: the choice whose longest pair is done first.  A step
   // of a tile costs four cycles per token on the tensor cores, or the 900 of the unpacking; a slice at least four steps, and
   // eight for its sums to be written and joined.
   double best = 0.0;
-  const int widest = p.pair ? 256 : 128, whole = (int)round_up((size_t)T, 32);
-  for (int bn = std::min(widest, whole); bn >= (p.pair ? 160 : std::min(widest, whole)); bn -= 32) {
+  const int whole = std::min(256, (int)round_up((size_t)T, 32));
+  for (int bn = whole; bn >= std::min(160, whole); bn -= 32) {
     const int tiles = p.tiles_m * ceil_div(T, bn);
     for (int split = 1; split <= 16 && (split == 1 || p.steps / split >= 4) && (split == 1 || tiles * split <= slots); ++split) {
       const int each = ceil_div(p.steps, split);
@@ -60,8 +59,9 @@ Plan w4_plan(int T, int N, int K, int group_size, bool grad, bool copy_tokens) {
   p.tiles_n = ceil_div(T, p.bn);
   p.steps_per_split = ceil_div(p.steps, p.split);
   p.split = ceil_div(p.steps, p.steps_per_split);
-  // The transposed group words pay for their kernel (3 us) where the weight is unpacked more than once.
-  p.with_table = p.tiles_n > 1;
+  // The transposed group words cost a kernel of 3 us.  They pay where the weight is unpacked for several token tiles, and with
+  // fine groups always (28672 x 4096, groups of 64, 17 tokens: 45 us against 58).
+  p.with_table = p.tiles_n > 1 || group_size < 128;
   if (p.with_table) {
     p.table = p.total;
     p.total += round_up((size_t)ceil_div(K, group_size) * N * 4, 256);
@@ -100,30 +100,6 @@ W4Weight weight_of(int N, int K, const uint32_t* packed, const void* scales, con
   return w;
 }
 
-// Scales (and zeros) of a block's fine groups can be read as one 8- or 4-byte word (and one 4- or 2-byte word).
-int vector_groups(const W4Weight& w) {
-  return w.shift < 2 && w.groups % (4 >> w.shift) == 0 && (reinterpret_cast<uintptr_t>(w.scale) & 7) == 0 &&
-         (reinterpret_cast<uintptr_t>(w.zero) & 3) == 0;
-}
-
-// Launch that may begin while the previous kernel of the stream ends; the kernel waits before it reads anything.
-template <typename P>
-int launch_dependent(void (*kern)(P), const P& p, int grid, int threads, size_t smem, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = host_use_pdl() ? 1 : 0;
-  MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
-  host_count_launches(1);
-  return MP_OK;
-}
-
 template <bool BF16, int NT, int GPB>
 int launch_stream(const HostDevice& d, const W4StreamParams& p, cudaStream_t stream) {
   const W4Weight& w = p.w;
@@ -157,7 +133,7 @@ int launch_stream(const HostDevice& d, const W4StreamParams& p, cudaStream_t str
     MP_HOST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
     done = true;
   }
-  return launch_dependent<W4StreamParams>(kern, p, ctas, kW4StreamWarps * 32, (deep ? 8 : 4) * kBlock + fixed, stream);
+  return host_launch(kern, ctas, kW4StreamWarps * 32, (deep ? 8 : 4) * kBlock + fixed, stream, p);
 }
 
 template <bool BF16, int NT>
@@ -188,78 +164,37 @@ int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, in
   p.partial = reinterpret_cast<float*>(ws + l.partial);
   p.ld_partial = l.ld_partial;
   p.status = d.status;
-  const int hb = l.pair ? l.bn / 2 : l.bn;
+  const int hb = l.bn / 2;
   p.stage_bytes = kW4ABytes + hb * 256;
   // three stages, and the rest of the shared memory for packed bytes on their way from HBM
   p.stages = 3;
   p.raw_slots = std::min(kW4MaxRawSlots, (kPairSmem - 1024 - 256 - p.stages * p.stage_bytes) / kW4RawBytes);
-  p.vec = vector_groups(w);
   OperandMaps tokens;
   CUtensorMap tmW;
   if (int rc = operand_maps(&tokens, x, inner, T, ldx, hb, 2, &p.b_wide)) return rc;
   if (l.with_table) {
     p.table = reinterpret_cast<const uint32_t*>(ws + l.table);
     p.ld_table = w.N;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ceil_div(w.N, 32), (unsigned)ceil_div(w.groups, 32));
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = host_use_pdl() ? 1 : 0;
-    MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&cfg, w4_table_kernel, w.scale, w.zero, w.N, w.groups, reinterpret_cast<uint32_t*>(ws + l.table), w.N));
-    host_count_launches(1);
+    const int across = ceil_div(w.N, 32);
+    if (int rc = host_launch(w4_table_kernel, across * ceil_div(w.groups, 32), 256, 0, stream, w.scale, w.zero, w.N, w.groups, across,
+                                  reinterpret_cast<uint32_t*>(ws + l.table), w.N)) return rc;
   }
   const int line = grad ? 64 : 128;                      // packed bytes per row and box
   if (int rc = host_tmap(&tmW, kTmapByte, w.packed, (long long)w.blocks * 64, w.N, (long long)w.blocks * 64, line, 128, line)) return rc;
   const bool fine = w.shift < 2;
-  auto kern = l.pair ? (fine ? w4_mma_kernel<BF16, true, true> : w4_mma_kernel<BF16, false, true>)
-                     : (fine ? w4_mma_kernel<BF16, true, false> : w4_mma_kernel<BF16, false, false>);
-  static bool ready[64][4] = {};
-  bool& done = ready[d.index & 63][l.pair * 2 + fine];
+  auto kern = fine ? w4_mma_kernel<BF16, true> : w4_mma_kernel<BF16, false>;
+  static bool ready[64][2] = {};
+  bool& done = ready[d.index & 63][fine];
   if (!done) {
     MP_HOST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
     done = true;
   }
-  const int ctas = l.pair ? 2 : 1;
-  cudaLaunchConfig_t run = {};
-  run.gridDim = dim3((unsigned)(ctas * std::max(1, std::min(p.tiles_m * p.tiles_n * p.split, d.sms / ctas))));
-  run.blockDim = dim3(kW4Threads);
-  run.dynamicSmemBytes = kPairSmem;
-  run.stream = stream;
-  cudaLaunchAttribute early[2];
-  int num = 0;
-  if (l.pair) {
-    early[num].id = cudaLaunchAttributeClusterDimension;
-    early[num].val.clusterDim.x = 2;
-    early[num].val.clusterDim.y = early[num].val.clusterDim.z = 1;
-    ++num;
-  }
-  if (host_use_pdl()) {
-    early[num].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early[num].val.programmaticStreamSerializationAllowed = 1;
-    ++num;
-  }
-  run.attrs = early;
-  run.numAttrs = num;
-  MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&run, kern, tokens, tmW, p));
-  host_count_launches(1);
+  const int pairs = std::max(1, std::min(p.tiles_m * p.tiles_n * p.split, d.sms / 2));
+  if (int rc = host_launch(kern, 2 * pairs, kW4Threads, kPairSmem, stream, tokens, tmW, p)) return rc;
   if (p.split > 1) {
     const long long threads = (long long)T * (l.ld_partial / 4);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((threads + 255) / 256));
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = host_use_pdl() ? 1 : 0;
-    MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&cfg, w4_reduce_kernel<BF16>, (const float*)p.partial, p.split, T, p.rows, p.ld_partial, p.bias,
-                                        p.out, p.ldo));
-    host_count_launches(1);
+    return host_launch(w4_reduce_kernel<BF16>, (int)((threads + 255) / 256), 256, 0, stream, p.partial, p.split, T, p.rows, p.ld_partial,
+                            p.bias, p.out, p.ldo);
   }
   return MP_OK;
 }

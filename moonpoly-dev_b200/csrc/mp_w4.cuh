@@ -309,16 +309,16 @@ __global__ void __launch_bounds__(kW4StreamWarps * 32, 1) w4_stream_kernel(const
 }
 
 // ------------------------------------------------------------------------------------------------ more tokens: tcgen05
-// D[rows x bn tokens], rows = output channels (forward, contraction K) or input features (gradient, contraction N): 128 rows
-// per CTA.  PAIR: two CTAs share a 256 x 256 tile (cta_group::2, each loads half of the tokens), which halves the token
-// traffic where the tensor cores are the bound.  Alone: 128 x bn tiles with bn <= 128; with so few tokens a step is
-// over in 300 cycles, and the hand-over between two CTAs (550 cycles a step measured with four stages) and the pair's
-// 78 cycles per instruction at 64 tokens would be the bound.
-// A step is 128 contraction elements: 32 KB of unpacked weight and the tokens' 256 bytes each.  Both directions unpack the
-// same thing -- 128 rows of W by one block of 128 k -- into the same swizzled lines of 64 k; forward, the lines are a K-major
-// operand (line = row of D), in the gradient an MN-major one (line = contraction index).
+// D[rows x bn tokens], rows = output channels (forward, contraction K) or input features (gradient, contraction N): tiles of
+// 256 x bn on CTA pairs (cta_group::2), 128 rows of the weight and half of the tokens per CTA.
+// A step is 128 contraction elements: 32 KB of unpacked weight and bn / 2 token rows of 256 bytes per CTA.  Both directions
+// unpack the same thing -- 128 rows of W by one block of 128 k -- into the same swizzled lines of 64 k; forward, the lines are
+// a K-major operand (line = row of D), in the gradient an MN-major one (line = contraction index).
 // Warps: 0 = TMA of the tokens, 1 = MMA, 2 = TMA of the packed weight, 4..7 = epilogue, 8..15 and 16..23 = unpacking, two
 // groups that take turns of two steps.
+// Bound: up to 128 tokens by the unpacking (900 cycles of a step's two turns at 2100 warp instructions), from 256 on by the
+// tensor cores (1024 cycles a step).  Tiles of single CTAs (128 x bn) were 3 to 8 % faster at 33 and 64 tokens and 9 % slower
+// at 128 x 28672 x 4096, and went.
 constexpr int kW4Threads = 768;
 constexpr int kW4RawBytes = 2 * 128 * 64;     // packed bytes per turn and CTA
 constexpr int kW4MaxRawSlots = 6;
@@ -331,8 +331,7 @@ struct W4PairParams {
   int tiles_m, tiles_n, bn, split, steps_per_split;
   int b_wide;                   // whole blocks of 64 along the tokens' lines
   int stages, stage_bytes, raw_slots;
-  const uint32_t* table; int ld_table;   // PAIR: group words [groups][rows of W] (w4_table_kernel); may be null
-  int vec;                      // the scales (and zeros) of a block's runs are read in one load each
+  const uint32_t* table; int ld_table;   // group words [groups][rows of W] (w4_table_kernel); null: scales and zeros as given
   uint16_t* out; long long ldo; // out[token][row]
   const uint16_t* bias;
   float* partial;               // split > 1: [split][T][rows_pad]
@@ -365,12 +364,13 @@ template <bool BF16> __device__ __forceinline__ uint4 w4_weights(uint32_t word, 
 
 // Scale and zero of every group as one word, scale | zero << 16, transposed to [groups][rows]: the unpacking warps read a
 // step's 128 rows, and rows are neighbours only this way round.  Where they lie, [rows][groups], a step touches 256 lines of
-// L1 for 512 bytes, and the product of 4096 x 28672 x 4096 with groups of 64 took 914 us instead of 755.
-__global__ void __launch_bounds__(256) w4_table_kernel(const uint16_t* scale, const uint8_t* zero, int N, int groups, uint32_t* table, int ld_table) {
+// L1 for 512 bytes: the gradient of 4096 x 28672 x 4096 with groups of 64 took 929 us instead of 715.
+__global__ void __launch_bounds__(256) w4_table_kernel(const uint16_t* scale, const uint8_t* zero, int N, int groups, int across, uint32_t* table,
+                                                       int ld_table) {
   __shared__ uint32_t tile[32][33];
   griddep_launch_dependents();
   griddep_wait();
-  const int n0 = blockIdx.x * 32, g0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n0 = (int)blockIdx.x % across * 32, g0 = (int)blockIdx.x / across * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   for (int i = ty; i < 32; i += 8)
     if (n0 + i < N && g0 + tx < groups) {
       const long long at = (long long)(n0 + i) * groups + g0 + tx;
@@ -382,8 +382,8 @@ __global__ void __launch_bounds__(256) w4_table_kernel(const uint16_t* scale, co
 }
 
 // FINE: groups of 32 or 64, so the runs of a block have scales of their own.
-template <bool BF16, bool FINE, bool PAIR>
-__global__ void __launch_bounds__(kW4Threads, 1)
+template <bool BF16, bool FINE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
 w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant__ CUtensorMap tmW, const W4PairParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -398,46 +398,31 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
   auto rfull_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 4 + b); };
   auto rempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 4 + raw_slots + b); };
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (bar_base - smem_base) + 8u * (uint32_t)(2 * stages + 4 + 2 * raw_slots));
-  // barriers that the MMA issuer waits on live in rank 0 of a pair
-  auto at_leader = [&](uint32_t bar) { return PAIR ? mapa_shared(bar, 0) : bar; };
-  auto arrive = [&](uint32_t bar) {
-    if constexpr (PAIR) mbar_arrive_pair(mapa_shared(bar, 0));
-    else mbar_arrive(bar);
-  };
-  auto commit = [&](uint32_t bar) {
-    if constexpr (PAIR) tc_commit_pair(bar);
-    else tc_commit(bar);
-  };
-
-  constexpr int kCtas = PAIR ? 2 : 1, kRows = 128 * kCtas;
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
-  const int first = (int)blockIdx.x / kCtas, stride = (int)gridDim.x / kCtas;       // units of this CTA (pair)
+  const uint32_t rank = cluster_ctarank();
+  const int first = (int)blockIdx.x >> 1, stride = (int)gridDim.x >> 1;       // units of this pair
   const int units = p.tiles_m * p.tiles_n * p.split;
   int* status = p.status;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 1 + 8 * kCtas); mbar_init(empty_bar(s), 1); }   // TMA + unpacking warps
-    for (int b = 0; b < 2; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), 4 * kCtas); }
+    for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 17); mbar_init(empty_bar(s), 1); }   // 1 + 8 unpacking warps per CTA
+    for (int b = 0; b < 2; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), 8); }
     for (int b = 0; b < raw_slots; ++b) { mbar_init(rfull_bar(b), 1); mbar_init(rempty_bar(b), 8); }
     mbar_fence_init();
     tma_prefetch_desc(&tokens.wide);
     tma_prefetch_desc(&tmW);
   }
-  if (warp == 1) {
-    if constexpr (PAIR) tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
-    else { tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512); tmem_relinquish(); }
-  }
+  if (warp == 1) tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  if constexpr (PAIR) cluster_sync_all();
+  cluster_sync_all();
   // Everything above may overlap the previous kernel of the stream; nothing of it is read or overwritten before it is done.
   griddep_launch_dependents();
   griddep_wait();
 
-  const int hb = p.bn / kCtas;                          // token rows per CTA
+  const int hb = p.bn >> 1;                             // token rows per CTA
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------------------ TMA: tokens
     if (lane == 0) {
@@ -449,8 +434,8 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
         const int b0 = u.tn * p.bn + (int)rank * hb;
         for (int st = u.s0; st < u.s1; ++st) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
-          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), (uint32_t)(kCtas * hb * 256));
-          pair_load<PAIR>(smem_base + (uint32_t)s * (uint32_t)p.stage_bytes + kW4ABytes, tokens, at_leader(full_bar(s)), 0, p.b_wide, hb, b0, st * 2, 2);
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), (uint32_t)(2 * hb * 256));
+          pair_load(smem_base + (uint32_t)s * (uint32_t)p.stage_bytes + kW4ABytes, tokens, mapa_shared(full_bar(s), 0), 0, p.b_wide, hb, b0, st * 2, 2);
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
       }
@@ -469,7 +454,7 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
       int s = 0;
       uint32_t ph = 0, ui = 0;
       bool ok = true;
-      const uint32_t idesc = umma_idesc(1u, BF16 ? 1u : 0u, kRows, (uint32_t)p.bn) | ((uint32_t)p.grad << 15);
+      const uint32_t idesc = umma_idesc(1u, BF16 ? 1u : 0u, kPairRows, (uint32_t)p.bn) | ((uint32_t)p.grad << 15);
       const uint64_t a_base = p.grad ? umma_smem_desc_mn(smem_base, 16384u) : umma_smem_desc_sw128(smem_base);
       const uint64_t b_base = umma_smem_desc_sw128(smem_base) + (kW4ABytes >> 4);
       const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4;
@@ -490,16 +475,15 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
 #pragma unroll
             for (uint32_t kk = 0; kk < 8; ++kk) {
               const uint64_t da = ad + (kk >> 2) * a_blk + (kk & 3u) * a_step, db = bd + (kk >> 2) * b_blk + (kk & 3u) * 2u;
-              if constexpr (PAIR) umma_f16_pair(d_tmem, da, db, idesc, kk > 0 ? 1u : more);
-              else umma_f16(d_tmem, da, db, idesc, kk > 0 ? 1u : more);
+              umma_f16_pair(d_tmem, da, db, idesc, kk > 0 ? 1u : more);
             }
-            commit(empty_bar(s));
+            tc_commit_pair(empty_bar(s));
           }
           __syncwarp();
           more = 1u;
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
-        if (ok && elect_one()) commit(tfull_bar((int)buf));
+        if (ok && elect_one()) tc_commit_pair(tfull_bar((int)buf));
         __syncwarp();
       }
     }
@@ -516,10 +500,10 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
           mbar_arrive_expect_tx(rfull_bar(rs), kW4RawBytes);
           const uint32_t dst = raw_base + (uint32_t)rs * kW4RawBytes;
           if (p.grad) {                                  // two tiles of 128 rows, one block wide
-            tma_load_2d(dst, &tmW, rfull_bar(rs), (u.tm * kCtas + (int)rank) * 64, st * 128);
-            tma_load_2d(dst + kW4RawBytes / 2, &tmW, rfull_bar(rs), (u.tm * kCtas + (int)rank) * 64, st * 128 + 128);
+            tma_load_2d(dst, &tmW, rfull_bar(rs), (u.tm * 2 + (int)rank) * 64, st * 128);
+            tma_load_2d(dst + kW4RawBytes / 2, &tmW, rfull_bar(rs), (u.tm * 2 + (int)rank) * 64, st * 128 + 128);
           } else {                                       // one tile, two blocks wide
-            tma_load_2d(dst, &tmW, rfull_bar(rs), st * 64, u.tm * kRows + (int)rank * 128);
+            tma_load_2d(dst, &tmW, rfull_bar(rs), st * 64, u.tm * kPairRows + (int)rank * 128);
           }
           if (++rs == raw_slots) { rs = 0; rph ^= 1u; }
         }
@@ -539,51 +523,23 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
     const W4Weight& w = p.w;
     constexpr int R = FINE ? 4 : 1;                     // groups that a block of a row meets
     uint32_t sz[2][R];                                  // scale | zero << 16
-    // Scales and zeros of the lane's two rows, a step ahead of their use.  Weights that do not exist (rows past N, runs past
-    // K) get scale 0: they are zero whatever their bits say.
+    // Scales and zeros of the lane's two rows, a step ahead of their use: from the table, or (one group per block and row) from
+    // where they lie.  Weights that do not exist (rows past N, runs past K) get scale 0: they are zero whatever their bits say.
     const auto fetch = [&](int tm, int st) {
-      const int blk = p.grad ? tm * kCtas + (int)rank : st;
-      const int row = (p.grad ? st * 128 : tm * kRows + (int)rank * 128) + r0;
-      if (PAIR && p.table != nullptr) {
+      const int blk = p.grad ? tm * 2 + (int)rank : st;
+      const int row = (p.grad ? st * 128 : tm * kPairRows + (int)rank * 128) + r0;
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-          const int run = blk * 4 + i;
-          const uint32_t* at = p.table + (long long)(run >> w.shift) * p.ld_table + row;
+      for (int i = 0; i < R; ++i) {
+        const int run = blk * 4 + i, group_at = run >> w.shift;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) sz[h][i] = row + 8 * h < w.N && run * 32 < w.K ? __ldg(at + 8 * h) : 8u << 16;
-        }
-        return;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long long line = (long long)(row + 8 * h) * w.groups;
-        const bool real = row + 8 * h < w.N;
-        if (FINE && p.vec) {
-          // groups of 32: four per block; of 64: two.  The last block of a row may have fewer, its line is still whole.
-          uint32_t s0 = 0, s1 = 0, z = 0x08080808u;
-          if (real && blk < w.blocks) {
-            if (w.shift == 0) {
-              const uint2 v = __ldg(reinterpret_cast<const uint2*>(w.scale + line + 4 * blk));
-              s0 = v.x; s1 = v.y;
-              if (w.zero != nullptr) z = __ldg(reinterpret_cast<const uint32_t*>(w.zero + line + 4 * blk));
-            } else {
-              const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(w.scale + line + 2 * blk));
-              s0 = __byte_perm(v, v, 0x1010); s1 = __byte_perm(v, v, 0x3232);
-              if (w.zero != nullptr) z = __byte_perm(__ldg(reinterpret_cast<const uint16_t*>(w.zero + line + 2 * blk)), 0, 0x1100);
-            }
-          }
-          sz[h][0] = (s0 & 0xffffu) | (z & 0xffu) << 16;
-          sz[h][1 % R] = (s0 >> 16) | (z & 0xff00u) << 8;
-          sz[h][2 % R] = (s1 & 0xffffu) | (z & 0xff0000u);
-          sz[h][3 % R] = (s1 >> 16) | (z >> 24) << 16;
-        } else {
-#pragma unroll
-          for (int i = 0; i < R; ++i) {
-            const int run = blk * 4 + i;
-            const bool there = real && run * 32 < w.K;
-            const long long at = line + (run >> w.shift);
-            const uint32_t z = there && w.zero != nullptr ? (uint32_t)__ldg(w.zero + at) : 8u;
-            sz[h][i] = (there ? (uint32_t)__ldg(w.scale + at) : 0u) | z << 16;
+        for (int h = 0; h < 2; ++h) {
+          const bool real = row + 8 * h < w.N && run * 32 < w.K;
+          if (FINE || p.table != nullptr) {
+            sz[h][i] = real ? __ldg(p.table + (long long)group_at * p.ld_table + row + 8 * h) : 8u << 16;
+          } else {
+            const long long at = (long long)(row + 8 * h) * w.groups + group_at;
+            const uint32_t z = real && w.zero != nullptr ? (uint32_t)__ldg(w.zero + at) : 8u;
+            sz[h][i] = (real ? (uint32_t)__ldg(w.scale + at) : 0u) | z << 16;
           }
         }
       }
@@ -651,7 +607,7 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
         st_smem_v4<17408>(od, w4_weights<BF16>(q1.w, magic, zero[1][3 % R], scale[1][3 % R]));
         fence_async_smem();                              // the tensor cores read through the async proxy
         __syncwarp();
-        if (lane == 0) arrive(full_bar(sh));
+        if (lane == 0) mbar_arrive_pair(mapa_shared(full_bar(sh), 0));
         if (++sh == stages) { sh = 0; phh ^= 1u; }
       }
       pass(mine);
@@ -665,7 +621,7 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
     for (int unit = first; unit < units; unit += stride, ++ui) {
       const W4Unit u = w4_unit(p, unit);
       const uint32_t buf = ui & 1u, use = ui >> 1;
-      const int row = u.tm * kRows + (int)rank * 128 + quad * 32 + lane;
+      const int row = u.tm * kPairRows + (int)rank * 128 + quad * 32 + lane;
       const bool live = row < p.rows;
       const float bias = live && p.bias != nullptr ? from16<BF16>(p.bias[row]) : 0.0f;
       if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
@@ -691,18 +647,17 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive(tempty_bar((int)buf));
+      if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));
     }
   }
 
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync_all();
+  cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, 512);
-    else tmem_dealloc(tmem_base, 512);
+    tmem_dealloc_pair(tmem_base, 512);
   }
 }
 

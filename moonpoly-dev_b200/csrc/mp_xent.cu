@@ -208,24 +208,6 @@ void shape_problem(PairProblem* q, int rows, int cols, int contraction, int bn, 
   q->kb_per_split = q->kblocks;
 }
 
-// A launch that may begin while the previous kernel of the stream ends; every kernel here waits before it touches memory.
-template <typename... P, typename... A>
-int launch(void (*kern)(P...), int grid, int threads, size_t smem, cudaStream_t stream, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = host_use_pdl() ? 1 : 0;
-  MP_HOST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, P(args)...));
-  host_count_launches(1);
-  return MP_OK;
-}
-
 template <int EPI>
 int launch_pair(const HostDevice& d, PairParams& p, const PairMaps& maps, cudaStream_t stream) {
   auto kern = pair_gemm_kernel<EPI>;
@@ -241,7 +223,7 @@ int launch_pair(const HostDevice& d, PairParams& p, const PairMaps& maps, cudaSt
   p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - 256) / p.stage_bytes);
   p.status = d.status;
   const int pairs = std::max(1, std::min(p.total_tiles, d.sms / 2));
-  return launch(kern, 2 * pairs, kPairThreads, kPairSmem, stream, maps, p);
+  return host_launch(kern, 2 * pairs, kPairThreads, kPairSmem, stream, maps, p);
 }
 
 // Row tiles that run side by side against one column tile: their operand rows should stay in L2 while the columns pass.
@@ -294,7 +276,7 @@ int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx,
   if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, p.prob[0].a_rows, kStageBlocks, &p.prob[0].a_wide)) return rc;
   if (int rc = operand_maps(&maps.b[0], W, inner, V, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
   if (int rc = launch_pair<PAIR_LSE>(d, p, maps, stream)) return rc;
-  return launch(xent_join_kernel, ceil_div(M, 32), 1024, 0, stream, p.partial, 2 * p.prob[0].tiles_n, M, p.target_logit, target, p.target64,
+  return host_launch(xent_join_kernel, ceil_div(M, 32), 1024, 0, stream, p.partial, 2 * p.prob[0].tiles_n, M, p.target_logit, target, p.target64,
                 ignore_index, V, loss, lse);
 }
 
@@ -387,7 +369,7 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
   }
   if (slices > 0) {
     const long long threads = (long long)M * (l.ld_acc / 4);
-    return launch(xent_dx_kernel, (int)((threads + 255) / 256), 256, 0, stream, reinterpret_cast<const float*>(ws + l.acc), slices, l.acc_slice,
+    return host_launch(xent_dx_kernel, (int)((threads + 255) / 256), 256, 0, stream, reinterpret_cast<const float*>(ws + l.acc), slices, l.acc_slice,
                   l.ld_acc, M, H, scale, reinterpret_cast<uint16_t*>(dX), bf16);
   }
   return MP_OK;

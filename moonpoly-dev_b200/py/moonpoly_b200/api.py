@@ -503,7 +503,7 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zero
             raise ValueError("bias must be a CUDA tensor of N elements in the input dtype")
         bias = bias.contiguous()
     with _device_of(x):
-        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        y = x.new_empty((M, N))
         x, ldx = _rows(x)
         ws, at, size = _w4_workspace(M, N, K, group_size, x, ldx, 0)
         rc = lib().mp_linear_w4(code, M, N, K, x.data_ptr(), ldx, qweight.data_ptr(), scales.data_ptr(), _addr(zeros), group_size,
@@ -521,7 +521,7 @@ def linear_w4_grad_input(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.
     code, N, group_size, qweight, scales, zeros = _w4_checks("linear_w4_grad_input", dy, qweight, scales, zeros, group_size, True, K)
     M = dy.shape[0]
     with _device_of(dy):
-        dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
+        dx = dy.new_empty((M, K))
         dy, ld = _rows(dy)
         ws, at, size = _w4_workspace(M, N, K, group_size, dy, ld, 1)
         rc = lib().mp_linear_w4_grad_input(code, M, N, K, dy.data_ptr(), ld, qweight.data_ptr(), scales.data_ptr(), _addr(zeros),
@@ -619,8 +619,8 @@ def linear_cross_entropy_grad(x: torch.Tensor, w: torch.Tensor, target: torch.Te
         if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != M or t.device != x.device:
             raise ValueError(f"{name} must be M fp32 values on the operands' device")
     with _device_of(x):
-        dx = torch.empty((M, H), dtype=x.dtype, device=x.device) if need_dx else None
-        dw = torch.empty((V, H), dtype=x.dtype, device=x.device) if need_dw else None
+        dx = x.new_empty((M, H)) if need_dx else None
+        dw = x.new_empty((V, H)) if need_dw else None
         x, ldx = _rows(x)
         w, ldw = _rows(w)
         target, lse, grad_loss = target.contiguous(), lse.contiguous(), grad_loss.contiguous()

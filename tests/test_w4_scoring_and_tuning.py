@@ -147,7 +147,7 @@ def test_scoring_and_tuning_through_autograd(api, m):
     within(hidden.detach(), x.detach(), wq, None, m > 16)
     e = exact(hidden.detach(), w.detach(), target, torch.full((m,), 1.0 / float(kept), device="cuda"))
     fwd, bx, bw = bounds(hidden.detach(), w.detach(), e)
-    assert abs(float(loss) - float(e["loss"].sum() / kept)) <= float(fwd.mean()) + 1e-6
+    assert abs(float(loss.detach()) - float(e["loss"].sum() / kept)) <= float(fwd.mean()) + 1e-6
     assert ((hidden.grad.double() - e["dx"]).abs() <= bx).all()
     assert ((w.grad.double() - e["dw"]).abs() <= bw).all()
     within(x.grad, hidden.grad, wq.t(), None, True)

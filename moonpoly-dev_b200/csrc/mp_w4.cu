@@ -113,7 +113,7 @@ int launch_stream(const HostDevice& d, const W4StreamParams& p, cudaStream_t str
     const int rows = ceil_div(w.N, c), tiles = ceil_div(rows, 16);
     // shares are `rows` or `rows` - 1 long, and the shorter may be a single tile, whose sums are parked 16 times
     sums = (size_t)std::max(tiles * 8, 16) * NT * 512;
-    staged = (size_t)rows * w.groups * 4;
+    staged = (size_t)tiles * 16 * w.groups * 4;
     ctas = c;
   };
   bool stage = false;

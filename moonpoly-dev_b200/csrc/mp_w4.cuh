@@ -165,24 +165,26 @@ __global__ void __launch_bounds__(kW4StreamWarps * 32, 1) w4_stream_kernel(const
   const int tiles = (share + 15) >> 4;
   const int kw = tiles > 1 ? 8 : 16, kpart = warp & (kw - 1), tile0 = warp / kw, tile_step = kW4StreamWarps / kw;
   const int outer = kpart < w.blocks && tile0 < tiles ? (w.blocks - kpart + kw - 1) / kw : 0;      // blocks of this warp
-  // shared memory: ring | parked sums | group words
+  // shared memory: ring | parked sums | group words (of whole tiles; those behind the share are whatever was there)
   uint8_t* sums = smem_raw + DEPTH * kSlot;
   uint32_t* words = reinterpret_cast<uint32_t*>(sums + (size_t)tiles * kw * (NT * 512));
 
-  // rows past the end of the share read its last row; their sums are not stored.  Offsets inside a share fit 32 bits: a
-  // share of 4 GB would make a weight of 600 GB.
-  const auto row_in = [&](int tile, int half) { return min(tile * 16 + half * 8 + g, share - 1); };
+  // The last tile of a share may reach into the next one's rows: they are read like any other, their sums are not stored.
+  // Rows past N read as zeros.
   const uint32_t ring = smem_u32(smem_raw) + threadIdx.x * 16u;       // [slot][row half][thread]
-  const uint32_t pitch = (uint32_t)w.blocks * 64u;
-  const uint8_t* base = reinterpret_cast<const uint8_t*>(w.packed) + (size_t)cta_lo * pitch + t * 16;
+  const long long pitch = (long long)w.blocks * 64, tile_bytes = pitch * 16 * tile_step;
+  const int rows_left = w.N - cta_lo - g;                 // from this lane's first row of tile 0 on
+  const uint8_t* src0 = reinterpret_cast<const uint8_t*>(w.packed) + (size_t)(cta_lo + tile0 * 16 + g) * pitch + kpart * 64 + t * 16;
+  const uint8_t* src = src0;
   int b_in = outer > 0 ? kpart : w.blocks, tile_in = tile0;
   const auto issue = [&](uint32_t slot) {
     if (b_in < w.blocks) {
-      const uint8_t* src = base + (size_t)b_in * 64;
-      cp_async16(ring + slot * kSlot, src + (uint32_t)row_in(tile_in, 0) * pitch, true);
-      cp_async16(ring + slot * kSlot + kThreads * 16u, src + (uint32_t)row_in(tile_in, 1) * pitch, true);
+      const bool lo = tile_in * 16 < rows_left, hi = tile_in * 16 + 8 < rows_left;
+      cp_async16(ring + slot * kSlot, lo ? src : reinterpret_cast<const uint8_t*>(w.packed), lo);
+      cp_async16(ring + slot * kSlot + kThreads * 16u, hi ? src + 8 * pitch : reinterpret_cast<const uint8_t*>(w.packed), hi);
+      src += tile_bytes;
       tile_in += tile_step;
-      if (tile_in >= tiles) { tile_in = tile0; b_in += kw; }
+      if (tile_in >= tiles) { tile_in = tile0; b_in += kw; src0 += kw * 64; src = src0; }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -235,15 +237,17 @@ __global__ void __launch_bounds__(kW4StreamWarps * 32, 1) w4_stream_kernel(const
     uint4 xn[4][NT];
     if constexpr (NT == 1) load_x(xn, min(b + kw, w.blocks - 1));
     else if (o > 0) load_x(x, b);
-    // one tile's 16 rows against this block; WHOLE: all four runs exist
-    const auto tile_block = [&](int tile, auto whole) {
-      constexpr bool WHOLE = decltype(whole)::value;
-      uint4* park = reinterpret_cast<uint4*>(sums) + (size_t)(tile * kw + kpart) * (NT * 32) + lane;
-      const int at_lo = row_in(tile, 0) * w.groups + group0, at_hi = row_in(tile, 1) * w.groups + group0;
+    // this warp's tiles, 16 rows each, against this block; WHOLE: all four runs exist
+    const auto tile_block = [&](auto whole, auto start) {
+      constexpr bool WHOLE = decltype(whole)::value, START = decltype(start)::value;
+      uint4* park = reinterpret_cast<uint4*>(sums) + (size_t)(tile0 * kw + kpart) * (NT * 32) + lane;
+      int at_lo = (tile0 * 16 + g) * w.groups + group0;
+      for (int tile = tile0; tile < tiles; tile += tile_step, park += tile_step * kw * (NT * 32), at_lo += tile_step * 16 * w.groups) {
+      const int at_hi = at_lo + 8 * w.groups;
       float acc[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const uint4 v = o > 0 ? park[n * 32] : make_uint4(0, 0, 0, 0);
+        const uint4 v = START ? make_uint4(0, 0, 0, 0) : park[n * 32];
         acc[n][0] = __uint_as_float(v.x); acc[n][1] = __uint_as_float(v.y); acc[n][2] = __uint_as_float(v.z); acc[n][3] = __uint_as_float(v.w);
       }
       asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
@@ -253,7 +257,10 @@ __global__ void __launch_bounds__(kW4StreamWarps * 32, 1) w4_stream_kernel(const
         if (!WHOLE && gi * G >= valid) break;
         uint32_t word_lo, word_hi;
         if constexpr (STAGED) { word_lo = words[at_lo + gi]; word_hi = words[at_hi + gi]; }
-        else { word_lo = w4_group_word<BF16>(w, group_base + at_lo + gi); word_hi = w4_group_word<BF16>(w, group_base + at_hi + gi); }
+        else {                                             // rows past N: any word will do
+          word_lo = tile * 16 < rows_left ? w4_group_word<BF16>(w, group_base + at_lo + gi) : 0u;
+          word_hi = tile * 16 + 8 < rows_left ? w4_group_word<BF16>(w, group_base + at_hi + gi) : 0u;
+        }
         const W4Zero z_lo = w4_zero_of<BF16>(word_lo), z_hi = w4_zero_of<BF16>(word_hi);
         float part[NT][4];
 #pragma unroll
@@ -284,9 +291,16 @@ __global__ void __launch_bounds__(kW4StreamWarps * 32, 1) w4_stream_kernel(const
 #pragma unroll
       for (int n = 0; n < NT; ++n)
         park[n * 32] = make_uint4(__float_as_uint(acc[n][0]), __float_as_uint(acc[n][1]), __float_as_uint(acc[n][2]), __float_as_uint(acc[n][3]));
+      }
     };
-    if (valid >= 4) for (int tile = tile0; tile < tiles; tile += tile_step) tile_block(tile, std::true_type{});
-    else for (int tile = tile0; tile < tiles; tile += tile_step) tile_block(tile, std::false_type{});
+    if (valid < 4) {
+      if (o == 0) tile_block(std::false_type{}, std::true_type{});
+      else tile_block(std::false_type{}, std::false_type{});
+    } else if (o == 0) {
+      tile_block(std::true_type{}, std::true_type{});
+    } else {
+      tile_block(std::true_type{}, std::false_type{});
+    }
     if constexpr (NT == 1) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i][0] = xn[i][0];

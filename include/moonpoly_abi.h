@@ -77,7 +77,7 @@ int mp_w4_pack(int N, int K, const uint8_t* q, long long ldq, uint32_t* packed, 
 
 /* Y[M,N] = X[M,K] * W[N,K]^T (+ bias[N]); dtype MP_FP16 or MP_BF16 is the type of X, scales, bias and Y.  scales: [N, G] and
  * zeros: [N, G] bytes of 0..63 (NULL: 8 everywhere), G = ceil(K / group_size); group_size: a power of two of at least 32
- * (one of at least K gives one scale per row); K a multiple of 32.  X has rows ldx >= K elements apart, Y packed rows.
+ * (one of at least K gives one scale per row); K a multiple of 32, MP_ERR_UNALIGNED_K otherwise.  X has rows ldx >= K elements apart, Y packed rows.
  * fp32 sums; the bias is added to the sum before the only rounding of the result.  Up to 16 rows of X the scale multiplies
  * fp32 sums; beyond, each weight (q - zero) * scale is rounded once to dtype, so it has to be representable there. */
 int mp_linear_w4(int dtype, int M, int N, int K, const void* X, long long ldx, const uint32_t* packed, const void* scales,
@@ -107,7 +107,7 @@ int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx,
  *   d[m,v] = grad_loss[m] * (exp(z[m,v] - lse[m]) - (v == target[m])),   0 in rows whose target is ignore_index
  *   dX[M,H] = d * W,   dW[V,H] = d^T * X          (packed rows, the type of X and W)
  * lse is what mp_linear_xent returned for the same operands.  dX or dW may be NULL.  grad_loss is not read for ignored
- * rows' results.  A target out of range gives NaN gradients.  dW is overwritten, not accumulated. */
+ * rows' results.  A target out of range gives NaN gradients; a row of X that is not finite reaches dW, ignored or not.  dW is overwritten, not accumulated. */
 int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long ldx, const void* W, long long ldw,
                         const void* target, int target_bytes, long long ignore_index, const float* lse, const float* grad_loss,
                         void* dX, void* dW, void* workspace, size_t workspace_bytes, void* stream);

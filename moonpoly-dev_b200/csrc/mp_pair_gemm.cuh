@@ -197,7 +197,10 @@ inline int operand_maps(OperandMaps* m, const void* ptr, long long inner, long l
   }
   if (inner % 64 != 0) {
     if (int rc = host_tmap(&m->narrow, kTmap16, ptr, inner, rows, ld * 2, 64, box_lines, 128)) return rc;
+  } else {
+    m->narrow = m->wide;
   }
+  if (inner < 64) m->wide = m->narrow;                         // never loaded through, but a valid map
   return 0;
 }
 

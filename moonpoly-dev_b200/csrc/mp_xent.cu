@@ -90,14 +90,6 @@ __global__ void __launch_bounds__(256) xent_dx_kernel(const float* acc, int slic
 }
 
 // ------------------------------------------------------------------------------------------------------------ problem
-struct Xent {
-  int dtype, M, V, H;
-  const void* X; long long ldx;
-  const void* W; long long ldw;
-  const void* target; int target64;
-  long long ignore_index;
-};
-
 // Sizes that follow from the shape alone, so that the workspace query and the call agree.
 struct Layout {
   size_t x_copy, w_copy;                  // aligned copies of operands whose rows miss TMA's 16 bytes
@@ -192,7 +184,6 @@ int check_workspace(const char* op, void* ws, size_t have, size_t need) {
   if (reinterpret_cast<uintptr_t>(ws) & 255) return host_fail(MP_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", op);
   return MP_OK;
 }
-
 
 void shape_problem(PairProblem* q, int rows, int cols, int contraction, int bn, int a_mn, int b_mn, int group_m, int tile0) {
   q->rows = rows; q->cols = cols;
@@ -309,8 +300,10 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
   float* scale = reinterpret_cast<float*>(ws + l.scale);
   unsigned* counter = reinterpret_cast<unsigned*>(ws + l.scale) + 1;
   uint16_t* dl = reinterpret_cast<uint16_t*>(ws + l.dl);
-  // the same slices in every piece (a short last piece may leave the last ones without work): sums stay in their order
+  // slices of the same length in every piece: a short last piece leaves the last ones without work, and none is added to
+  // that the first piece has not written
   const int split = dX == nullptr ? 1 : dx_split(M, H, std::min(V, l.piece), dW != nullptr);
+  const int kb_per_split = (int)round_up((size_t)ceil_div(ceil_div(std::min(V, l.piece), 64), split), kStageBlocks);
   const int bf16 = dtype == MP_BF16, target64 = target_bytes == 8;
 
   int slices = 0;                                     // of dX, waiting to be joined
@@ -328,7 +321,7 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       p.col0 = col0; p.lse = lse; p.grad_loss = grad_loss; p.vocab = V; p.scale_out = scale; p.next_unit = counter; p.dlogits = dl; p.ld_dl = l.ld_dl;
       if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, p.prob[0].a_rows, kStageBlocks, &p.prob[0].a_wide)) return rc;
       if (int rc = operand_maps(&maps.b[0], Wp, inner, cols, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
-          if (int rc = launch_pair<PAIR_DLOGITS>(d, p, maps, stream)) return rc;
+      if (int rc = launch_pair<PAIR_DLOGITS>(d, p, maps, stream)) return rc;
     }
     PairParams p{};
     p.bf16 = bf16;
@@ -342,8 +335,8 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       q.acc_slice = l.acc_slice;
       q.add_acc32 = i > 0;
       if (split > 1) {
-        q.kb_per_split = (int)round_up((size_t)ceil_div(q.kblocks, split), kStageBlocks);
-        q.split = ceil_div(q.kblocks, q.kb_per_split);
+        q.kb_per_split = kb_per_split;
+        q.split = ceil_div(q.kblocks, kb_per_split);
         if (i == 0) slices = q.split;
       } else if (i == l.pieces - 1) {
         q.out16 = dX; q.ld_out = H; q.scale = scale;

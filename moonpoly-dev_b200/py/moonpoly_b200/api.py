@@ -571,7 +571,6 @@ def _addr(t: Optional[torch.Tensor]) -> int:
 
 def _xent_checks(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor) -> None:
     _linear_checks(x, w)
-    _dtype16(x, "linear_cross_entropy")
     if w.shape[0] == 0 or w.shape[1] == 0:
         raise ValueError("the weight [V, H] must not be empty")
     if target.dim() != 1 or target.shape[0] != x.shape[0] or target.dtype not in (torch.int64, torch.int32):
@@ -580,11 +579,19 @@ def _xent_checks(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor) -> None
         raise ValueError("x, w and target must be on one device")
 
 
+@functools.lru_cache(maxsize=4096)
+def _xent_workspace_bytes(code: int, M: int, V: int, H: int, aligned: bool, backward: int) -> int:
+    # addresses and row strides that are 16-byte aligned or not: the library looks at nothing else
+    need, ld = ctypes.c_size_t(), (H + 7) // 8 * 8
+    _check(lib().mp_linear_xent_workspace(code, M, V, H, 4096, ld, 4096 if aligned else 4098, ld, backward, ctypes.byref(need)))
+    return need.value
+
+
 def _xent_workspace(code, M, V, H, x, ldx, w, ldw, backward) -> torch.Tensor:
     # a fresh tensor per call: calls on other streams and captured graphs never share it
-    need = ctypes.c_size_t()
-    _check(lib().mp_linear_xent_workspace(code, M, V, H, x.data_ptr(), ldx, w.data_ptr(), ldw, backward, ctypes.byref(need)))
-    return torch.empty((need.value,), dtype=torch.uint8, device=x.device)
+    aligned = (x.data_ptr() | w.data_ptr()) & 15 == 0 and (ldx | ldw) & 7 == 0
+    need = _xent_workspace_bytes(code, M, V, H, aligned, backward)
+    return torch.empty((need,), dtype=torch.uint8, device=x.device)
 
 
 def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, ignore_index: int = -100):

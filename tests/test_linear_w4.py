@@ -114,7 +114,8 @@ def test_forward_against_64_bits(api, m, group, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,n,k,group", [(1, 1, 32, 32), (5, 37, 96, 32), (40, 1, 32, 32), (33, 9473, 256, 64), (1, 9500, 256, 128),
-                                         (20, 9500, 160, 32), (257, 515, 2080, 128), (64, 300, 4096, -1), (3, 300, 4096, -1), (700, 260, 288, 32)])
+                                         (20, 9500, 160, 32), (257, 515, 2080, 128), (64, 300, 4096, -1), (3, 300, 4096, -1), (700, 260, 288, 32),
+                                         (1, 40, 80000, 32), (16, 70000, 64, 32), (3, 30000, 2048, 32), (9, 2400, 1056, 64)])
 def test_forward_sizes(api, m, n, k, group, dtype):
     real = group if group > 0 else 4096
     q, s, z = make(n, k, real, dtype, seed=n)

@@ -125,6 +125,13 @@ def test_many_pieces_of_the_vocabulary(api, dtype):
 
 
 @pytest.mark.gpu
+def test_many_pieces_and_slices(api):
+    # 1000 rows: a piece holds 131072 entries, so 140001 entries are two pieces, and dx's few tiles are cut into slices of the
+    # vocabulary that the short second piece does not fill
+    check(api, *inputs(1000, 140001, 64, torch.float16, seed=6))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("h", [1, 7, 63, 100, 333])
 def test_rows_that_miss_16_bytes(api, h):
     check(api, *inputs(37, 400, h, torch.bfloat16, seed=h))

@@ -167,20 +167,36 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int bf16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// `n` consecutive 16-bit outputs starting at o from v[0..31] (n <= 32); 16-byte stores where the address allows.
-__device__ __forceinline__ void store_row32(uint16_t* o, const float (&v)[32], int n, int bf16) {
-  uint32_t w[16];
+// A warp's block of 32 rows x 64 columns of 16-bit outputs, one row per lane in w, to `o` (its first element; rows `ld`
+// elements apart; `rows` x `cols` of it exist).  By way of 4 KB of shared memory, so that eight lanes write 128 contiguous
+// bytes of a row.  Lanes that wrote their own rows, 16 bytes each, left a part of a sector in 32 rows behind every instruction
+// (both gradients, us: 128 x 32768 x 4096 260 -> 218, 2048 x 32768 x 1023, where rows miss 16 bytes, 538 -> 347,
+// 10 x 21273 x 3280 148 -> 135).
+__device__ __forceinline__ void store_rows64(uint32_t stage, uint16_t* o, long long ld, int rows, int cols, const uint32_t (&w)[32], int lane) {
+  __syncwarp();                                          // the previous block has been read
 #pragma unroll
-  for (int j = 0; j < 16; ++j) w[j] = pack16(v[2 * j], v[2 * j + 1], bf16);
-  if (n == 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+  for (int c = 0; c < 8; ++c)
+    st_smem_v4(stage + (uint32_t)(lane * 128 + ((c ^ (lane & 7)) << 4)), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+  __syncwarp();
+  if (cols >= 64 && ((reinterpret_cast<uintptr_t>(o) | (uintptr_t)(ld * 2)) & 15) == 0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) reinterpret_cast<uint4*>(o)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < n) o[j] = (uint16_t)(j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3), c = lane & 7;
+      uint4 v;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "r"(stage + (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4))) : "memory");
+      if (r < rows) *reinterpret_cast<uint4*>(o + r * ld + c * 8) = v;
+    }
+  } else {                                               // rows that miss 16 bytes, or end inside the block
+    for (int r = 0; r < min(rows, 32); ++r)
+      for (int c = lane; c < min(cols, 64); c += 32) {
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(stage + (uint32_t)(r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2)) : "memory");
+        o[r * ld + c] = v;
+      }
   }
 }
+constexpr int kPairStoreBytes = 8 * 4096;                // of the eight epilogue warps
 
 // The tensor maps of an operand.  `wide` is 3-D and one box brings 256 contiguous bytes per line, two blocks of 64 (1.07 times
 // as fast a main loop as 128-byte boxes); it covers whole blocks only.  `narrow` covers the lines to their last element and is
@@ -353,7 +369,7 @@ __device__ __forceinline__ float pair_grad_max(const PairParams& p, int rows, fl
 // largest |grad_loss| is divided out (a mean over the tokens then rounds exactly: the factors are 1) and, for fp16, replaced
 // by 2^15: a probability of 2e-9 is still a normal fp16 number beside a one.  The products are multiplied by *scale_out.
 __device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
-                                                      int ncols, int half_cols, float grad_max) {
+                                                      int ncols, int half_cols, float grad_max, uint32_t stage) {
   const bool live = row < q.rows;
   long long target = -1;
   float lse = 0.0f, coef = 0.0f;
@@ -365,55 +381,68 @@ __device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const
     lse = p.lse[row];
     coef = t < 0 || t >= p.vocab ? NAN : p.grad_loss[row] / grad_max * (p.bf16 ? 1.0f : 32768.0f);
   }
-  uint16_t* o = p.dlogits + (long long)row * p.ld_dl + c_begin;
-  for (int c0 = 0; c0 < half_cols; c0 += 32) {
-    uint32_t v[32];
-    __syncwarp();
-    tmem_ld_x32(t_addr + (uint32_t)c0, v);
-    tmem_ld_wait();
-    float d[32];
+  const int lane = row & 31, row0 = row - lane;
+  uint16_t* o = p.dlogits + (long long)row0 * p.ld_dl + c_begin;
+  for (int c0 = 0; c0 < half_cols; c0 += 64) {
+    uint32_t w[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) d[j] = kept ? coef * exp2_approx((__uint_as_float(v[j]) - lse) * kLog2e) : 0.0f;
-    if (kept && target >= c0 && target < c0 + 32) {
+    for (int part = 0; part < 2; ++part) {
+      const int c1 = c0 + 32 * part;
+      uint32_t v[32];
+      __syncwarp();
+      tmem_ld_x32(t_addr + (uint32_t)c1, v);
+      tmem_ld_wait();
+      float d[32];
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (target == c0 + j) d[j] = coef * (exp2_approx((__uint_as_float(v[j]) - lse) * kLog2e) - 1.0f);
+      for (int j = 0; j < 32; ++j) d[j] = kept ? coef * exp2_approx((__uint_as_float(v[j]) - lse) * kLog2e) : 0.0f;
+      if (kept && target >= c1 && target < c1 + 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (target == c1 + j) d[j] = coef * (exp2_approx((__uint_as_float(v[j]) - lse) * kLog2e) - 1.0f);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) w[16 * part + j] = pack16(d[2 * j], d[2 * j + 1], p.bf16);
     }
-    const int n = ncols - c0 < 32 ? ncols - c0 : 32;
-    if (live && n > 0) store_row32(o + c0, d, n, p.bf16);
+    if (c0 < ncols) store_rows64(stage, o + c0, p.ld_dl, q.rows - row0, ncols - c0, w, lane);
   }
 }
 
 __device__ __forceinline__ void pair_epilogue_store(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
-                                                    int ncols, int half_cols, int slice) {
+                                                    int ncols, int half_cols, int slice, uint32_t stage) {
   const bool live = row < q.rows;
+  const int lane = row & 31, row0 = row - lane;
   const float scale = (q.out16 != nullptr && q.scale != nullptr) ? *q.scale : 1.0f;
-  for (int c0 = 0; c0 < half_cols; c0 += 32) {
-    uint32_t r[32];
-    __syncwarp();
-    tmem_ld_x32(t_addr + (uint32_t)c0, r);
-    tmem_ld_wait();
-    const int n = ncols - c0 < 32 ? ncols - c0 : 32;
-    if (!live || n <= 0) continue;
-    float v[32];
+  for (int c0 = 0; c0 < half_cols; c0 += 64) {
+    uint32_t w[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-    float* a = q.acc32 + (long long)slice * q.acc_slice + (long long)row * q.ld_acc + c_begin + c0;
-    if (q.add_acc32) {                                  // ld_acc is a multiple of 32: rows of the scratch are padded
+    for (int part = 0; part < 2; ++part) {
+      const int c1 = c0 + 32 * part;
+      uint32_t r[32];
+      __syncwarp();
+      tmem_ld_x32(t_addr + (uint32_t)c1, r);
+      tmem_ld_wait();
+      float v[32];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float4 t = reinterpret_cast<const float4*>(a)[j];
-        v[4 * j] += t.x; v[4 * j + 1] += t.y; v[4 * j + 2] += t.z; v[4 * j + 3] += t.w;
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+      float* a = q.acc32 + (long long)slice * q.acc_slice + (long long)row * q.ld_acc + c_begin + c1;
+      const bool mine = live && c1 < ncols;                // ld_acc is a multiple of 32: rows of the scratch are padded
+      if (q.add_acc32 && mine) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 t = reinterpret_cast<const float4*>(a)[j];
+          v[4 * j] += t.x; v[4 * j + 1] += t.y; v[4 * j + 2] += t.z; v[4 * j + 3] += t.w;
+        }
+      }
+      if (q.out16 != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[16 * part + j] = pack16(v[2 * j] * scale, v[2 * j + 1] * scale, p.bf16);
+      } else if (mine) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) reinterpret_cast<float4*>(a)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
       }
     }
-    if (q.out16 != nullptr) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] *= scale;
-      store_row32(reinterpret_cast<uint16_t*>(q.out16) + (long long)row * q.ld_out + c_begin + c0, v, n, p.bf16);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) reinterpret_cast<float4*>(a)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    }
+    if (q.out16 != nullptr && c0 < ncols)
+      store_rows64(stage, reinterpret_cast<uint16_t*>(q.out16) + (long long)row0 * q.ld_out + c_begin + c0, q.ld_out, q.rows - row0, ncols - c0, w, lane);
   }
 }
 
@@ -565,6 +594,7 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
     uint32_t ui = 0;
     bool ok = true;
     float grad_max = 1.0f;
+    const uint32_t stage = bar_base + 256u + (uint32_t)(warp - 4) * 4096u;       // of this warp, where outputs are 16 bits (kPairStoreBytes)
     if constexpr (EPI == PAIR_DLOGITS) {
       grad_max = pair_grad_max(p, p.prob[0].rows, reinterpret_cast<float*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 48));
       if (blockIdx.x == 0 && threadIdx.x == 128) {
@@ -615,8 +645,8 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
         tc_fence_after();
         const uint32_t t_addr = t_half + buf * (uint32_t)kPairMaxBN;
-        if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols, grad_max);
-        else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols, u.slice);
+        if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols, grad_max, stage);
+        else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols, u.slice, stage);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));

@@ -211,7 +211,7 @@ int launch_pair(const HostDevice& d, PairParams& p, const PairMaps& maps, cudaSt
   p.kc = kStageBlocks;
   const int a_rows = p.num_problems == 2 ? 128 : p.prob[0].a_rows;
   p.stage_bytes = p.kc * (a_rows * 128 + bn / 2 * 128);
-  p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - 256) / p.stage_bytes);
+  p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - 256 - (EPI == PAIR_LSE ? 0 : kPairStoreBytes)) / p.stage_bytes);
   p.status = d.status;
   const int pairs = std::max(1, std::min(p.total_tiles, d.sms / 2));
   return host_launch(kern, 2 * pairs, kPairThreads, kPairSmem, stream, maps, p);

@@ -29,6 +29,8 @@ constexpr int kPairMaxBN = 256;
 constexpr int kPairThreads = 384;             // warps 2 and 3 only fill the first warpgroup up
 constexpr int kPairMaxStages = 8;
 constexpr int kPairSmem = 232448;            // 227 KB opt-in limit per CTA
+constexpr int kPairBarBytes = 512;           // behind the stages: barriers, unit box, TMEM address, 8 floats
+constexpr int kPairBox = 8, kPairAhead = 2;  // slots of the unit box, and units that it holds ahead of the slowest of its readers
 
 enum { PAIR_STORE = 0, PAIR_LSE = 1, PAIR_DLOGITS = 2 };
 
@@ -44,13 +46,12 @@ struct PairProblem {
   int group_m;                   // raster: tiles are walked in groups of `group_m` row tiles
   int tile0;                     // index of the problem's first unit in the launch
   int split, kb_per_split;       // PAIR_STORE: the contraction in `split` slices of kb_per_split blocks, a unit each
-  // PAIR_STORE: out16 = scale * acc (+ acc32 before scaling), or acc32[slice] (+)= acc when out16 is null
+  // PAIR_STORE: out16 = scale * (acc (+ acc32)), or acc32[slice] (+)= acc when out16 is null
   void* out16;
   float* acc32;
   long long ld_out;              // row stride of out16 in elements
   long long ld_acc, acc_slice;   // row stride of acc32, and elements from slice to slice
   int add_acc32;                 // 1: acc32 holds earlier contributions
-  const float* scale;            // device scalar, may be null (1.0)
 };
 
 struct PairParams {
@@ -61,6 +62,7 @@ struct PairParams {
   int stages, stage_bytes;
   int kc;                        // 64-element blocks of the contraction per stage (1 or 2)
   int bf16;                      // operand and output type: 1 = bf16, 0 = fp16
+  const float* scale;            // PAIR_STORE: device scalar
   int* status;
   // PAIR_LSE / PAIR_DLOGITS (the columns of D are vocabulary entries col0 ... col0 + cols - 1)
   const void* target; int target64;
@@ -171,29 +173,34 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int bf16) {
 // elements apart; `rows` x `cols` of it exist).  By way of 4 KB of shared memory, so that eight lanes write 128 contiguous
 // bytes of a row.  Lanes that wrote their own rows, 16 bytes each, left a part of a sector in 32 rows behind every instruction
 // (both gradients, us: 128 x 32768 x 4096 260 -> 218, 2048 x 32768 x 1023, where rows miss 16 bytes, 538 -> 347,
-// 10 x 21273 x 3280 148 -> 135).
+// 10 x 21273 x 3280 148 -> 135).  Blocks that end inside the 64 columns take the same path while whole 16 bytes of them are
+// left (2 x 9964 x 1744: 47 -> 41).
 __device__ __forceinline__ void store_rows64(uint32_t stage, uint16_t* o, long long ld, int rows, int cols, const uint32_t (&w)[32], int lane) {
   __syncwarp();                                          // the previous block has been read
 #pragma unroll
   for (int c = 0; c < 8; ++c)
     st_smem_v4(stage + (uint32_t)(lane * 128 + ((c ^ (lane & 7)) << 4)), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
   __syncwarp();
-  if (cols >= 64 && ((reinterpret_cast<uintptr_t>(o) | (uintptr_t)(ld * 2)) & 15) == 0) {
+  if ((cols >= 64 || cols % 8 == 0) && ((reinterpret_cast<uintptr_t>(o) | (uintptr_t)(ld * 2)) & 15) == 0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = i * 4 + (lane >> 3), c = lane & 7;
       uint4 v;
       asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                    : "r"(stage + (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4))) : "memory");
-      if (r < rows) *reinterpret_cast<uint4*>(o + r * ld + c * 8) = v;
+      if (r < rows && c * 8 < cols) *reinterpret_cast<uint4*>(o + r * ld + c * 8) = v;
     }
-  } else {                                               // rows that miss 16 bytes, or end inside the block
-    for (int r = 0; r < min(rows, 32); ++r)
-      for (int c = lane; c < min(cols, 64); c += 32) {
-        uint16_t v;
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(stage + (uint32_t)(r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2)) : "memory");
-        o[r * ld + c] = v;
-      }
+  } else {                                               // rows that miss 16 bytes
+    const bool c0 = lane < cols, c1 = lane + 32 < cols;
+    const uint32_t in = stage + (uint32_t)(lane & 7) * 2;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      uint16_t v0, v1;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v0) : "r"(in + (uint32_t)(r * 128 + (((lane >> 3) ^ (r & 7)) << 4))) : "memory");
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v1) : "r"(in + (uint32_t)(r * 128 + (((4 + (lane >> 3)) ^ (r & 7)) << 4))) : "memory");
+      if (c0 && r < rows) o[r * ld + lane] = v0;
+      if (c1 && r < rows) o[r * ld + lane + 32] = v1;
+    }
   }
 }
 constexpr int kPairStoreBytes = 8 * 4096;                // of the eight epilogue warps
@@ -262,35 +269,40 @@ __host__ __device__ __forceinline__ PairUnit pair_unit(const PairParams& p, int 
 
 // Where the roles of a CTA get their units from.  Static: pair, pair + pairs, ...  Dynamic (units of different lengths):
 // the first unit is the pair's own number, further ones come from a counter in global memory; warp 2 of rank 0 fetches them
-// and posts them in a two-slot box in the shared memory of both CTAs, which every role reads and hands back.  Which pair
-// computes a unit has no influence on its result.
+// and posts them in a box in the shared memory of both CTAs.  The producers and the MMA issuer hand a unit back when they
+// read it.  The epilogue warps do not: an arrival in the other CTA would wait for the stores behind them (128 x 32768 x 4096,
+// both gradients: 218 us instead of 204).  The box has kPairBox slots for that: a unit is posted when the one kPairAhead
+// before it has been handed back; the MMA issuer has then seen the accumulator free that the third unit before that one
+// filled, and kPairAhead + 3 <= kPairBox.  Taking 3 or 4 units ahead is no faster, 1 is slower by 5 %.
+// Which pair computes a unit has no influence on its result.
 template <bool DYNAMIC>
 struct PairUnits {
   const PairParams& p;
-  uint32_t box, bars;            // slots (4 bytes each) and barriers (box_full[2], box_empty[2], 8 bytes each)
+  uint32_t box, bars;            // slots (4 bytes each) and barriers (box_full[kPairBox], box_empty[kPairBox], 8 bytes each)
   int unit, step;
   uint32_t n = 0;
   __device__ PairUnits(const PairParams& p_, uint32_t box_, uint32_t bars_, int pair, int pairs) : p(p_), box(box_), bars(bars_), unit(pair - pairs), step(pairs) {}
   // The next unit, or -1.  Called by one lane.
-  __device__ __forceinline__ int next() {
+  __device__ __forceinline__ int next(bool hands_back = true) {
     if constexpr (!DYNAMIC) {
       unit += step;
       return unit < p.total_tiles ? unit : -1;
     } else {
-      const uint32_t slot = n & 1u, ph = (n >> 1) & 1u;
+      const uint32_t slot = n % kPairBox, ph = n / kPairBox & 1u;
       ++n;
       if (!mbar_wait_cluster(bars + 8u * slot, ph, p.status, MP_DEV_TIMEOUT_CLUSTER)) return -1;
       int v;
       asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(box + 4u * slot) : "memory");
-      mbar_arrive_cluster(mapa_shared(bars + 16u + 8u * slot, 0));
+      if (hands_back) mbar_arrive_cluster(mapa_shared(bars + 8u * (kPairBox + slot), 0));
       return v < p.total_tiles ? v : -1;
     }
   }
   // Warp 2 of rank 0, one lane: posts units until the roles have been told that there are none left.
   __device__ __forceinline__ void post(int pair, int pairs) {
     for (uint32_t i = 0;; ++i) {
-      const uint32_t slot = i & 1u, ph = (i >> 1) & 1u;
-      if (!mbar_wait_cluster(bars + 16u + 8u * slot, ph ^ 1u, p.status, MP_DEV_TIMEOUT_CLUSTER)) return;
+      const uint32_t slot = i % kPairBox, back = i - (uint32_t)kPairAhead;
+      if (i >= (uint32_t)kPairAhead &&
+          !mbar_wait_cluster(bars + 8u * (kPairBox + back % kPairBox), back / kPairBox & 1u, p.status, MP_DEV_TIMEOUT_CLUSTER)) return;
       const int v = i == 0 ? pair : (int)atomicAdd(p.next_unit, 1u) + pairs;
       for (uint32_t r = 0; r < 2; ++r) {
         asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(mapa_shared(box + 4u * slot, r)), "r"(v) : "memory");
@@ -408,10 +420,9 @@ __device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const
 }
 
 __device__ __forceinline__ void pair_epilogue_store(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
-                                                    int ncols, int half_cols, int slice, uint32_t stage) {
+                                                    int ncols, int half_cols, int slice, float scale, uint32_t stage) {
   const bool live = row < q.rows;
   const int lane = row & 31, row0 = row - lane;
-  const float scale = (q.out16 != nullptr && q.scale != nullptr) ? *q.scale : 1.0f;
   for (int c0 = 0; c0 < half_cols; c0 += 64) {
     uint32_t w[32];
 #pragma unroll
@@ -460,8 +471,8 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
   auto empty_bar = [&](int s) { return bar_base + 8u * (uint32_t)(stages + s); };
   auto tfull_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + b); };
   auto tempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 2 + b); };
-  const uint32_t unit_bars = bar_base + 8u * (uint32_t)(2 * stages + 4), unit_box = unit_bars + 32u;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 40);
+  const uint32_t unit_bars = bar_base + 8u * (uint32_t)(2 * stages + 4), unit_box = unit_bars + 16u * kPairBox;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 20 * kPairBox);
   constexpr bool DYNAMIC = EPI == PAIR_STORE;
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -473,9 +484,9 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(tfull_bar(b), 1); mbar_init(tempty_bar(b), 16); }
-    for (uint32_t b = 0; b < 2; ++b) {
+    for (uint32_t b = 0; b < (uint32_t)kPairBox; ++b) {
       mbar_init(unit_bars + 8u * b, 1);
-      mbar_init(unit_bars + 16u + 8u * b, 19);          // two producers, the MMA issuer, sixteen epilogue warps
+      mbar_init(unit_bars + 8u * (uint32_t)(kPairBox + b), 3);           // two producers and the MMA issuer
     }
     mbar_fence_init();
     for (int i = 0; i < p.num_problems; ++i) { tma_prefetch_desc(&maps.a[i].wide); tma_prefetch_desc(&maps.b[i].wide); }
@@ -594,9 +605,10 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
     uint32_t ui = 0;
     bool ok = true;
     float grad_max = 1.0f;
-    const uint32_t stage = bar_base + 256u + (uint32_t)(warp - 4) * 4096u;       // of this warp, where outputs are 16 bits (kPairStoreBytes)
+    const uint32_t stage = bar_base + kPairBarBytes + (uint32_t)(warp - 4) * 4096u;       // of this warp, where outputs are 16 bits (kPairStoreBytes)
+    const float scale = EPI == PAIR_STORE ? *p.scale : 1.0f;
     if constexpr (EPI == PAIR_DLOGITS) {
-      grad_max = pair_grad_max(p, p.prob[0].rows, reinterpret_cast<float*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 48));
+      grad_max = pair_grad_max(p, p.prob[0].rows, reinterpret_cast<float*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 20 * kPairBox + 8));
       if (blockIdx.x == 0 && threadIdx.x == 128) {
         *p.scale_out = grad_max / (p.bf16 ? 1.0f : 32768.0f);
         *p.next_unit = 0u;                               // of the products' launch
@@ -605,7 +617,7 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
     while (ok) {
       int unit = 0;
       if constexpr (DYNAMIC) {
-        if (lane == 0) unit = units.next();
+        if (lane == 0) unit = units.next(false);
         unit = __shfl_sync(0xffffffffu, unit, 0);
       } else {
         unit = units.next();
@@ -646,7 +658,7 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         tc_fence_after();
         const uint32_t t_addr = t_half + buf * (uint32_t)kPairMaxBN;
         if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols, grad_max, stage);
-        else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols, u.slice, stage);
+        else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols, u.slice, scale, stage);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));

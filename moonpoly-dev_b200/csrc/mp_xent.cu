@@ -211,7 +211,7 @@ int launch_pair(const HostDevice& d, PairParams& p, const PairMaps& maps, cudaSt
   p.kc = kStageBlocks;
   const int a_rows = p.num_problems == 2 ? 128 : p.prob[0].a_rows;
   p.stage_bytes = p.kc * (a_rows * 128 + bn / 2 * 128);
-  p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - 256 - (EPI == PAIR_LSE ? 0 : kPairStoreBytes)) / p.stage_bytes);
+  p.stages = std::min(kPairMaxStages, (kPairSmem - 1024 - kPairBarBytes - (EPI == PAIR_LSE ? 0 : kPairStoreBytes)) / p.stage_bytes);
   p.status = d.status;
   const int pairs = std::max(1, std::min(p.total_tiles, d.sms / 2));
   return host_launch(kern, 2 * pairs, kPairThreads, kPairSmem, stream, maps, p);
@@ -326,6 +326,7 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
     PairParams p{};
     p.bf16 = bf16;
     p.next_unit = counter;
+    p.scale = scale;
     int n = 0;
     if (dX != nullptr) {                              // dX[M, H] (+)= d[M, cols] W[cols, H]
       PairProblem& q = p.prob[n];
@@ -339,7 +340,7 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
         q.split = ceil_div(q.kblocks, kb_per_split);
         if (i == 0) slices = q.split;
       } else if (i == l.pieces - 1) {
-        q.out16 = dX; q.ld_out = H; q.scale = scale;
+        q.out16 = dX; q.ld_out = H;
       }
       if (int rc = operand_maps(&maps.a[n], dl, cols, M, l.ld_dl, q.a_rows, kStageBlocks, &q.a_wide)) return rc;
       if (int rc = operand_maps(&maps.b[n], Wp, inner, cols, ldw, kStageBlocks * 64, q.bn / 2 / 64, &q.b_wide)) return rc;
@@ -351,7 +352,6 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       shape_problem(&q, cols, H, M, kPairMaxBN, 1, 1, 8, p.total_tiles);
       q.out16 = reinterpret_cast<uint16_t*>(dW) + (long long)col0 * H;
       q.ld_out = H;
-      q.scale = scale;
       if (int rc = operand_maps(&maps.a[n], dl, cols, M, l.ld_dl, kStageBlocks * 64, 128 / 64, &q.a_wide)) return rc;
       if (int rc = operand_maps(&maps.b[n], X, inner, M, ldx, kStageBlocks * 64, q.bn / 2 / 64, &q.b_wide)) return rc;
       p.total_tiles += q.tiles_m * q.tiles_n;

@@ -26,7 +26,7 @@ namespace mp {
 
 constexpr int kPairRows = 256;               // rows of D per tile
 constexpr int kPairMaxBN = 256;
-constexpr int kPairThreads = 384;             // warps 2 and 3 only fill the first warpgroup up
+constexpr int kPairThreads = 384;             // warp 2 of PAIR_STORE posts units; it and warp 3 fill the first warpgroup up
 constexpr int kPairMaxStages = 8;
 constexpr int kPairSmem = 232448;            // 227 KB opt-in limit per CTA
 constexpr int kPairBarBytes = 512;           // behind the stages: barriers, unit box, TMEM address, 8 floats

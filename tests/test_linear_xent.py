@@ -132,6 +132,36 @@ def test_many_pieces_and_slices(api):
 
 
 @pytest.mark.gpu
+def test_many_short_units(api):
+    # 5 rows: 274 x 6 tiles of dw of one short product each, some twenty for every pair of CTAs, the last of 24 columns
+    check(api, *inputs(5, 70013, 1304, torch.bfloat16, seed=12))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0, 1, 4, 8])
+@pytest.mark.parametrize("h", [264, 315, 332])
+def test_outputs_keep_to_their_elements(api, h, offset):
+    # gradients that start at any element of a larger buffer: the same values, and nothing around them is written
+    import ctypes
+    m, v = 37, 1003
+    x, w, target, g = inputs(m, v, h, torch.float16, seed=h)
+    lse = api.linear_cross_entropy(x, w, target)[1]
+    want = api.linear_cross_entropy_grad(x, w, target, lse, g)
+    bufs = [torch.full((r * h + 64,), 7.0, dtype=x.dtype, device="cuda") for r in (m, v)]
+    views = [b[16 + offset:16 + offset + r * h].view(r, h) for b, r in zip(bufs, (m, v))]
+    n, p = ctypes.c_size_t(), lambda t: ctypes.c_void_p(t.data_ptr())
+    common = [api.MP_FP16, m, v, h, p(x), h, p(w), h]
+    assert api.lib().mp_linear_xent_workspace(*common, 1, ctypes.byref(n)) == 0
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert api.lib().mp_linear_xent_grad(*common, p(target), 8, IGNORE, p(lse), p(g), p(views[0]), p(views[1]), p(ws), n.value, stream) == 0
+    torch.cuda.synchronize()
+    for b, t, r, e in zip(bufs, views, (m, v), want):
+        assert torch.equal(t, e)
+        assert (b[:16 + offset] == 7.0).all() and (b[16 + offset + r * h:] == 7.0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("h", [1, 7, 63, 100, 333])
 def test_rows_that_miss_16_bytes(api, h):
     check(api, *inputs(37, 400, h, torch.bfloat16, seed=h))

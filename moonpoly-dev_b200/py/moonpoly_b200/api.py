@@ -426,6 +426,8 @@ def scaled_int8_mm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_s
 def pack_w4(q: torch.Tensor) -> torch.Tensor:
     """q [N, K] uint8 of values 0..15 -> the packed weight of `linear_w4`, int32 [N, 16 * ceil(K / 128)] (the bit layout
     is in moonpoly_abi.h).  Once per weight, when a model is loaded."""
+    if q.dim() == 2:
+        _fits_int("pack_w4", q.shape[0] | q.shape[1])
     if q.dim() != 2 or q.dtype != torch.uint8 or not q.is_cuda:
         raise ValueError("q must be a 2-D CUDA uint8 tensor [N, K]")
     N, K = q.shape
@@ -436,12 +438,19 @@ def pack_w4(q: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _fits_int(op: str, extents: int) -> None:
+    """Extents, or-ed.  The library takes them as C ints, and ctypes would drop their upper bits."""
+    if extents > 0x7fffffff:
+        raise ValueError(f"{op}: an extent does not fit 32 bits")
+
+
 _W4_CODES = {torch.float16: MP_FP16, torch.bfloat16: MP_BF16}
 
 
 def _w4_checks(op: str, x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros, group_size: int, grad: bool, K: int):
     if x.dim() != 2 or qweight.dim() != 2:
         raise ValueError(f"{op}: input and packed weight must be 2-D tensors")
+    _fits_int(op, x.shape[0] | qweight.shape[0] | K)
     code = _W4_CODES.get(x.dtype)
     if code is None:
         raise ValueError(f"{op} serves fp16 and bf16")
@@ -456,6 +465,8 @@ def _w4_checks(op: str, x: torch.Tensor, qweight: torch.Tensor, scales: torch.Te
         group_size = max(32, 1 << (K - 1).bit_length())
     elif group_size < 32 or group_size & (group_size - 1):
         raise ValueError(f"{op}: group_size must be a power of two of at least 32, or -1")
+    else:
+        _fits_int(op, group_size)
     shape = (N, (K + group_size - 1) // group_size)
     if scales.dtype != x.dtype or scales.shape != shape:
         raise ValueError(f"{op}: scales must be {list(shape)} in the input dtype")
@@ -570,6 +581,8 @@ def _addr(t: Optional[torch.Tensor]) -> int:
 
 
 def _xent_checks(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor) -> None:
+    if x.dim() == w.dim() == 2:
+        _fits_int("linear_cross_entropy", x.shape[0] | w.shape[0] | w.shape[1])
     _linear_checks(x, w)
     if w.shape[0] == 0 or w.shape[1] == 0:
         raise ValueError("the weight [V, H] must not be empty")
@@ -618,7 +631,7 @@ def linear_cross_entropy_grad(x: torch.Tensor, w: torch.Tensor, target: torch.Te
                               ignore_index: int = -100, need_dx: bool = True, need_dw: bool = True):
     """(dx [M,H], dw [V,H]) of `linear_cross_entropy` for grad_loss [M] (fp32, the gradient with respect to `loss`); `lse`
     is what the forward call returned.  A gradient that is not needed is None and costs nothing.  The logits are computed
-    again, a piece of the vocabulary at a time.  Deterministic: no atomics, fixed order of sums."""
+    again, a piece of the vocabulary at a time.  Deterministic: every sum has a fixed order."""
     _xent_checks(x, w, target)
     code = _dtype16(x, "linear_cross_entropy_grad")
     (M, H), V = x.shape, w.shape[0]

@@ -213,6 +213,12 @@ std::tuple<int, int, int, int> scaled_mm_config(int id) {
 }
 
 // ------------------------------------------------------------------------------------------ 4-bit Linear (not in the reference)
+// The library takes extents as ints.
+void require_int(const char* op, std::initializer_list<int64_t> extents) {
+  for (int64_t e : extents)
+    if (e > INT32_MAX) require(false, std::string(op) + ": an extent does not fit 32 bits");
+}
+
 int code16(const at::Tensor& t, const char* op) {
   require(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, std::string(op) + ": fp16 or bf16 only");
   return t.scalar_type() == at::kHalf ? MP_FP16 : MP_BF16;
@@ -233,6 +239,7 @@ at::Tensor workspace_of(size_t bytes, const at::Tensor& like) {
 
 at::Tensor pack_w4(const at::Tensor& q) {
   require(q.is_cuda() && q.dim() == 2 && q.scalar_type() == at::kByte, "pack_w4: q must be a 2D CUDA uint8 tensor [N, K]");
+  require_int("pack_w4", {q.size(0), q.size(1)});
   c10::cuda::CUDAGuard guard(q.device());
   long long ld = 0;
   const at::Tensor qc = packed_rows(q, &ld);
@@ -256,6 +263,7 @@ W4Args w4_args(const char* name, const at::Tensor& x, const at::Tensor& qweight,
   W4Args a;
   a.code = code16(x, name);
   const int64_t N = qweight.size(0);
+  require_int(name, {x.size(0), N, K, group_size});
   require(qweight.scalar_type() == at::kInt && N > 0 && K > 0 && qweight.size(1) == (K + 127) / 128 * 16, op + ": the packed weight must be int32 [N, 16 * ceil(K / 128)]");
   require(x.size(1) == (grad ? N : K), op + ": input width does not match the weight");
   require(K % 32 == 0, op + ": K must be a multiple of 32");
@@ -331,6 +339,7 @@ XentArgs xent_args(const char* name, const at::Tensor& x, const at::Tensor& w, c
   require(x.scalar_type() == w.scalar_type(), op + ": hidden states and weight dtypes differ");
   require(target.dim() == 1 && target.size(0) == x.size(0) && (target.scalar_type() == at::kLong || target.scalar_type() == at::kInt), op + ": target must be M integers (int64 or int32)");
   require(w.device() == x.device() && target.device() == x.device(), op + ": tensors must be on one device");
+  require_int(name, {x.size(0), w.size(0), x.size(1)});
   XentArgs a;
   a.code = code16(x, name);
   a.x = packed_rows(x, &a.ldx);

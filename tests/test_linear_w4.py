@@ -79,6 +79,18 @@ def test_argument_checks(api):
             call()
 
 
+def test_extents_beyond_32_bits_are_refused(api):
+    # 2^32 + 8 rows would reach the library as 8
+    big = 2 ** 32 + 8
+    meta = lambda *shape, t=torch.float16: torch.empty(shape, dtype=t, device="meta")
+    w, s = meta(8, 16, t=torch.int32), meta(8, 2)
+    for call in (lambda: api.linear_w4(meta(big, 64), w, s, group_size=32), lambda: api.linear_w4(meta(2, 64), meta(big, 16, t=torch.int32), meta(big, 2), group_size=32),
+                 lambda: api.linear_w4(meta(2, 64), w, meta(8, 1), group_size=2 ** 40), lambda: api.linear_w4_grad_input(meta(big, 8), w, s, group_size=32, in_features=64),
+                 lambda: api.pack_w4(meta(big, 1, t=torch.uint8))):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+
+
 # ------------------------------------------------------------------------------------------------------------ results
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,k", [(1, 32), (3, 160), (17, 128), (64, 4096), (5, 100), (2, 1)])

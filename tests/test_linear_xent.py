@@ -77,6 +77,17 @@ def test_refusals_name_their_argument(api):
             bad()
 
 
+def test_extents_beyond_32_bits_are_refused(api):
+    # 2^32 + 10 entries would reach the library as 10
+    big = 2 ** 32 + 10
+    meta = lambda *shape, t=torch.float16: torch.empty(shape, dtype=t, device="meta")
+    for m, v in ((4, big), (big, 4)):
+        x, w, target, g = meta(m, 1), meta(v, 1), meta(m, t=torch.int64), meta(m, t=torch.float32)
+        for call in (lambda: api.linear_cross_entropy(x, w, target), lambda: api.linear_cross_entropy_grad(x, w, target, g, g)):
+            with pytest.raises(ValueError, match="32 bits"):
+                call()
+
+
 def test_abi_refusals_need_no_gpu(api):
     import ctypes
     L, n = api.lib(), ctypes.c_size_t()

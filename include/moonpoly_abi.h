@@ -77,7 +77,8 @@ int mp_w4_pack(int N, int K, const uint8_t* q, long long ldq, uint32_t* packed, 
 
 /* Y[M,N] = X[M,K] * W[N,K]^T (+ bias[N]); dtype MP_FP16 or MP_BF16 is the type of X, scales, bias and Y.  scales: [N, G] and
  * zeros: [N, G] bytes of 0..63 (NULL: 8 everywhere), G = ceil(K / group_size); group_size: a power of two of at least 32
- * (one of at least K gives one scale per row); K a multiple of 32, MP_ERR_UNALIGNED_K otherwise.  X has rows ldx >= K elements apart, Y packed rows.
+ * (one of at least K gives one scale per row); K a multiple of 32, MP_ERR_UNALIGNED_K otherwise; M, N and K up to 2^28.
+ * X has rows ldx >= K elements apart, Y packed rows.
  * fp32 sums; the bias is added to the sum before the only rounding of the result.  Up to 16 rows of X the scale multiplies
  * fp32 sums; beyond, each weight (q - zero) * scale is rounded once to dtype, so it has to be representable there. */
 int mp_linear_w4(int dtype, int M, int N, int K, const void* X, long long ldx, const uint32_t* packed, const void* scales,
@@ -98,7 +99,7 @@ int mp_linear_w4_workspace(int M, int N, int K, int group_size, const void* X, l
  *             ignore_index nor in [0, V).
  * dtype: MP_FP16 or MP_BF16 (X and W); loss, lse: M floats.  X and W are row-major with row strides ldx, ldw >= H in
  * elements.  target: target_bytes = 4 (int32) or 8 (int64).  Operands whose rows are not 16-byte aligned are copied into
- * the workspace once per call.  M = 0 computes nothing. */
+ * the workspace once per call.  M, V and H up to 2^30; M = 0 computes nothing. */
 int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx, const void* W, long long ldw, const void* target,
                    int target_bytes, long long ignore_index, float* loss, float* lse, void* workspace, size_t workspace_bytes,
                    void* stream);

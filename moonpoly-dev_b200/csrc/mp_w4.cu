@@ -74,10 +74,12 @@ Plan w4_plan(int T, int N, int K, int group_size, bool grad, bool copy_tokens) {
   return p;
 }
 
+constexpr int kMaxExtent = 1 << 28;
+
 int check_args(const char* op, int dtype, int M, int N, int K, const void* x, long long ldx, int width, const uint32_t* packed,
                const void* scales, int group_size) {
   if (dtype != MP_FP16 && dtype != MP_BF16) return host_fail(MP_ERR_INVALID_ARG, "%s: dtype must be MP_FP16 or MP_BF16", op);
-  if (M < 0 || N <= 0 || K <= 0 || M > (1 << 28) || N > (1 << 28) || K > (1 << 28))
+  if (M < 0 || N <= 0 || K <= 0 || M > kMaxExtent || N > kMaxExtent || K > kMaxExtent)
     return host_fail(MP_ERR_INVALID_ARG, "%s: needs M >= 0, N > 0, K > 0, none above 2^28 (got %d, %d, %d)", op, M, N, K);
   if (K % 32 != 0) return host_fail(MP_ERR_UNALIGNED_K, "%s: K = %d is not a multiple of 32", op, K);
   if (group_size < 32 || (group_size & (group_size - 1)) != 0)
@@ -242,7 +244,8 @@ int run_w4(const char* op, bool grad, int dtype, int M, int N, int K, const void
 extern "C" {
 
 int mp_w4_pack(int N, int K, const uint8_t* q, long long ldq, uint32_t* packed, void* stream) {
-  if (N < 0 || K < 0 || ldq < K) return host_fail(MP_ERR_INVALID_ARG, "mp_w4_pack: needs N >= 0, K >= 0, ldq >= K");
+  if (N < 0 || K < 0 || ldq < K || N > kMaxExtent || K > kMaxExtent)
+    return host_fail(MP_ERR_INVALID_ARG, "mp_w4_pack: needs N >= 0, K >= 0, neither above 2^28, ldq >= K");
   if (N == 0 || K == 0) return MP_OK;
   if (q == nullptr || packed == nullptr) return host_fail(MP_ERR_INVALID_ARG, "mp_w4_pack: null pointer");
   HostDevice d;
@@ -257,8 +260,8 @@ int mp_w4_pack(int N, int K, const uint8_t* q, long long ldq, uint32_t* packed, 
 }
 
 int mp_linear_w4_workspace(int M, int N, int K, int group_size, const void* X, long long ldx, int grad_input, size_t* bytes) {
-  if (bytes == nullptr || M < 0 || N <= 0 || K <= 0 || group_size <= 0)
-    return host_fail(MP_ERR_INVALID_ARG, "mp_linear_w4_workspace: needs M >= 0, N > 0, K > 0, group_size > 0 and a result pointer");
+  if (bytes == nullptr || M < 0 || N <= 0 || K <= 0 || M > kMaxExtent || N > kMaxExtent || K > kMaxExtent || group_size <= 0)
+    return host_fail(MP_ERR_INVALID_ARG, "mp_linear_w4_workspace: needs M >= 0, N > 0, K > 0, none above 2^28, group_size > 0 and a result pointer");
   *bytes = M == 0 ? 0 : w4_plan(M, N, K, group_size, grad_input != 0, !tokens_aligned(X, ldx)).total;
   return MP_OK;
 }

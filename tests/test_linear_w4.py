@@ -79,6 +79,13 @@ def test_argument_checks(api):
             call()
 
 
+def test_extents_above_the_limit_are_refused(api):
+    L, p, z, n, big = api.lib(), ctypes.c_void_p(4096), ctypes.c_void_p(0), ctypes.c_size_t(), (1 << 28) + 32
+    assert L.mp_w4_pack(1, big, p, big, p, z) == 1 and L.mp_w4_pack(big, 1, p, 1, p, z) == 1
+    for m, rows, k in ((big, 8, 64), (8, big, 64), (8, 8, big)):
+        assert L.mp_linear_w4_workspace(m, rows, k, 32, p, k, 0, ctypes.byref(n)) == 1
+
+
 def test_extents_beyond_32_bits_are_refused(api):
     # 2^32 + 8 rows would reach the library as 8
     big = 2 ** 32 + 8

@@ -450,7 +450,6 @@ _W4_CODES = {torch.float16: MP_FP16, torch.bfloat16: MP_BF16}
 def _w4_checks(op: str, x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros, group_size: int, grad: bool, K: int):
     if x.dim() != 2 or qweight.dim() != 2:
         raise ValueError(f"{op}: input and packed weight must be 2-D tensors")
-    _fits_int(op, x.shape[0] | qweight.shape[0] | K)
     code = _W4_CODES.get(x.dtype)
     if code is None:
         raise ValueError(f"{op} serves fp16 and bf16")
@@ -465,8 +464,7 @@ def _w4_checks(op: str, x: torch.Tensor, qweight: torch.Tensor, scales: torch.Te
         group_size = max(32, 1 << (K - 1).bit_length())
     elif group_size < 32 or group_size & (group_size - 1):
         raise ValueError(f"{op}: group_size must be a power of two of at least 32, or -1")
-    else:
-        _fits_int(op, group_size)
+    _fits_int(op, x.shape[0] | N | K | group_size)
     shape = (N, (K + group_size - 1) // group_size)
     if scales.dtype != x.dtype or scales.shape != shape:
         raise ValueError(f"{op}: scales must be {list(shape)} in the input dtype")

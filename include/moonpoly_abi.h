@@ -194,6 +194,11 @@ int mp_debug_scratch_must_grow(size_t have_bytes, size_t have_counter_bytes, siz
 int mp_debug_stream_launch(int dtype, int m, int n, int k, int out[4]);
 int mp_debug_f32_tile_launch(int m, int n, int k, int out[3]);
 
+/* Test aid (host only): how mp_linear_w4 (grad_input = 0) or mp_linear_w4_grad_input (1) runs a problem whose tokens are aligned.
+ * out: 1 if on the streaming kernel (the rest is then 0), tokens per tile, units of work, slices of the contraction, steps of the
+ * contraction, steps per slice, pipeline stages, slots of the ring of packed weights. */
+int mp_debug_w4_launch(int M, int N, int K, int group_size, int grad_input, int out[8]);
+
 /* get_gemm_workspace_size_fp16_row_col_col (core/fp16/fp16_rcc.cu:3306-3316), extended to every
  * pid and dtype: bytes of scratch mp_gemm_rcc_pid needs for this problem (0 when split_k == 1). */
 int mp_workspace_size(int dtype, int pid, int m, int n, int k, int split_k, size_t* bytes);

@@ -23,11 +23,23 @@ constexpr int kSmsModel = 148;            // workspace sizes must not depend on 
 struct Plan {
   bool stream, with_table;
   int bn, tiles_m, tiles_n, steps, split, steps_per_split;
+  int stages, stage_bytes, raw_slots;
   size_t copy, partial, table, total;     // workspace: aligned copy of the tokens, partial sums, group words
   long long ld_copy, ld_partial;
 };
 
 bool tokens_aligned(const void* x, long long ld) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld % 8 == 0; }
+
+// Slots of the ring of packed weights: what three stages leave of the shared memory, but never three.  The two unpacking groups
+// take turns, and a wait tells a slot's fill from the one before it by the parity of the phase alone, so a group may wait for a
+// fill only where the one before it is known to have landed.  With an even number of slots that one was the group's own.  With
+// five, it was turn T - 5 of the other group: the group's last stage of turn T - 2 was free only after the product of the step
+// three before it, turns T - 4 ... T - 2 hold at least three steps, so turn T - 5 has been multiplied.  Three slots go wrong
+// where a turn of one step (the end of a unit with an odd number of steps) comes into it.
+int w4_raw_slots(int stages, int stage_bytes) {
+  const int room = std::min(kW4MaxRawSlots, (kPairSmem - 1024 - 256 - stages * stage_bytes) / kW4RawBytes);
+  return room == 3 ? 2 : room;
+}
 
 // rows = output features of this direction, contraction = input features.
 Plan w4_plan(int T, int N, int K, int group_size, bool grad, bool copy_tokens) {
@@ -59,6 +71,10 @@ Plan w4_plan(int T, int N, int K, int group_size, bool grad, bool copy_tokens) {
   p.tiles_n = ceil_div(T, p.bn);
   p.steps_per_split = ceil_div(p.steps, p.split);
   p.split = ceil_div(p.steps, p.steps_per_split);
+  // three stages, and the rest of the shared memory for packed bytes on their way from HBM
+  p.stages = 3;
+  p.stage_bytes = kW4ABytes + p.bn / 2 * 256;
+  p.raw_slots = w4_raw_slots(p.stages, p.stage_bytes);
   // The transposed group words cost a kernel of 3 us.  They pay where the weight is unpacked for several token tiles, and with
   // fine groups always (28672 x 4096, groups of 64, 17 tokens: 45 us against 58).
   p.with_table = p.tiles_n > 1 || group_size < 128;
@@ -166,14 +182,10 @@ int run_mma(const HostDevice& d, const Plan& l, const W4Weight& w, bool grad, in
   p.partial = reinterpret_cast<float*>(ws + l.partial);
   p.ld_partial = l.ld_partial;
   p.status = d.status;
-  const int hb = l.bn / 2;
-  p.stage_bytes = kW4ABytes + hb * 256;
-  // three stages, and the rest of the shared memory for packed bytes on their way from HBM
-  p.stages = 3;
-  p.raw_slots = std::min(kW4MaxRawSlots, (kPairSmem - 1024 - 256 - p.stages * p.stage_bytes) / kW4RawBytes);
+  p.stages = l.stages; p.stage_bytes = l.stage_bytes; p.raw_slots = l.raw_slots;
   OperandMaps tokens;
   CUtensorMap tmW;
-  if (int rc = operand_maps(&tokens, x, inner, T, ldx, hb, 2, &p.b_wide)) return rc;
+  if (int rc = operand_maps(&tokens, x, inner, T, ldx, l.bn / 2, 2, &p.b_wide)) return rc;
   if (l.with_table) {
     p.table = reinterpret_cast<const uint32_t*>(ws + l.table);
     p.ld_table = w.N;
@@ -263,6 +275,15 @@ int mp_linear_w4_workspace(int M, int N, int K, int group_size, const void* X, l
   if (bytes == nullptr || M < 0 || N <= 0 || K <= 0 || M > kMaxExtent || N > kMaxExtent || K > kMaxExtent || group_size <= 0)
     return host_fail(MP_ERR_INVALID_ARG, "mp_linear_w4_workspace: needs M >= 0, N > 0, K > 0, none above 2^28, group_size > 0 and a result pointer");
   *bytes = M == 0 ? 0 : w4_plan(M, N, K, group_size, grad_input != 0, !tokens_aligned(X, ldx)).total;
+  return MP_OK;
+}
+
+int mp_debug_w4_launch(int M, int N, int K, int group_size, int grad_input, int out[8]) {
+  if (out == nullptr || M < 1 || N < 1 || K < 1 || M > kMaxExtent || N > kMaxExtent || K > kMaxExtent || group_size < 32)
+    return host_fail(MP_ERR_INVALID_ARG, "mp_debug_w4_launch: positive sizes up to 2^28, group_size of at least 32");
+  const Plan l = w4_plan(M, N, K, group_size, grad_input != 0, false);
+  const int v[8] = {l.stream, l.bn, l.tiles_m * l.tiles_n * l.split, l.split, l.steps, l.steps_per_split, l.stages, l.raw_slots};
+  std::copy(v, v + 8, out);
   return MP_OK;
 }
 

@@ -8,6 +8,9 @@ of the step `stages` before it."""
 import ctypes
 
 import pytest
+import torch
+
+from test_linear_w4 import DTYPES, make, tokens, weight, within
 
 
 def turns_of(unit_steps):
@@ -74,3 +77,59 @@ def test_the_aid_refuses_bad_arguments(api):
     for args in ((0, 64, 64, 32, 0, out), (1, 0, 64, 32, 0, out), (1, 64, 0, 32, 0, out), (1, 64, 64, 16, 0, out),
                  ((1 << 28) + 1, 64, 64, 32, 0, out), (1, 64, 64, 32, 0, None)):
         assert aid(*args) != 0
+
+
+# ------------------------------------------------------------------------------------ many units per pair of CTAs (GPU)
+MANY = [  # tokens, N, K, group: even and odd steps of 128 along the contraction, tiles of 160 to 256 tokens and of fewer
+    (40, 20000, 256, 32), (40, 20000, 384, 64), (96, 20000, 128, 32), (120, 20000, 384, 128), (150, 19000, 640, 128), (150, 20000, 512, 32), (180, 28672, 3456, 128), (192, 20000, 128, 64),
+    (380, 9728, 896, 128), (512, 9728, 896, 32), (380, 9728, 1024, 64), (700, 9000, 416, 256), (1100, 9728, 128, 128), (2047, 4100, 1056, 64)]
+
+
+def zeros_to_63(q, s, z):
+    """Zero points over their whole range, and a scale that keeps the weights' size."""
+    gen = torch.Generator().manual_seed(7)
+    z = torch.randint(0, 64, z.shape, generator=gen, dtype=torch.uint8).to(z.device)
+    z.view(-1)[:2] = torch.tensor([0, 63], dtype=torch.uint8)
+    return q, s, z
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k,group", MANY)
+def test_pairs_with_several_units(api, m, n, k, group, dtype):
+    p = launch(api, m, n, k, group)
+    assert p["units"] > 74 and p["split"] == 1
+    q, s, z = zeros_to_63(*make(n, k, group, dtype, seed=m))
+    x, pw = tokens(m, k, dtype), api.pack_w4(q)
+    y = api.linear_w4(x, pw, s, z, group_size=group)
+    assert api.device_status() == 0
+    within(y, x, weight(q, s, z, group), None, True)
+    assert all(torch.equal(api.linear_w4(x, pw, s, z, group_size=group), y) for _ in range(3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k,group", [(40, 256, 20000, 32), (40, 300, 20000, 64), (192, 128, 20000, 32), (380, 896, 9728, 128),
+                                         (512, 1000, 9728, 64), (1537, 5760, 2880, 128), (1001, 4096, 5120, 256), (2047, 33, 4128, 32)])
+def test_pairs_with_several_units_of_the_gradient(api, m, n, k, group, dtype):
+    p = launch(api, m, n, k, group, 1)
+    assert p["units"] > 74 and p["split"] == 1
+    q, s, z = zeros_to_63(*make(n, k, group, dtype, seed=m))
+    dy, pw = tokens(m, n, dtype), api.pack_w4(q)
+    dx = api.linear_w4_grad_input(dy, pw, s, z, group_size=group, in_features=k)
+    assert api.device_status() == 0
+    within(dx, dy, weight(q, s, z, group).t(), None, True)
+    assert all(torch.equal(api.linear_w4_grad_input(dy, pw, s, z, group_size=group, in_features=k), dx) for _ in range(3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [1, 7, 16, 17, 100])
+def test_zero_points_over_their_whole_range(api, m, dtype):
+    for group in (32, 128):
+        q, s, z = zeros_to_63(*make(150, 672, group, dtype, seed=m))
+        x = tokens(m, 672, dtype)
+        within(api.linear_w4(x, api.pack_w4(q), s, z, group_size=group), x, weight(q, s, z, group), None, m > 16)
+        dy = tokens(m, 150, dtype)
+        dx = api.linear_w4_grad_input(dy, api.pack_w4(q), s, z, group_size=group, in_features=672)
+        within(dx, dy, weight(q, s, z, group).t(), None, True)

@@ -352,9 +352,8 @@ __device__ __forceinline__ void pair_epilogue_lse(const PairParams& p, const Pai
 #pragma unroll
     for (int j = 0; j < 128; ++j) if (j < ncols) s0 += exp2_approx((z[j] - base) * kLog2e);
   }
-  // a half without columns keeps (-inf, 0); an infinite maximum is stored as its base
-  const float mm = m == -INFINITY ? m : base;
-  if (live) p.partial[(size_t)(2 * tn + half) * q.rows + row] = make_float2(mm, s0 + s1);
+  // a half without columns keeps (-inf, 0)
+  if (live) p.partial[(size_t)(2 * tn + half) * q.rows + row] = make_float2(m, s0 + s1);
 }
 
 // The largest finite |grad_loss| of the rows that have a loss (1 if there is none), by the eight epilogue warps while the

@@ -23,6 +23,10 @@ using namespace mp;
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // ---------------------------------------------------------------------------------------------------- small kernels
+// What a sum of exp(z - m) is to be multiplied by where the row's maximum is `top`.  Equal maxima, two infinite ones among them, keep
+// their sums as they are; an infinite one makes the others vanish, but lets NaN through.
+__device__ __forceinline__ float rescale(float m, float top) { return m == top ? 1.0f : exp2_approx((m - top) * kLog2e); }
+
 // loss and logsumexp of every row from the partial (max, sum) pairs; 32 rows x 32 groups of partials per block.
 __global__ void __launch_bounds__(1024) xent_join_kernel(const float2* partial, int num, int rows, const float* target_logit,
                                                          const void* target, int target64, long long ignore_index, int vocab,
@@ -37,12 +41,8 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const float2* partial, 
     for (int i = g; i < num; i += 32) {
       const float2 v = partial[(size_t)i * rows + row];
       const float mn = fmaxf(m, v.x);
-      if (mn != -INFINITY) {                       // two empty pieces would give exp(-inf + inf)
-        s = s * exp2_approx((m - mn) * kLog2e) + v.y * exp2_approx((v.x - mn) * kLog2e);
-        m = mn;
-      } else {
-        s += v.y;                                  // 0, or NaN from a row of NaN
-      }
+      s = s * rescale(m, mn) + v.y * rescale(v.x, mn);
+      m = mn;
     }
   }
   sm[g][rx] = m;
@@ -51,9 +51,9 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const float2* partial, 
   if (g != 0 || row >= rows) return;
   float top = -INFINITY;
   for (int i = 0; i < 32; ++i) top = fmaxf(top, sm[i][rx]);
-  const float base = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f;
-  for (int i = 0; i < 32; ++i) sum += ss[i][rx] * exp2_approx((sm[i][rx] - base) * kLog2e);
+  for (int i = 0; i < 32; ++i) sum += ss[i][rx] * rescale(sm[i][rx], top);
+  const float base = isinf(top) ? 0.0f : top;      // the sum is then infinite, zero or NaN itself
   const float logsum = logf(sum);
   lse[row] = base + logsum;
   const long long t = target64 ? reinterpret_cast<const long long*>(target)[row] : reinterpret_cast<const int*>(target)[row];

@@ -51,10 +51,16 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const float2* partial, 
   if (g != 0 || row >= rows) return;
   float top = -INFINITY;
   for (int i = 0; i < 32; ++i) top = fmaxf(top, sm[i][rx]);
-  float sum = 0.0f;
-  for (int i = 0; i < 32; ++i) sum += ss[i][rx] * rescale(sm[i][rx], top);
+  float sum[32];                                   // added in pairs, like the terms of a piece
+#pragma unroll
+  for (int i = 0; i < 32; ++i) sum[i] = ss[i][rx] * rescale(sm[i][rx], top);
+#pragma unroll
+  for (int w = 16; w; w >>= 1) {
+#pragma unroll
+    for (int i = 0; i < w; ++i) sum[i] += sum[i + w];
+  }
   const float base = isinf(top) ? 0.0f : top;      // the sum is then infinite, zero or NaN itself
-  const float logsum = logf(sum);
+  const float logsum = logf(sum[0]);
   lse[row] = base + logsum;
   const long long t = target64 ? reinterpret_cast<const long long*>(target)[row] : reinterpret_cast<const int*>(target)[row];
   if (t == ignore_index) loss[row] = 0.0f;

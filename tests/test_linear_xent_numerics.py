@@ -1,4 +1,9 @@
-"""Linear with softmax cross entropy where its arithmetic is strained: infinite logits beside large finite ones."""
+"""Linear with softmax cross entropy where its arithmetic is strained: infinite logits beside large finite ones, rows whose
+target is nearly certain, long contractions.
+
+The tensor cores drop what an addition shifts out, towards zero.  One addition takes 16 products; it loses half a unit of the
+running sum on average, a unit being 2^-24 to 2^-23 of it.  A sum that grows evenly over n additions thus ends short by
+n / 2 * 2^-24 of itself at most (the running sum is half the final one on average)."""
 import pytest
 import torch
 
@@ -30,3 +35,36 @@ def test_infinite_logits_beside_large_ones(api, v, dtype):
             w[large], w[at] = NAN, INF
             assert torch.isnan(api.linear_cross_entropy(x, w, target)[1]).all()
     assert api.device_status() == 0
+
+
+def confident(m, v, h, dtype, level, gap):
+    """Rows of h elements whose target's logit is near `level` and the others' `gap` below, the same way for every row."""
+    gen = torch.Generator().manual_seed(3)
+    half = h // 2
+    b = torch.randn((m, half), generator=gen)
+    x = torch.cat([torch.ones(m, half), b], 1)                             # the first half carries what the logits share
+    w = torch.randn((v, h), generator=gen) * 0.5 / half ** 0.5
+    w[:, :half] = w[:, :half] * 0.1 + (level - gap) / half
+    target = torch.randperm(v, generator=gen)[:m]
+    w[target, half:] = gap * b / (b * b).sum(1, keepdim=True)
+    return x.to(dtype).cuda(), w.to(dtype).cuda(), target.cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [2000, 70000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_loss_of_confident_rows(api, v, dtype):
+    # The loss is log(1 + r) with an r of many terms, each below half a unit of the 1: added to it one by one they all vanish.
+    # Added in pairs, a sum of 128 terms passes 7 additions, that of the pieces one for every 32 of them and 5 more; each is off by
+    # half a unit of a number between 1 and 2, 2^-24.  r itself moves by exp (2^-21 with the rounding of its argument) and by the
+    # truncation of the gap between the logits.
+    level, gap = 22.0, 17.3
+    x, w, target = confident(90, v, 2048, dtype, level, gap)
+    loss, _ = api.linear_cross_entropy(x, w, target)
+    e = exact(x, w, target, torch.ones(90, device="cuda"))
+    r = e["loss"].expm1()
+    assert (r / v > 2.0 ** -27).all() and (r / v < 2.0 ** -23).all()
+    off = (loss.double() - e["loss"]).abs()
+    tol = (12 + v // 4096) * 2.0 ** -24 + r * (2.0 ** -21 + 64 * 2.0 ** -23 * 2 * level)
+    print(float((off / tol).max()), float(off.max()), float((loss.double() - e["loss"]).mean()), float(r.mean()))
+    assert (off <= tol).all(), (off, tol)

@@ -314,16 +314,31 @@ struct PairUnits {
 };
 
 // ------------------------------------------------------------------------------------------------------ the epilogues
-// Softmax statistics of this warp's half (128 columns) of a 256-column tile, one row per lane.  The tensor cores drop the
-// bits that an addition shifts out, always towards zero, so a long contraction pulls every logit to zero (H = 4096:
-// 2e-5, which the mean over a vocabulary does not average away).  The contraction therefore comes in chunks of
-// kLseChunk blocks, each in an accumulator of its own, and the chunks are added here, rounded to nearest: 1.6e-6 ->
-// 0.6e-6 relative error of the loss at H = 4096, while the other accumulator is being filled.
+// The tensor cores drop the bits that an addition shifts out, always towards zero, so a long contraction pulls every logit to
+// zero (H = 4096: 2e-5, which the mean over a vocabulary does not average away).  The contraction therefore comes in chunks of
+// kPairChunk blocks, each in an accumulator of its own, and the chunks are added here, rounded to nearest, while the other
+// accumulator is being filled.  The forward pass and the gradients' logits take the same chunks and get the same bits: at the
+// target d is exp(z - lse) - 1, and of a nearly certain row nothing else is left.
+constexpr int kPairChunk = 16;               // blocks of 64 contraction elements per accumulator
+
+// z += this warp's half (128 columns) of the accumulator, one row per lane; t_addr: its first column.
+__device__ __forceinline__ void pair_add_chunk(float (&z)[128], uint32_t t_addr) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t v[32];
+    __syncwarp();
+    tmem_ld_x32(t_addr + 32u * c, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) z[32 * c + j] += __uint_as_float(v[j]);
+  }
+}
+
+// Softmax statistics of this warp's half of a 256-column tile, one row per lane.
 // The maximum is taken first and z - max is formed before the multiplication by log2(e), so that the sum is exact to a
 // few units in the last place whatever the logits' size.  An infinite maximum is replaced by 0 (exp then gives 0 or
 // infinity as the definition does); NaN passes through the sum.  The 128 terms are added in pairs: beside a nearly certain entry's 1,
 // terms below 2^-24 would vanish one by one (2000 entries of 4e-8: the loss is off by 2e-7 instead of 1.7e-6).
-constexpr int kLseChunk = 16;                // blocks of 64 contraction elements per accumulator
 __device__ __forceinline__ void pair_epilogue_lse(const PairParams& p, const PairProblem& q, float (&z)[128], int row, int c_begin,
                                                   int tn, int half, int ncols) {
   const bool live = row < q.rows;
@@ -377,8 +392,8 @@ __device__ __forceinline__ float pair_grad_max(const PairParams& p, int rows, fl
 // d = grad_loss[row] * (softmax - onehot), rounded once to the operand type and parked for the two gradient products.  The
 // largest |grad_loss| is divided out (a mean over the tokens then rounds exactly: the factors are 1) and, for fp16, replaced
 // by 2^15: a probability of 2e-9 is still a normal fp16 number beside a one.  The products are multiplied by *scale_out.
-__device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
-                                                      int ncols, int half_cols, float grad_max, uint32_t stage) {
+__device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const PairProblem& q, const float (&z)[128], int row, int c_begin,
+                                                      int ncols, float grad_max, uint32_t stage) {
   const bool live = row < q.rows;
   long long target = -1;
   float lse = 0.0f, coef = 0.0f;
@@ -392,22 +407,19 @@ __device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const
   }
   const int lane = row & 31, row0 = row - lane;
   uint16_t* o = p.dlogits + (long long)row0 * p.ld_dl + c_begin;
-  for (int c0 = 0; c0 < half_cols; c0 += 64) {
+#pragma unroll
+  for (int c0 = 0; c0 < 128; c0 += 64) {
     uint32_t w[32];
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
       const int c1 = c0 + 32 * part;
-      uint32_t v[32];
-      __syncwarp();
-      tmem_ld_x32(t_addr + (uint32_t)c1, v);
-      tmem_ld_wait();
       float d[32];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) d[j] = kept ? coef * exp2_approx((__uint_as_float(v[j]) - lse) * kLog2e) : 0.0f;
+      for (int j = 0; j < 32; ++j) d[j] = kept ? coef * exp2_approx((z[c1 + j] - lse) * kLog2e) : 0.0f;
       if (kept && target >= c1 && target < c1 + 32) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (target == c1 + j) d[j] = coef * (exp2_approx((__uint_as_float(v[j]) - lse) * kLog2e) - 1.0f);
+          if (target == c1 + j) d[j] = coef * (exp2_approx((z[c1 + j] - lse) * kLog2e) - 1.0f);
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) w[16 * part + j] = pack16(d[2 * j], d[2 * j + 1], p.bf16);
@@ -499,7 +511,7 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
   griddep_wait();
 
   if (warp < 4) {
-    if constexpr (EPI == PAIR_LSE) regs_fewer_88();      // its epilogue holds 128 sums per thread
+    if constexpr (EPI != PAIR_STORE) regs_fewer_88();    // the epilogue holds 128 sums per thread
     // ------------------------------------------------------------------------------------------ TMA producer (one lane)
     if (warp == 0 && lane == 0) {
       int s = 0;
@@ -561,8 +573,8 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         const uint32_t a_step = q.a_mn ? 2048u >> 4 : 2u, b_step = q.b_mn ? 2048u >> 4 : 2u;
         const uint32_t a_blk = q.a_mn ? 8192u >> 4 : (uint32_t)q.a_rows * 128u >> 4, b_blk = q.b_mn ? 8192u >> 4 : (uint32_t)(q.bn >> 1) * 128u >> 4;
         const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4;
-        // an accumulator takes the whole contraction, or a chunk of it (PAIR_LSE)
-        const int chunk = EPI == PAIR_LSE ? kLseChunk : q.kblocks;
+        // an accumulator takes the whole contraction, or a chunk of it
+        const int chunk = EPI == PAIR_STORE ? q.kblocks : kPairChunk;
         for (int k0 = u.kb0; ok && k0 < u.kb1; k0 += chunk, ++ui) {
           const uint32_t buf = ui & 1u, use = ui >> 1;
           if (!wait_all(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
@@ -597,7 +609,7 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
     }
   } else {
     // -------------------------------------------------------------------------------------------------- epilogue warps
-    if constexpr (EPI == PAIR_LSE) regs_more_208();
+    if constexpr (EPI != PAIR_STORE) regs_more_208();
     const int quad = warp & 3, half = (warp - 4) >> 2;
     uint32_t ui = 0;
     bool ok = true;
@@ -627,35 +639,28 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
       const int c_begin = u.tn * q.bn + half * half_cols;                // first column of this warp's half
       const int ncols = min(half_cols, q.cols - c_begin);                // may be <= 0 in the last column tile
       const uint32_t t_half = tmem_base + (uint32_t)(half * half_cols) + ((uint32_t)(quad * 32) << 16);
-      if constexpr (EPI == PAIR_LSE) {
+      if constexpr (EPI != PAIR_STORE) {
         float z[128];
 #pragma unroll
         for (int j = 0; j < 128; ++j) z[j] = 0.0f;
-        for (int k0 = 0; ok && k0 < q.kblocks; k0 += kLseChunk, ++ui) {
+        for (int k0 = 0; ok && k0 < q.kblocks; k0 += kPairChunk, ++ui) {
           const uint32_t buf = ui & 1u, use = ui >> 1;
           if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
           tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            __syncwarp();
-            tmem_ld_x32(t_half + buf * (uint32_t)kPairMaxBN + 32u * c, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) z[32 * c + j] += __uint_as_float(v[j]);
-          }
+          pair_add_chunk(z, t_half + buf * (uint32_t)kPairMaxBN);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));
         }
-        if (ok) pair_epilogue_lse(p, q, z, row, c_begin, u.tn, half, ncols);
+        if (!ok) break;
+        if constexpr (EPI == PAIR_LSE) pair_epilogue_lse(p, q, z, row, c_begin, u.tn, half, ncols);
+        else pair_epilogue_dlogits(p, q, z, row, c_begin, ncols, grad_max, stage);
       } else {
         const uint32_t buf = ui & 1u, use = ui >> 1;
         if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
         tc_fence_after();
         const uint32_t t_addr = t_half + buf * (uint32_t)kPairMaxBN;
-        if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, t_addr, row, c_begin, ncols, half_cols, grad_max, stage);
-        else pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols, u.slice, scale, stage);
+        pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols, u.slice, scale, stage);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));

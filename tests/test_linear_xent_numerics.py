@@ -68,3 +68,31 @@ def test_loss_of_confident_rows(api, v, dtype):
     tol = (12 + v // 4096) * 2.0 ** -24 + r * (2.0 ** -21 + 64 * 2.0 ** -23 * 2 * level)
     print(float((off / tol).max()), float(off.max()), float((loss.double() - e["loss"]).mean()), float(r.mean()))
     assert (off <= tol).all(), (off, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("level", [22.0, -22.0])
+@pytest.mark.parametrize("h", [4096, 8192])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_of_confident_rows(api, h, level, dtype):
+    # d at the target is -(1 - p), the difference of two numbers near one: the logits of the gradient have to be those that lse was
+    # summed from.  lse in fp32 is off by 2^-24 of itself, its sum of exponentials by 12 additions of 2^-24 (test_loss_of_confident_rows),
+    # exp by 2^-22: 2^-24 |lse| + 2^-20 in all, measured against 1 - p.  d and the result are rounded to 16 bits, u each.  The
+    # others' probabilities move by the truncation of the gap between the logits.
+    x, w, target = confident(60, 2000, h, dtype, level, 18.0)
+    g = torch.full((60,), 1024.0, device="cuda")
+    _, lse = api.linear_cross_entropy(x, w, target)
+    dx, dw = api.linear_cross_entropy_grad(x, w, target, lse, g)
+    e = exact(x, w, target, g)
+    rest = -e["d"].gather(1, target[:, None]).squeeze(1) / g               # 1 - p
+    assert (rest > 1e-5).all() and (rest < 1e-3).all()
+    u = torch.finfo(dtype).eps / 2
+    off = (dx.double() - e["dx"]).norm(dim=1) / e["dx"].norm(dim=1)
+    # w at the target is the longest of what the row sums up: an error of d there counts by |w_t| / |w_t - mean of the others|
+    lever = w[target].double().norm(dim=1) * rest * g / e["dx"].norm(dim=1)
+    tol = 2 * u + lever * (2.0 ** -24 * e["lse"].abs() + 2.0 ** -20) / rest + 64 * 2.0 ** -23 * 2 * abs(level)
+    print(float(off.max()), float((off / tol).max()), float(rest.max()), float(lever.max()))
+    assert (off <= tol).all(), (off, tol)
+    # the same through dw: row t of it is d_t x
+    off = (dw.double() - e["dw"])[target].norm(dim=1) / e["dw"][target].norm(dim=1)
+    assert (off <= 2 * u + (2.0 ** -24 * e["lse"].abs() + 2.0 ** -20) / rest + 64 * 2.0 ** -23 * 2 * abs(level)).all(), off

@@ -26,13 +26,14 @@ namespace mp {
 
 constexpr int kPairRows = 256;               // rows of D per tile
 constexpr int kPairMaxBN = 256;
-constexpr int kPairThreads = 384;             // warp 2 of PAIR_STORE posts units; it and warp 3 fill the first warpgroup up
+constexpr int kPairThreads = 384;             // warp 2 of PAIR_STORE(_LONG) posts units; it and warp 3 fill the first warpgroup up
 constexpr int kPairMaxStages = 8;
 constexpr int kPairSmem = 232448;            // 227 KB opt-in limit per CTA
 constexpr int kPairBarBytes = 512;           // behind the stages: barriers, unit box, TMEM address, 8 floats
 constexpr int kPairBox = 8, kPairAhead = 2;  // slots of the unit box, and units that it holds ahead of the slowest of its readers
 
-enum { PAIR_STORE = 0, PAIR_LSE = 1, PAIR_DLOGITS = 2 };
+// PAIR_STORE_LONG: PAIR_STORE for contractions of more than kPairStoreChunk blocks, which no single accumulator sums.
+enum { PAIR_STORE = 0, PAIR_LSE = 1, PAIR_DLOGITS = 2, PAIR_STORE_LONG = 3 };
 
 // One GEMM of a launch.  A launch may hold two (they share the persistent grid, so the partly empty last wave of one is
 // filled by the other).
@@ -45,8 +46,8 @@ struct PairProblem {
   int a_wide, b_wide;            // whole blocks of 64 along the operand's lines (see OperandMaps)
   int group_m;                   // raster: tiles are walked in groups of `group_m` row tiles
   int tile0;                     // index of the problem's first unit in the launch
-  int split, kb_per_split;       // PAIR_STORE: the contraction in `split` slices of kb_per_split blocks, a unit each
-  // PAIR_STORE: out16 = scale * (acc (+ acc32)), or acc32[slice] (+)= acc when out16 is null
+  int split, kb_per_split;       // PAIR_STORE(_LONG): the contraction in `split` slices of kb_per_split blocks, a unit each
+  // PAIR_STORE(_LONG): out16 = scale * (acc (+ acc32)), or acc32[slice] (+)= acc when out16 is null
   void* out16;
   float* acc32;
   long long ld_out;              // row stride of out16 in elements
@@ -58,11 +59,11 @@ struct PairParams {
   int num_problems;
   PairProblem prob[2];
   int total_tiles;               // units of the launch
-  unsigned* next_unit;           // counter that hands out the units of PAIR_STORE; PAIR_DLOGITS, which goes before, clears it
+  unsigned* next_unit;           // counter that hands out the units of PAIR_STORE(_LONG); PAIR_DLOGITS, which goes before, clears it
   int stages, stage_bytes;
   int kc;                        // 64-element blocks of the contraction per stage (1 or 2)
   int bf16;                      // operand and output type: 1 = bf16, 0 = fp16
-  const float* scale;            // PAIR_STORE: device scalar
+  const float* scale;            // PAIR_STORE(_LONG): device scalar
   int* status;
   // PAIR_LSE / PAIR_DLOGITS (the columns of D are vocabulary entries col0 ... col0 + cols - 1)
   const void* target; int target64;
@@ -320,6 +321,15 @@ struct PairUnits {
 // accumulator is being filled.  The forward pass and the gradients' logits take the same chunks and get the same bits: at the
 // target d is exp(z - lse) - 1, and of a nearly certain row nothing else is left.
 constexpr int kPairChunk = 16;               // blocks of 64 contraction elements per accumulator
+// The gradients, rounded to 16 bits in the end, take longer chunks: 512 additions leave a sum short by 2^-16 of itself at most, 1/32 of
+// fp16's half step; the 8192 of 131072 vocabulary entries left 1.3e-4.  The chunks of PAIR_STORE_LONG are summed in registers, and
+// tiles with little to multiply then leave more slowly: loss and both gradients of 128 x 32768 x 4096 take 284 us with it and 271
+// with PAIR_STORE, whose slices of one chunk are written in 32 bits and joined.  At 2048 x 32768 x 1024 it costs 1 %.
+constexpr int kPairStoreChunk = 128;
+template <int EPI> struct PairEpi {
+  static constexpr bool kStores = EPI == PAIR_STORE || EPI == PAIR_STORE_LONG, kSums = EPI != PAIR_STORE;
+  static constexpr int kChunk = kStores ? kPairStoreChunk : kPairChunk;      // PAIR_STORE never has more than one
+};
 
 // z += this warp's half (128 columns) of the accumulator, one row per lane; t_addr: its first column.
 __device__ __forceinline__ void pair_add_chunk(float (&z)[128], uint32_t t_addr) {
@@ -428,22 +438,31 @@ __device__ __forceinline__ void pair_epilogue_dlogits(const PairParams& p, const
   }
 }
 
-__device__ __forceinline__ void pair_epilogue_store(const PairParams& p, const PairProblem& q, uint32_t t_addr, int row, int c_begin,
-                                                    int ncols, int half_cols, int slice, float scale, uint32_t stage) {
+// z: the unit's sums where it has several chunks (SUMS); the only chunk is read from t_addr.
+template <bool SUMS>
+__device__ __forceinline__ void pair_epilogue_store(const PairParams& p, const PairProblem& q, uint32_t t_addr, const float (&z)[128], int row,
+                                                    int c_begin, int ncols, int slice, float scale, uint32_t stage) {
   const bool live = row < q.rows;
   const int lane = row & 31, row0 = row - lane;
-  for (int c0 = 0; c0 < half_cols; c0 += 64) {
+  constexpr int kUnroll = SUMS ? 2 : 1;                    // z is indexed
+#pragma unroll kUnroll
+  for (int c0 = 0; c0 < 128; c0 += 64) {
     uint32_t w[32];
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
       const int c1 = c0 + 32 * part;
-      uint32_t r[32];
-      __syncwarp();
-      tmem_ld_x32(t_addr + (uint32_t)c1, r);
-      tmem_ld_wait();
       float v[32];
+      if constexpr (SUMS) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        for (int j = 0; j < 32; ++j) v[j] = z[c1 + j];
+      } else {
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld_x32(t_addr + (uint32_t)c1, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+      }
       float* a = q.acc32 + (long long)slice * q.acc_slice + (long long)row * q.ld_acc + c_begin + c1;
       const bool mine = live && c1 < ncols;                // ld_acc is a multiple of 32: rows of the scratch are padded
       if (q.add_acc32 && mine) {
@@ -482,7 +501,8 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
   auto tempty_bar = [&](int b) { return bar_base + 8u * (uint32_t)(2 * stages + 2 + b); };
   const uint32_t unit_bars = bar_base + 8u * (uint32_t)(2 * stages + 4), unit_box = unit_bars + 16u * kPairBox;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 20 * kPairBox);
-  constexpr bool DYNAMIC = EPI == PAIR_STORE;
+  constexpr bool DYNAMIC = PairEpi<EPI>::kStores, SUMS = PairEpi<EPI>::kSums;
+  constexpr int kChunk = PairEpi<EPI>::kChunk;
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -511,7 +531,7 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
   griddep_wait();
 
   if (warp < 4) {
-    if constexpr (EPI != PAIR_STORE) regs_fewer_88();    // the epilogue holds 128 sums per thread
+    if constexpr (SUMS) regs_fewer_88();                 // the epilogue holds 128 sums per thread
     // ------------------------------------------------------------------------------------------ TMA producer (one lane)
     if (warp == 0 && lane == 0) {
       int s = 0;
@@ -573,14 +593,12 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         const uint32_t a_step = q.a_mn ? 2048u >> 4 : 2u, b_step = q.b_mn ? 2048u >> 4 : 2u;
         const uint32_t a_blk = q.a_mn ? 8192u >> 4 : (uint32_t)q.a_rows * 128u >> 4, b_blk = q.b_mn ? 8192u >> 4 : (uint32_t)(q.bn >> 1) * 128u >> 4;
         const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4;
-        // an accumulator takes the whole contraction, or a chunk of it
-        const int chunk = EPI == PAIR_STORE ? q.kblocks : kPairChunk;
-        for (int k0 = u.kb0; ok && k0 < u.kb1; k0 += chunk, ++ui) {
+        for (int k0 = u.kb0; ok && k0 < u.kb1; k0 += kChunk, ++ui) {       // a chunk of the contraction per accumulator
           const uint32_t buf = ui & 1u, use = ui >> 1;
           if (!wait_all(tempty_bar((int)buf), (use & 1u) ^ 1u, status, MP_DEV_TIMEOUT_MMA_TMEM)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + buf * (uint32_t)kPairMaxBN;
-          const int k1 = min(u.kb1, k0 + chunk);
+          const int k1 = min(u.kb1, k0 + kChunk);
           uint32_t more = 0u;
           for (int kb = k0; kb < k1; kb += p.kc) {
             if (!wait_all(full_bar(s), ph, status, MP_DEV_TIMEOUT_MMA_FULL)) { ok = false; break; }
@@ -609,13 +627,13 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
     }
   } else {
     // -------------------------------------------------------------------------------------------------- epilogue warps
-    if constexpr (EPI != PAIR_STORE) regs_more_208();
+    if constexpr (SUMS) regs_more_208();
     const int quad = warp & 3, half = (warp - 4) >> 2;
     uint32_t ui = 0;
     bool ok = true;
     float grad_max = 1.0f;
     const uint32_t stage = bar_base + kPairBarBytes + (uint32_t)(warp - 4) * 4096u;       // of this warp, where outputs are 16 bits (kPairStoreBytes)
-    const float scale = EPI == PAIR_STORE ? *p.scale : 1.0f;
+    const float scale = DYNAMIC ? *p.scale : 1.0f;
     if constexpr (EPI == PAIR_DLOGITS) {
       grad_max = pair_grad_max(p, p.prob[0].rows, reinterpret_cast<float*>(smem + (size_t)stages * p.stage_bytes + 8 * (2 * stages + 4) + 20 * kPairBox + 8));
       if (blockIdx.x == 0 && threadIdx.x == 128) {
@@ -639,11 +657,11 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
       const int c_begin = u.tn * q.bn + half * half_cols;                // first column of this warp's half
       const int ncols = min(half_cols, q.cols - c_begin);                // may be <= 0 in the last column tile
       const uint32_t t_half = tmem_base + (uint32_t)(half * half_cols) + ((uint32_t)(quad * 32) << 16);
-      if constexpr (EPI != PAIR_STORE) {
-        float z[128];
+      float z[128];
+      if constexpr (SUMS) {
 #pragma unroll
         for (int j = 0; j < 128; ++j) z[j] = 0.0f;
-        for (int k0 = 0; ok && k0 < q.kblocks; k0 += kPairChunk, ++ui) {
+        for (int k0 = u.kb0; ok && k0 < u.kb1; k0 += kChunk, ++ui) {
           const uint32_t buf = ui & 1u, use = ui >> 1;
           if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
           tc_fence_after();
@@ -654,13 +672,13 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         }
         if (!ok) break;
         if constexpr (EPI == PAIR_LSE) pair_epilogue_lse(p, q, z, row, c_begin, u.tn, half, ncols);
-        else pair_epilogue_dlogits(p, q, z, row, c_begin, ncols, grad_max, stage);
+        else if constexpr (EPI == PAIR_DLOGITS) pair_epilogue_dlogits(p, q, z, row, c_begin, ncols, grad_max, stage);
+        else pair_epilogue_store<true>(p, q, 0u, z, row, c_begin, ncols, u.slice, scale, stage);
       } else {
         const uint32_t buf = ui & 1u, use = ui >> 1;
         if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
         tc_fence_after();
-        const uint32_t t_addr = t_half + buf * (uint32_t)kPairMaxBN;
-        pair_epilogue_store(p, q, t_addr, row, c_begin, ncols, half_cols, u.slice, scale, stage);
+        pair_epilogue_store<false>(p, q, t_half + buf * (uint32_t)kPairMaxBN, z, row, c_begin, ncols, u.slice, scale, stage);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar((int)buf), 0));

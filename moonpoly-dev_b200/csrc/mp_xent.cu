@@ -125,17 +125,19 @@ constexpr int kPairsModel = 74;          // workspace sizes must not depend on t
 // Slices of the vocabulary in the product dX = d W of one piece.  It has few, long tiles (M / 256 x H / 256, cols / 64 blocks
 // each), so whole tiles leave SMs idle: 300 x 2040 are 16 tiles for 74 pairs.  The slices' sums are joined by a kernel of
 // its own; its traffic, in units of a block's time (a third of a microsecond), is weighed against the shorter critical path.
-// dW's many short tiles fill the gaps where there is a dW.
+// dW's many short tiles fill the gaps where there is a dW.  With few rows those are bound by their epilogue, which PAIR_STORE_LONG
+// slows down, so no slice is then longer than an accumulator may sum.
 int dx_split(int M, int H, int cols, bool with_dw) {
   const int tiles = ceil_div(M, kPairRows) * ceil_div(H, kPairMaxBN), blocks = ceil_div(cols, 64);
   const double even = (with_dw ? 2.0 : 1.0) * tiles * blocks / kPairsModel;          // dW is as much work as dX
   const long long slice_bytes = (long long)M * (long long)round_up((size_t)H, 32) * 4;
+  const int fewest = with_dw && M <= kPairRows ? ceil_div(blocks, kPairStoreChunk) : 1, first = fewest * slice_bytes <= (512ll << 20) ? fewest : 1;
   double best = 0.0;
   int split = 1;
-  for (int s = 1; s <= 16 && (s == 1 || s * slice_bytes <= (512ll << 20)) && blocks / s >= 16; ++s) {
+  for (int s = first; s == first || (s <= 16 && s * slice_bytes <= (512ll << 20) && blocks / s >= 16); ++s) {
     const double longest = (double)ceil_div(tiles * s, kPairsModel) * (ceil_div(blocks, s) + 8);
     const double cost = std::max(longest, even) + (s > 1 ? 10.0 + 2.0 * s * slice_bytes / 1.7e6 : 0.0);
-    if (s == 1 || cost < 0.97 * best) { best = cost; split = s; }
+    if (s == first || cost < 0.97 * best) { best = cost; split = s; }
   }
   return split;
 }
@@ -364,7 +366,9 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       ++n;
     }
     p.num_problems = n;
-    if (int rc = launch_pair<PAIR_STORE>(d, p, maps, stream)) return rc;
+    bool chunks = false;
+    for (int j = 0; j < n; ++j) chunks |= p.prob[j].kb_per_split > kPairStoreChunk;
+    if (int rc = chunks ? launch_pair<PAIR_STORE_LONG>(d, p, maps, stream) : launch_pair<PAIR_STORE>(d, p, maps, stream)) return rc;
   }
   if (slices > 0) {
     const long long threads = (long long)M * (l.ld_acc / 4);

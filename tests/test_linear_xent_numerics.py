@@ -96,3 +96,23 @@ def test_gradient_of_confident_rows(api, h, level, dtype):
     # the same through dw: row t of it is d_t x
     off = (dw.double() - e["dw"])[target].norm(dim=1) / e["dw"][target].norm(dim=1)
     assert (off <= 2 * u + (2.0 ** -24 * e["lse"].abs() + 2.0 ** -20) / rest + 64 * 2.0 ** -23 * 2 * abs(level)).all(), off
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,v,h", [(1024, 131072, 4096), (131072, 1024, 256)])
+def test_long_sums_of_the_gradients_are_not_short(api, m, v, h):
+    # dx is summed over the vocabulary, dw over the rows: 8192 additions of 16 products each.  In one accumulator such a sum ends short
+    # by up to 8192 / 2 * 2^-24 = 2.4e-4 (what it loses comes to 0.5 to 1 of that, as the unit is 2^-24 to 2^-23 of the sum).  In
+    # chunks of 512 additions it is 512 / 2 * 2^-24.  Measured along the exact gradient, where the roundings of d and of the result do
+    # not add up: d at the m targets, u / sqrt(3) each, leaves u / sqrt(3 m); the logits' own shortness, of chunks of 64 additions,
+    # moves p by 64 / 2 * 2^-24 (z - mean z), |z - mean z| < 20 here.
+    x, w, target, g = inputs(m, v, h, torch.float16, seed=2, skip=0.0)
+    g = torch.ones_like(g)
+    _, lse = api.linear_cross_entropy(x, w, target)
+    grads = api.linear_cross_entropy_grad(x, w, target, lse, g)
+    e = exact(x, w, target, g)
+    tol = 256 * 2.0 ** -24 + 20 * 32 * 2.0 ** -24 + 4 * 2.0 ** -11 / (3 * m) ** 0.5
+    for name, got in zip(("dx", "dw"), grads):
+        short = float((got.double() * e[name]).sum() / (e[name] ** 2).sum()) - 1.0
+        print(name, short, tol)
+        assert abs(short) <= tol, (name, short, tol)

@@ -316,10 +316,11 @@ struct PairUnits {
 
 // ------------------------------------------------------------------------------------------------------ the epilogues
 // The tensor cores drop the bits that an addition shifts out, always towards zero, so a long contraction pulls every logit to
-// zero (H = 4096: 2e-5, which the mean over a vocabulary does not average away).  The contraction therefore comes in chunks of
-// kPairChunk blocks, each in an accumulator of its own, and the chunks are added here, rounded to nearest, while the other
-// accumulator is being filled.  The forward pass and the gradients' logits take the same chunks and get the same bits: at the
-// target d is exp(z - lse) - 1, and of a nearly certain row nothing else is left.
+// zero, which the mean over a vocabulary does not average away.  The contraction therefore comes in chunks of kPairChunk
+// blocks, each in an accumulator of its own, and the chunks are added here, rounded to nearest, while the other accumulator is
+// being filled: at H = 4096 and logits of deviation 2, lse (11 in size) is off by 4e-6 on average instead of 1.7e-5, at H = 16384 by
+// 4e-6 instead of 6.8e-5.  The forward pass and the gradients' logits take the same chunks and get the same bits: at the target d
+// is exp(z - lse) - 1, and of a nearly certain row nothing else is left.
 constexpr int kPairChunk = 16;               // blocks of 64 contraction elements per accumulator
 // The gradients, rounded to 16 bits in the end, take longer chunks: 512 additions leave a sum short by 2^-16 of itself at most, 1/32 of
 // fp16's half step; the 8192 of 131072 vocabulary entries left 1.3e-4.  The chunks of PAIR_STORE_LONG are summed in registers, and

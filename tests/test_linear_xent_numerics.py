@@ -116,3 +116,36 @@ def test_long_sums_of_the_gradients_are_not_short(api, m, v, h):
         short = float((got.double() * e[name]).sum() / (e[name] ** 2).sum()) - 1.0
         print(name, short, tol)
         assert abs(short) <= tol, (name, short, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("h", [1024, 4096, 16384])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_mean_and_rms_errors_over_a_long_hidden_size(api, h, dtype):
+    # A chunk of 64 additions leaves its part of a logit short by f <= 64 / 2 * 2^-24 of it, so a logit by f of itself, whatever h,
+    # and lse by f E[z] (the mean under the softmax), loss by f (E[z] - z_target).  With a single accumulator f would be 128 * 2^-24 at
+    # h = 4096, and never below half of that.  lse in fp32 is rounded by 2^-24 of itself at random; exp moves it by 2^-22 at
+    # most; single additions scatter by half a unit each, 2 sqrt(h / 16) 2^-24 max |z| over a row's logits.
+    m, v = 512, 8192
+    x, w, target, g = inputs(m, v, h, dtype, seed=h, skip=0.0)
+    loss, lse = api.linear_cross_entropy(x, w, target)
+    dx, dw = api.linear_cross_entropy_grad(x, w, target, lse, g)
+    e = exact(x, w, target, g)
+    z = x.double() @ w.double().t()
+    mean_z = ((z - e["lse"][:, None]).exp() * z).sum(1)
+    f = 32 * 2.0 ** -24
+    for name, got, part in (("lse", lse, mean_z), ("loss", loss, mean_z - (e["lse"] - e["loss"]))):
+        off = got.double() - e[name]
+        mean, rms = float(off.mean()), float(off.square().mean().sqrt())
+        # the means of the random parts: over m rows
+        noise = 2.0 ** -24 * float(e["lse"].abs().max()) + 2 * (h / 16) ** 0.5 * 2.0 ** -24 * float(z.abs().max()) / 8
+        tol = f * abs(float(part.mean())) + 2.0 ** -22 + 4 * noise / m ** 0.5
+        print(h, name, mean, rms, tol, float(part.mean()))
+        assert abs(mean) <= tol, (name, mean, tol)
+        assert rms <= f * float(part.square().mean().sqrt()) + 2.0 ** -22 + noise, (name, rms)
+    # d and the result are rounded once each: a relative error of u at most, u / sqrt(3) in the mean square if spread evenly
+    u = torch.finfo(dtype).eps / 2
+    for name, got in (("dx", dx), ("dw", dw)):
+        off = float((got.double() - e[name]).norm() / e[name].norm())
+        print(h, name, off / u)
+        assert off <= (2.0 / 3.0) ** 0.5 * u + 2e-5, (name, off)

@@ -142,15 +142,16 @@ int dx_split(int M, int H, int cols, bool with_dw) {
   return split;
 }
 
-Layout xent_layout(int M, int V, int H, bool copies, bool backward) {
+// Operands whose rows miss TMA's 16 bytes.
+struct Copies { bool x, w; };
+
+Layout xent_layout(int M, int V, int H, Copies copies, bool backward) {
   Layout l{};
   size_t at = 0;
   const auto take = [&](size_t bytes) { const size_t p = at; at += round_up(bytes, 256); return p; };
   l.hp = (int)round_up((size_t)H, 64);     // whole blocks: every box is a wide one
-  if (copies) {
-    l.x_copy = take((size_t)M * l.hp * 2);
-    l.w_copy = take((size_t)V * l.hp * 2);
-  }
+  if (copies.x) l.x_copy = take((size_t)M * l.hp * 2);
+  if (copies.w) l.w_copy = take((size_t)V * l.hp * 2);
   if (!backward) {
     const size_t tiles_n = ((size_t)V + kPairMaxBN - 1) / kPairMaxBN;
     l.partial = take(2 * tiles_n * M * sizeof(float2));
@@ -171,8 +172,22 @@ Layout xent_layout(int M, int V, int H, bool copies, bool backward) {
   return l;
 }
 
-bool needs_copies(const void* X, long long ldx, const void* W, long long ldw) {
-  return ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(W)) & 15) != 0 || ldx % 8 != 0 || ldw % 8 != 0;
+bool misses_16_bytes(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || ld % 8 != 0; }
+Copies needs_copies(const void* X, long long ldx, const void* W, long long ldw) { return {misses_16_bytes(X, ldx), misses_16_bytes(W, ldw)}; }
+
+// Puts the copies in place of the operands.  A copy's lines end in zeros, so that they are whole blocks.
+int make_copies(const Layout& l, Copies copies, uint8_t* ws, int M, int V, int H, const void** X, long long* ldx, int* inner_x, const void** W,
+                long long* ldw, int* inner_w, cudaStream_t stream) {
+  *inner_x = *inner_w = H;
+  if (copies.x) {
+    if (int rc = host_pad_rows16(*X, *ldx, ws + l.x_copy, M, H, l.hp, stream)) return rc;
+    *X = ws + l.x_copy; *ldx = *inner_x = l.hp;
+  }
+  if (copies.w) {
+    if (int rc = host_pad_rows16(*W, *ldw, ws + l.w_copy, V, H, l.hp, stream)) return rc;
+    *W = ws + l.w_copy; *ldw = *inner_w = l.hp;
+  }
+  return MP_OK;
 }
 
 int check_args(const char* op, int dtype, int M, int V, int H, const void* X, long long ldx, const void* W, long long ldw,
@@ -250,19 +265,15 @@ int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx,
   if (int rc = check_args(op, dtype, M, V, H, X, ldx, W, ldw, target, target_bytes)) return rc;
   if (M == 0) return MP_OK;
   if (loss == nullptr || lse == nullptr) return host_fail(MP_ERR_INVALID_ARG, "%s: null output", op);
-  const bool copies = needs_copies(X, ldx, W, ldw);
+  const Copies copies = needs_copies(X, ldx, W, ldw);
   const Layout l = xent_layout(M, V, H, copies, false);
   if (int rc = check_workspace(op, workspace, workspace_bytes, l.total)) return rc;
   HostDevice d;
   if (int rc = host_device(&d)) return rc;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  if (copies) {
-    if (int rc = host_pad_rows16(X, ldx, ws + l.x_copy, M, H, l.hp, stream)) return rc;
-    if (int rc = host_pad_rows16(W, ldw, ws + l.w_copy, V, H, l.hp, stream)) return rc;
-    X = ws + l.x_copy; W = ws + l.w_copy; ldx = ldw = l.hp;
-  }
-  const int inner = copies ? l.hp : H;               // a copy's lines end in zeros
+  int inner_x, inner_w;
+  if (int rc = make_copies(l, copies, ws, M, V, H, &X, &ldx, &inner_x, &W, &ldw, &inner_w, stream)) return rc;
   PairParams p{};
   p.num_problems = 1;
   shape_problem(&p.prob[0], M, V, H, kPairMaxBN, 0, 0, group_rows((long long)H * 2), 0);
@@ -272,8 +283,8 @@ int mp_linear_xent(int dtype, int M, int V, int H, const void* X, long long ldx,
   p.partial = reinterpret_cast<float2*>(ws + l.partial);
   p.target_logit = reinterpret_cast<float*>(ws + l.target_logit);
   PairMaps maps{};
-  if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, p.prob[0].a_rows, kStageBlocks, &p.prob[0].a_wide)) return rc;
-  if (int rc = operand_maps(&maps.b[0], W, inner, V, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
+  if (int rc = operand_maps(&maps.a[0], X, inner_x, M, ldx, p.prob[0].a_rows, kStageBlocks, &p.prob[0].a_wide)) return rc;
+  if (int rc = operand_maps(&maps.b[0], W, inner_w, V, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
   if (int rc = launch_pair<PAIR_LSE>(d, p, maps, stream)) return rc;
   return host_launch(xent_join_kernel, ceil_div(M, 32), 1024, 0, stream, p.partial, 2 * p.prob[0].tiles_n, M, p.target_logit, target, p.target64,
                 ignore_index, V, loss, lse);
@@ -294,17 +305,13 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
     return MP_OK;
   }
   if (lse == nullptr || grad_loss == nullptr) return host_fail(MP_ERR_INVALID_ARG, "%s: null pointer", op);
-  const bool copies = needs_copies(X, ldx, W, ldw);
+  const Copies copies = needs_copies(X, ldx, W, ldw);
   const Layout l = xent_layout(M, V, H, copies, true);
   if (int rc = check_workspace(op, workspace, workspace_bytes, l.total)) return rc;
   if (int rc = host_device(&d)) return rc;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  if (copies) {
-    if (int rc = host_pad_rows16(X, ldx, ws + l.x_copy, M, H, l.hp, stream)) return rc;
-    if (int rc = host_pad_rows16(W, ldw, ws + l.w_copy, V, H, l.hp, stream)) return rc;
-    X = ws + l.x_copy; W = ws + l.w_copy; ldx = ldw = l.hp;
-  }
-  const int inner = copies ? l.hp : H;               // a copy's lines end in zeros
+  int inner_x, inner_w;
+  if (int rc = make_copies(l, copies, ws, M, V, H, &X, &ldx, &inner_x, &W, &ldw, &inner_w, stream)) return rc;
   float* scale = reinterpret_cast<float*>(ws + l.scale);
   unsigned* counter = reinterpret_cast<unsigned*>(ws + l.scale) + 1;
   uint16_t* dl = reinterpret_cast<uint16_t*>(ws + l.dl);
@@ -327,8 +334,8 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       p.bf16 = bf16;
       p.target = target; p.target64 = target64; p.ignore_index = ignore_index;
       p.col0 = col0; p.lse = lse; p.grad_loss = grad_loss; p.vocab = V; p.scale_out = scale; p.next_unit = counter; p.dlogits = dl; p.ld_dl = l.ld_dl;
-      if (int rc = operand_maps(&maps.a[0], X, inner, M, ldx, p.prob[0].a_rows, kStageBlocks, &p.prob[0].a_wide)) return rc;
-      if (int rc = operand_maps(&maps.b[0], Wp, inner, cols, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
+      if (int rc = operand_maps(&maps.a[0], X, inner_x, M, ldx, p.prob[0].a_rows, kStageBlocks, &p.prob[0].a_wide)) return rc;
+      if (int rc = operand_maps(&maps.b[0], Wp, inner_w, cols, ldw, p.prob[0].bn / 2, kStageBlocks, &p.prob[0].b_wide)) return rc;
       if (int rc = launch_pair<PAIR_DLOGITS>(d, p, maps, stream)) return rc;
     }
     PairParams p{};
@@ -351,7 +358,7 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
         q.out16 = dX; q.ld_out = H;
       }
       if (int rc = operand_maps(&maps.a[n], dl, cols, M, l.ld_dl, q.a_rows, kStageBlocks, &q.a_wide)) return rc;
-      if (int rc = operand_maps(&maps.b[n], Wp, inner, cols, ldw, kStageBlocks * 64, q.bn / 2 / 64, &q.b_wide)) return rc;
+      if (int rc = operand_maps(&maps.b[n], Wp, inner_w, cols, ldw, kStageBlocks * 64, q.bn / 2 / 64, &q.b_wide)) return rc;
       p.total_tiles += q.tiles_m * q.tiles_n * q.split;
       ++n;
     }
@@ -361,7 +368,7 @@ int mp_linear_xent_grad(int dtype, int M, int V, int H, const void* X, long long
       q.out16 = reinterpret_cast<uint16_t*>(dW) + (long long)col0 * H;
       q.ld_out = H;
       if (int rc = operand_maps(&maps.a[n], dl, cols, M, l.ld_dl, kStageBlocks * 64, 128 / 64, &q.a_wide)) return rc;
-      if (int rc = operand_maps(&maps.b[n], X, inner, M, ldx, kStageBlocks * 64, q.bn / 2 / 64, &q.b_wide)) return rc;
+      if (int rc = operand_maps(&maps.b[n], X, inner_x, M, ldx, kStageBlocks * 64, q.bn / 2 / 64, &q.b_wide)) return rc;
       p.total_tiles += q.tiles_m * q.tiles_n;
       ++n;
     }

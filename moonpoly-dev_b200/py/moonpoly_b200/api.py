@@ -591,17 +591,16 @@ def _xent_checks(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor) -> None
 
 
 @functools.lru_cache(maxsize=4096)
-def _xent_workspace_bytes(code: int, M: int, V: int, H: int, aligned: bool, backward: int) -> int:
+def _xent_workspace_bytes(code: int, M: int, V: int, H: int, aligned_x: bool, aligned_w: bool, backward: int) -> int:
     # addresses and row strides that are 16-byte aligned or not: the library looks at nothing else
     need, ld = ctypes.c_size_t(), (H + 7) // 8 * 8
-    _check(lib().mp_linear_xent_workspace(code, M, V, H, 4096, ld, 4096 if aligned else 4098, ld, backward, ctypes.byref(need)))
+    _check(lib().mp_linear_xent_workspace(code, M, V, H, 4096 if aligned_x else 4098, ld, 4096 if aligned_w else 4098, ld, backward, ctypes.byref(need)))
     return need.value
 
 
 def _xent_workspace(code, M, V, H, x, ldx, w, ldw, backward) -> torch.Tensor:
     # a fresh tensor per call: calls on other streams and captured graphs never share it
-    aligned = (x.data_ptr() | w.data_ptr()) & 15 == 0 and (ldx | ldw) & 7 == 0
-    need = _xent_workspace_bytes(code, M, V, H, aligned, backward)
+    need = _xent_workspace_bytes(code, M, V, H, x.data_ptr() & 15 == 0 and ldx & 7 == 0, w.data_ptr() & 15 == 0 and ldw & 7 == 0, backward)
     return torch.empty((need,), dtype=torch.uint8, device=x.device)
 
 

@@ -30,6 +30,7 @@ from __future__ import annotations
 import os
 import re
 import threading
+import warnings
 from typing import Callable, Dict, Optional, Tuple
 
 import torch
@@ -182,36 +183,53 @@ def apply_moonpoly_linear(weight: torch.Tensor, x: torch.Tensor, bias: Optional[
     return out.view(*lead, n)
 
 
+def _linear_w4(x, qweight, scales, zeros, group_size, bias):
+    """(result, None), or (None, the reason why this path declines): an error that says so, the operator's own where it refused its
+    arguments.  Errors of the device and of memory go through."""
+    ops = _ops()
+    if not _flag("VLLM_USE_MOONPOLY_LINEAR", "0"):
+        return None, RuntimeError("VLLM_USE_MOONPOLY_LINEAR is not set")
+    if ops is None or not hasattr(ops, "linear_w4"):
+        why = "moonpoly_ops.linear_w4 is not registered"
+    elif x.device.type != "cuda" or qweight.device.type != "cuda" or x.dtype not in (torch.float16, torch.bfloat16):
+        why = "the 4-bit Linear serves fp16 and bf16 tensors on CUDA devices"
+    else:
+        try:
+            out = ops.linear_w4(x.reshape(-1, x.shape[-1]), qweight, scales, zeros, group_size, bias)
+        except ValueError as error:
+            STATS["declined"] += 1
+            return None, error
+        STATS["linear_w4"] += 1
+        return out.view(*x.shape[:-1], qweight.shape[0]), None
+    STATS["declined"] += 1
+    return None, RuntimeError(why)
+
+
 def apply_moonpoly_linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
                              group_size: int = 128, bias: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """x[..., K] @ W[N, K]^T (+ bias) for a layer whose weight is held in 4 bits with a scale (and zero point) per group, through
     `moonpoly_ops.linear_w4` (qweight from `moonpoly_ops.pack_w4`), or None when this path declines: the switch is off, the
-    tensors are not CUDA or not fp16 / bf16, or the operator refuses them.  Not in the reference, which serves unquantized
-    and INT8 layers only."""
-    if not _flag("VLLM_USE_MOONPOLY_LINEAR", "0"):
-        return None
-    ops = _ops()
-    if (ops is None or not hasattr(ops, "linear_w4") or x.device.type != "cuda" or qweight.device.type != "cuda"
-            or x.dtype not in (torch.float16, torch.bfloat16)):
-        STATS["declined"] += 1
-        return None
-    x2 = x.reshape(-1, x.shape[-1])
-    try:
-        out = ops.linear_w4(x2, qweight, scales, zeros, group_size, bias)
-    except Exception:
-        STATS["declined"] += 1
-        return None
-    STATS["linear_w4"] += 1
-    return out.view(*x.shape[:-1], qweight.shape[0])
+    tensors are not CUDA or not fp16 / bf16, or the operator refuses its arguments.  Errors of the device are raised.  Not in
+    the reference, which serves unquantized and INT8 layers only."""
+    return _linear_w4(x, qweight, scales, zeros, group_size, bias)[0]
 
 
 def apply(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor] = None,
           fallback: Optional[Callable] = None) -> torch.Tensor:
     """Drop-in body of UnquantizedLinearMethod.apply(layer, x, bias): the operators first, `fallback(layer, x, bias)`
     (default torch.nn.functional.linear on the layer's weight) when they decline.  A layer that carries `moonpoly_w4 =
-    (qweight, scales, zeros or None, group_size)` runs from its 4-bit weight."""
+    (qweight, scales, zeros or None, group_size)` runs from its 4-bit weight; where that is declined and no fallback is given the
+    reason is raised, as the layer's other weight, if it has one, need not hold the same numbers.  With a fallback, a refusal
+    of the operator is a RuntimeWarning."""
     w4 = getattr(layer, "moonpoly_w4", None)
-    out = apply_moonpoly_linear_w4(x, *w4, bias=bias) if w4 is not None else apply_moonpoly_linear(layer.weight, x, bias)
+    if w4 is not None:
+        out, why = _linear_w4(x, *w4, bias)
+        if out is None and fallback is None:
+            raise why
+        if isinstance(why, ValueError):
+            warnings.warn(f"the layer's 4-bit weight is not used: {why}", RuntimeWarning, stacklevel=2)
+    else:
+        out = apply_moonpoly_linear(layer.weight, x, bias)
     if out is not None:
         return out
     if fallback is not None:
@@ -236,7 +254,8 @@ def install(linear_module=None) -> bool:
     original = cls.apply
 
     def patched(self, layer, x, bias=None):
-        return apply(layer, x, bias, fallback=lambda la, xx, bb: original(self, la, xx, bb))
+        only_w4 = getattr(layer, "moonpoly_w4", None) is not None and getattr(layer, "weight", None) is None
+        return apply(layer, x, bias, fallback=None if only_w4 else lambda la, xx, bb: original(self, la, xx, bb))
     patched._moonpoly_installed = True
     cls.apply = patched
     return True

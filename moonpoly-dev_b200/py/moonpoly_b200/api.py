@@ -12,6 +12,7 @@ import contextlib
 import ctypes
 import functools
 import os
+import warnings
 from typing import Optional
 
 import torch
@@ -444,6 +445,13 @@ def _fits_int(op: str, extents: int) -> None:
         raise ValueError(f"{op}: an extent does not fit 32 bits")
 
 
+def _cuts_graph(op: str, *tensors: torch.Tensor) -> None:
+    """Says so where a result that carries no graph leaves a gradient behind."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        warnings.warn(f"{op}: the result carries no autograd graph; call it in the forward of a torch.autograd.Function whose backward "
+                      f"calls {op}_grad{'_input' if op == 'linear_w4' else ''}, or under torch.no_grad()", RuntimeWarning, stacklevel=3)
+
+
 _W4_CODES = {torch.float16: MP_FP16, torch.bfloat16: MP_BF16}
 
 
@@ -503,10 +511,13 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zero
     """Y[M,N] = x[M,K] @ W[N,K]^T (+ bias[N]) with W[n,k] = (q[n,k] - zero[n, k // group_size]) * scale[n, k // group_size],
     qweight from `pack_w4`, scales [N, ceil(K / group_size)] in the type of x (fp16 or bf16), zeros the same shape in uint8
     (values 0..63; None: 8 everywhere).  group_size is a power of two of at least 32, or -1 for one group per row.  The
-    bias is added before the only rounding of the result."""
+    bias is added before the only rounding of the result.  The result carries no autograd graph (a RuntimeWarning where that loses
+    a gradient): `linear_w4_grad_input` is for the backward of a torch.autograd.Function."""
     K = x.shape[1] if x.dim() == 2 else 0
     code, N, group_size, qweight, scales, zeros = _w4_checks("linear_w4", x, qweight, scales, zeros, group_size, False, K)
     M = x.shape[0]
+    if x.requires_grad:
+        _cuts_graph("linear_w4", x)
     if bias is not None:
         if bias.dtype != x.dtype or bias.numel() != N or bias.device != x.device:
             raise ValueError("bias must be a CUDA tensor of N elements in the input dtype")
@@ -608,9 +619,11 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor,
     """(loss [M], lse [M]) in fp32 of the logits z = x[M,H] @ w[V,H]^T, which are never held: lse = logsumexp(z) per row,
     loss = lse - z[target], 0 where target == ignore_index, NaN where target is any other value outside [0, V).
     x and w fp16 or bf16.  Take the mean (or any other weighting) of `loss` outside; `linear_cross_entropy_grad` gives
-    the gradients from `lse` and the gradient with respect to `loss`."""
+    the gradients from `lse` and the gradient with respect to `loss`.  The results carry no autograd graph (a RuntimeWarning where
+    that loses a gradient): both functions are for a torch.autograd.Function."""
     _xent_checks(x, w, target)
     code = _dtype16(x, "linear_cross_entropy")
+    _cuts_graph("linear_cross_entropy", x, w)
     (M, H), V = x.shape, w.shape[0]
     with _device_of(x):
         x, ldx = _rows(x)

@@ -92,14 +92,19 @@ Plan w4_plan(int T, int N, int K, int group_size, bool grad, bool copy_tokens) {
 
 constexpr int kMaxExtent = 1 << 28;
 
-int check_args(const char* op, int dtype, int M, int N, int K, const void* x, long long ldx, int width, const uint32_t* packed,
-               const void* scales, int group_size) {
-  if (dtype != MP_FP16 && dtype != MP_BF16) return host_fail(MP_ERR_INVALID_ARG, "%s: dtype must be MP_FP16 or MP_BF16", op);
+int check_shape(const char* op, int M, int N, int K, int group_size) {
   if (M < 0 || N <= 0 || K <= 0 || M > kMaxExtent || N > kMaxExtent || K > kMaxExtent)
     return host_fail(MP_ERR_INVALID_ARG, "%s: needs M >= 0, N > 0, K > 0, none above 2^28 (got %d, %d, %d)", op, M, N, K);
   if (K % 32 != 0) return host_fail(MP_ERR_UNALIGNED_K, "%s: K = %d is not a multiple of 32", op, K);
   if (group_size < 32 || (group_size & (group_size - 1)) != 0)
     return host_fail(MP_ERR_INVALID_ARG, "%s: group_size %d is not a power of two of at least 32", op, group_size);
+  return MP_OK;
+}
+
+int check_args(const char* op, int dtype, int M, int N, int K, const void* x, long long ldx, int width, const uint32_t* packed,
+               const void* scales, int group_size) {
+  if (dtype != MP_FP16 && dtype != MP_BF16) return host_fail(MP_ERR_INVALID_ARG, "%s: dtype must be MP_FP16 or MP_BF16", op);
+  if (int rc = check_shape(op, M, N, K, group_size)) return rc;
   if (ldx < width) return host_fail(MP_ERR_INVALID_ARG, "%s: row stride %lld below the row's %d elements", op, ldx, width);
   if (packed == nullptr || scales == nullptr || (M > 0 && x == nullptr)) return host_fail(MP_ERR_INVALID_ARG, "%s: null pointer", op);
   if (reinterpret_cast<uintptr_t>(packed) & 15) return host_fail(MP_ERR_INVALID_ARG, "%s: the packed weight must be 16-byte aligned", op);
@@ -272,15 +277,15 @@ int mp_w4_pack(int N, int K, const uint8_t* q, long long ldq, uint32_t* packed, 
 }
 
 int mp_linear_w4_workspace(int M, int N, int K, int group_size, const void* X, long long ldx, int grad_input, size_t* bytes) {
-  if (bytes == nullptr || M < 0 || N <= 0 || K <= 0 || M > kMaxExtent || N > kMaxExtent || K > kMaxExtent || group_size <= 0)
-    return host_fail(MP_ERR_INVALID_ARG, "mp_linear_w4_workspace: needs M >= 0, N > 0, K > 0, none above 2^28, group_size > 0 and a result pointer");
+  if (bytes == nullptr) return host_fail(MP_ERR_INVALID_ARG, "mp_linear_w4_workspace: null pointer");
+  if (int rc = check_shape("mp_linear_w4_workspace", M, N, K, group_size)) return rc;
   *bytes = M == 0 ? 0 : w4_plan(M, N, K, group_size, grad_input != 0, !tokens_aligned(X, ldx)).total;
   return MP_OK;
 }
 
 int mp_debug_w4_launch(int M, int N, int K, int group_size, int grad_input, int out[8]) {
-  if (out == nullptr || M < 1 || N < 1 || K < 1 || M > kMaxExtent || N > kMaxExtent || K > kMaxExtent || group_size < 32)
-    return host_fail(MP_ERR_INVALID_ARG, "mp_debug_w4_launch: positive sizes up to 2^28, group_size of at least 32");
+  if (out == nullptr || M == 0) return host_fail(MP_ERR_INVALID_ARG, "mp_debug_w4_launch: needs M > 0 and a result pointer");
+  if (int rc = check_shape("mp_debug_w4_launch", M, N, K, group_size)) return rc;
   const Plan l = w4_plan(M, N, K, group_size, grad_input != 0, false);
   const int v[8] = {l.stream, l.bn, l.tiles_m * l.tiles_n * l.split, l.split, l.steps, l.steps_per_split, l.stages, l.raw_slots};
   std::copy(v, v + 8, out);

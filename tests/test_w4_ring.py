@@ -79,6 +79,23 @@ def test_the_aid_refuses_bad_arguments(api):
         assert aid(*args) != 0
 
 
+def test_the_workspace_query_refuses_what_the_call_refuses(api):
+    # a group size near 2^31 overflowed the number of groups, and sizes came back for calls that are refused
+    n, p, z = ctypes.c_size_t(7), ctypes.c_void_p(4096), ctypes.c_void_p(0)
+    L = api.lib()
+    for group in (0, -1, 16, 33, 48, 2 ** 31 - 1, 2 ** 31 - 64):
+        call = L.mp_linear_w4(api.MP_FP16, 100, 64, 4096, p, 4096, p, p, z, group, z, p, p, 1 << 30, z)
+        assert call == 1 and L.mp_linear_w4_workspace(100, 64, 4096, group, p, 4096, 0, ctypes.byref(n)) == call, group
+        assert L.mp_debug_w4_launch(100, 64, 4096, group, 0, (ctypes.c_int * 8)()) == call
+    assert L.mp_linear_w4_workspace(100, 64, 4080, 32, p, 4080, 0, ctypes.byref(n)) == 3 and n.value == 7
+    # one group per row: any size of at least K asks for the same
+    sizes = set()
+    for shift in range(12, 31):
+        assert L.mp_linear_w4_workspace(300, 64, 4096, 1 << shift, p, 4096, 0, ctypes.byref(n)) == 0
+        sizes.add(n.value)
+    assert len(sizes) == 1
+
+
 # ------------------------------------------------------------------------------------ many units per pair of CTAs (GPU)
 MANY = [  # tokens, N, K, group: even and odd steps of 128 along the contraction, tiles of 160 to 256 tokens and of fewer
     (40, 20000, 256, 32), (40, 20000, 384, 64), (96, 20000, 128, 32), (120, 20000, 384, 128), (150, 19000, 640, 128), (150, 20000, 512, 32), (180, 28672, 3456, 128), (192, 20000, 128, 64),

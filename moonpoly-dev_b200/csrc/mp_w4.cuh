@@ -10,7 +10,8 @@
 // subtraction (or a multiply-add with 1 / 16) gives q - zero exactly; for bf16, 0x4300 | q is 128 + q.
 //
 // Two kernels.  Up to 16 tokens: w4_stream_kernel, warp-level MMAs on q - zero, exact in 16 bits, with the scale applied to
-// 32-bit sums -- bound by reading the weight.  More tokens, and the gradient of the input: w4_mma_kernel, tcgen05 tiles whose
+// 32-bit sums; its floor is reading the weight, of which it takes 2.2 times at 4 x 28672 x 4096 (21.8 us; nothing is saturated:
+// latency, start and join).  More tokens, and the gradient of the input: w4_mma_kernel, tcgen05 tiles whose
 // weight operand is unpacked into shared memory by sixteen warps while the tensor cores work on earlier stages.
 #pragma once
 #include <type_traits>

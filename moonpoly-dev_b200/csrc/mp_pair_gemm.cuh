@@ -144,7 +144,8 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
 // Registers per thread of a warpgroup from here on.  The launch has 384 x 168; 128 x 88 + 256 x 208 is just that.
 __device__ __forceinline__ void regs_fewer_88() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 __device__ __forceinline__ void regs_more_208() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
-// mbar_wait by a whole warp, with one answer for it.
+// mbar_wait by a whole warp, with one answer for it: where a wait gives up, no lane may go on to the warp's next aligned instruction
+// or __syncwarp without the others.
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int* status, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code)) != 0;
 }
@@ -664,7 +665,7 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         for (int j = 0; j < 128; ++j) z[j] = 0.0f;
         for (int k0 = u.kb0; ok && k0 < u.kb1; k0 += kChunk, ++ui) {
           const uint32_t buf = ui & 1u, use = ui >> 1;
-          if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
+          if (!wait_all(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
           tc_fence_after();
           pair_add_chunk(z, t_half + buf * (uint32_t)kPairMaxBN);
           tc_fence_before();
@@ -677,7 +678,7 @@ pair_gemm_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
         else pair_epilogue_store<true>(p, q, 0u, z, row, c_begin, ncols, u.slice, scale, stage);
       } else {
         const uint32_t buf = ui & 1u, use = ui >> 1;
-        if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
+        if (!wait_all(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
         tc_fence_after();
         pair_epilogue_store<false>(p, q, t_half + buf * (uint32_t)kPairMaxBN, z, row, c_begin, ncols, u.slice, scale, stage);
         tc_fence_before();

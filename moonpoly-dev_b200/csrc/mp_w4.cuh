@@ -588,7 +588,7 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
       const int mine = advance(nxt);
       int theirs = 0;
       if (nxt.unit < units) theirs = advance(nxt);
-      if (!mbar_wait(rfull_bar(rs), rph, status, MP_DEV_TIMEOUT_MMA_FULL)) break;
+      if (!wait_all(rfull_bar(rs), rph, status, MP_DEV_TIMEOUT_MMA_FULL)) break;
       const uint32_t slot = (uint32_t)rs * kW4RawBytes;
       int sh = s;
       uint32_t phh = ph;
@@ -609,7 +609,7 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
           __syncwarp();
           if (lane == 0) mbar_arrive(rempty_bar(rs));
         }
-        if (!mbar_wait(empty_bar(sh), phh ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
+        if (!wait_all(empty_bar(sh), phh ^ 1u, status, MP_DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
         const uint32_t ev = even_at + (uint32_t)sh * (uint32_t)p.stage_bytes, od = odd_at + (uint32_t)sh * (uint32_t)p.stage_bytes;
         // the weight in the operand type: one rounding of the exact product (q - zero) * scale
         st_smem_v4<0>(ev, w4_weights<BF16>(q0.x, magic, zero[0][0], scale[0][0]));
@@ -639,7 +639,7 @@ w4_mma_kernel(const __grid_constant__ OperandMaps tokens, const __grid_constant_
       const int row = u.tm * kPairRows + (int)rank * 128 + quad * 32 + lane;
       const bool live = row < p.rows;
       const float bias = live && p.bias != nullptr ? from16<BF16>(p.bias[row]) : 0.0f;
-      if (!mbar_wait(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
+      if (!wait_all(tfull_bar((int)buf), use & 1u, status, MP_DEV_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
       const uint32_t t_addr = tmem_base + buf * (uint32_t)kPairMaxBN + ((uint32_t)(quad * 32) << 16);
       const int tok0 = u.tn * p.bn, ntok = min(p.bn, p.T - tok0);
